@@ -481,6 +481,104 @@ int irodori_op_mx_quantize(const float* x, int rows, int dim, uint8_t* q, uint8_
 int irodori_op_gemm_fp8(const uint8_t* a, const uint8_t* a_scale, const uint8_t* w, const float* w_scale,
                         int M, int N, int K, float* c, void* stream);
 
+/* ---- described operators (device pointers on the current device; stream may be NULL) ----------
+ * No counterparts in the reference, whose model fuses these into its blocks: the parts of a
+ * cross-attention half block for callers with a block of their own, beside the norms above.  A call's
+ * shape is a description that the caller fills once and keeps; a call enqueues on `stream`, which
+ * must belong to the current device (else IRODORI_ERR_INVALID_ARG), without waiting, allocates
+ * nothing, keeps nothing between calls and may be captured from the first call on.  Tensors are in the
+ * description's dtype (IRODORI_DTYPE_F32, _BF16 or _F16) and need the alignment of an element;
+ * strides count elements.  An output may not overlap an input except where said. */
+
+/* Rotary positions: the pairs of a head turned by position * frequency.
+ *   (a, b) -> amplitude * (a cos - b sin, a sin + b cos)
+ * Pair p of the first rot_dim dimensions is (2p, 2p + 1) (INTERLEAVED) or (p, p + rot_dim / 2)
+ * (HALVES), its frequency theta^(-2p / rot_dim) radians per position, with
+ *   LINEAR    divided by factor;
+ *   NTK       theta times factor^(rot_dim / (rot_dim - 2)) instead of theta;
+ *   BY_PARTS  kept where the pair turns beta_fast times or more over trained_len positions, divided
+ *             by factor where beta_slow times or less, in proportion between.
+ * Angles are formed in float64, whatever the position.  Dimensions past rot_dim and heads past the
+ * rotating ones are copied.  inverse: the transposed map (turned back), which is the gradient's. */
+#define IRODORI_ROPE_INTERLEAVED 0
+#define IRODORI_ROPE_HALVES 1
+#define IRODORI_ROPE_UNSCALED 0
+#define IRODORI_ROPE_LINEAR 1
+#define IRODORI_ROPE_NTK 2
+#define IRODORI_ROPE_BY_PARTS 3
+typedef struct irodori_rope_desc {
+    int32_t dtype;
+    int32_t batch, seq;
+    int32_t head_dim;    /* even, <= 1024 */
+    int32_t rot_dim;     /* even, 2 .. min(head_dim, 512) */
+    int32_t q_heads, k_heads;          /* either may be 0; at most 16384 */
+    int32_t q_rot_heads, k_rot_heads;  /* the first heads of each, which rotate */
+    int32_t layout, scaling;
+    int32_t inverse;     /* nonzero: the transposed map */
+    int32_t first_pos;   /* without `positions`, token s sits at first_pos + s */
+    int32_t reserved;
+    double theta, factor, trained_len, beta_fast, beta_slow;
+    double amplitude;    /* 1 for a plain rotation */
+    int64_t q_strides[3], q_out_strides[3]; /* batch, token, head; a head's dimensions are contiguous */
+    int64_t k_strides[3], k_out_strides[3];
+} irodori_rope_desc;
+/* positions [batch, seq] or NULL; lengths [batch] or NULL (tokens at or past a row's length are left
+ * as they were in the outputs).  q_out may be q, and k_out k, with equal strides. */
+int irodori_op_rope(const irodori_rope_desc* desc, const void* q, void* q_out, const void* k, void* k_out,
+                    const int32_t* positions, const int32_t* lengths, void* stream);
+
+/* Linear layer: y[m, n] = residual[m, n] + gate[m / gate_rows, n] * act(sum_k x[m, k] w[n, k] + bias[n]),
+ * the sum and everything after it in f32, rounded once to out_dtype (dtype or F32).  w is [n, k] (each
+ * output's weights contiguous; a Burn [d_in, d_out] weight transposed once at load).  bias [n] and
+ * gate [ceil(m / gate_rows), n] are f32; bias, gate and residual (in out_dtype) may be NULL, a gate and a
+ * positive gate_rows go together.  y may be the residual, with ldy == ldr. */
+#define IRODORI_ACT_NONE 0
+#define IRODORI_ACT_RELU 1
+#define IRODORI_ACT_SILU 2
+#define IRODORI_ACT_SIGMOID 3
+#define IRODORI_ACT_TANH 4
+#define IRODORI_ACT_GELU 5      /* x / 2 (1 + erf(x / sqrt 2)) */
+#define IRODORI_ACT_GELU_TANH 6 /* its tanh approximation */
+typedef struct irodori_linear_desc {
+    int32_t dtype, out_dtype;
+    int32_t m, n, k;
+    int32_t activation;
+    int32_t gate_rows;           /* rows that share a row of the gate; 0 without one */
+    int32_t reserved;
+    int64_t ldx, ldw, ldy, ldr;  /* between rows */
+} irodori_linear_desc;
+/* Bytes of device workspace that a call of this description takes (often 0).  Its contents need not be
+ * kept between calls; calls that may run at the same time need one each. */
+int irodori_op_linear_workspace(const irodori_linear_desc* desc, uint64_t* bytes);
+int irodori_op_linear(const irodori_linear_desc* desc, const void* x, const void* w, const float* bias,
+                      const float* gate, const void* residual, void* y, void* workspace,
+                      uint64_t workspace_bytes, void* stream);
+
+/* Cross attention: queries [batch, seq_q, heads, head_dim] over an encoder's keys and values
+ * [batch, seq_kv, kv_heads, head_dim] (strides: batch, token, head; head_dim 64 or 128, contiguous):
+ *   out[b, s, h] = sum_t softmax_t(scale q[b, s, h] . k[b, t, h / (heads / kv_heads)]) v[b, t, ...]
+ * over the keys t < kv_len[b] whose mask byte [b * mask_stride + t] is nonzero (kv_len and mask may be
+ * NULL: all).  What masked keys and values hold, NaN included, never counts; a row without a key gives 0.
+ * Query tokens at or past q_len[b] (NULL: none) are left as they were in out.  Lengths are read on the
+ * device and clamped to the shape.  Scores, softmax and sums are f32; in the 16-bit forms the
+ * probabilities are rounded to dtype for the matrix cores.  seq_q may be 1 (a new token): few rows over
+ * many keys are split over the keys and joined in f32, through the workspace. */
+typedef struct irodori_cross_attention_desc {
+    int32_t dtype;
+    int32_t batch, seq_q, seq_kv;
+    int32_t heads, kv_heads;     /* heads a multiple of kv_heads */
+    int32_t head_dim;
+    float scale;
+    int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+    int64_t mask_stride;         /* between rows of the mask */
+} irodori_cross_attention_desc;
+/* As irodori_op_linear_workspace. */
+int irodori_op_cross_attention_workspace(const irodori_cross_attention_desc* desc, uint64_t* bytes);
+int irodori_op_cross_attention(const irodori_cross_attention_desc* desc, const void* q, const void* k,
+                               const void* v, const uint8_t* mask, const int32_t* q_len,
+                               const int32_t* kv_len, void* out, void* workspace,
+                               uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,492 @@
+// Cross attention on token-major operands as a caller has them (irodori_op_cross_attention): queries
+// of one length, an encoder's keys and values of another, heads sharing a key head in groups, lengths
+// and a key mask per batch row.
+//
+// Per key tile and wavefront (32 rows; a row is one token of one head of the group, so a group's
+// heads share every tile that is loaded), on the 32x32 matrix-core shapes:
+//   S^T = K Q^T      lane l holds row l % 32 and keys 8a + 4 (l / 32) + c of every 32.
+//   softmax          p = exp2(s c - m) in f32, c = scale log2(e).  The reference m is lazy: a row's
+//                    first score above -inf sets it, and it moves when a lane's sum of p over a tile
+//                    shows a p beyond the slack.
+//   O^T += V^T P^T   P^T is the S^T accumulator, rounded to the operand type in the 16-bit forms (the
+//                    matrix core's operand; its rounding averages out over the keys as V's own does);
+//                    V^T comes from the row-major tile, 16-bit by the transposing LDS read.
+// A tile that the mask empties is never loaded; in a tile that it thins, the masked scores are -inf and
+// the masked values zero, whatever their memory holds.
+#include <type_traits>
+
+#include "attn_util.hpp"
+#include "common.hpp"
+#include "cross_attention.hpp"
+
+namespace irodori {
+
+namespace {
+
+template <typename T>
+constexpr int kTile = sizeof(T) == 2 ? 64 : 32;  // keys
+// Lazy-reference slack: 2^16, and 2^15 for f16, whose largest finite value is below 2^16.
+template <typename T>
+constexpr float kSumMax = std::is_same<T, f16>::value ? 32768.f : 65536.f;
+
+// 16-byte chunk c of tile row r (ROWB bytes): K is read 32 rows at one chunk, 16-bit V 8 rows at two
+// neighbouring chunks, f32 V one row at a time.
+template <int ROWB>
+__device__ __forceinline__ int kswz(int r, int c) {
+    return ROWB == 128 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
+}
+template <typename T, int ROWB>
+__device__ __forceinline__ int vswz(int r, int c) {
+    if (sizeof(T) == 4) return c;
+    return ROWB == 128 ? c ^ (2 * ((r >> 1) & 3)) : c ^ (2 * (r & 7));
+}
+
+// The 8 reduction elements of a lane.
+template <typename T>
+struct Op8 {
+    typedef typename Vec8<T>::type type;
+};
+template <>
+struct Op8<float> {
+    typedef f32x8 type;
+};
+template <typename T>
+__device__ __forceinline__ f32x16 mma(typename Op8<T>::type a, typename Op8<T>::type b, f32x16 c) {
+    if constexpr (sizeof(T) == 2) {
+        return mma32x16(a, b, c);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+}
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+// V^T operand, keys 16 g + 8 j + 4 (lane / 32) + 0..3 (j = 0, 1) of dim 32 db + lane % 32.
+template <typename T, int DH>
+__device__ __forceinline__ typename Op8<T>::type read_v(const unsigned char* tile, int g, int db, int lane) {
+    constexpr int ROWB = DH * (int)sizeof(T);
+    if constexpr (sizeof(T) == 2) {
+        const int i = lane & 15, grp = lane >> 4;
+        const int col = 32 * db + 16 * (grp & 1) + 4 * (i & 3);
+        auto half = [&](int base) {
+            const int row = base + 4 * (grp >> 1) + (i >> 2);
+            const unsigned char* p = tile + row * ROWB + (vswz<T, ROWB>(row, col >> 3) << 4) + (col & 7) * 2;
+            return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)p);
+        };
+        struct { i16x4 a, b; } f = {half(16 * g), half(16 * g + 8)};
+        return __builtin_bit_cast(typename Op8<T>::type, f);
+    } else {
+        f32x8 f;
+        const float* p = reinterpret_cast<const float*>(tile) + (16 * g + 4 * (lane >> 5)) * DH + 32 * db + (lane & 31);
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = p[(8 * (e >> 2) + (e & 3)) * DH];
+        return f;
+    }
+}
+
+template <typename T, int DH>
+__device__ __forceinline__ f32x16 score_block(const unsigned char* kt, int kb, int fr, int fh,
+                                              const typename Op8<T>::type (&qf)[DH / 16]) {
+    constexpr int ROWB = DH * (int)sizeof(T);
+    typedef typename Op8<T>::type V8;
+    const int r = 32 * kb + fr;
+    f32x16 s;
+#pragma unroll
+    for (int e = 0; e < 16; e++) s[e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DH / 16; ks++) {
+        V8 kf;
+        if constexpr (sizeof(T) == 2) {
+            kf = *reinterpret_cast<const V8*>(kt + r * ROWB + (kswz<ROWB>(r, 2 * ks + fh) << 4));
+        } else {
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(kt + r * ROWB + (kswz<ROWB>(r, 4 * ks + 2 * fh) << 4));
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(kt + r * ROWB + (kswz<ROWB>(r, 4 * ks + 2 * fh + 1) << 4));
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                kf[e] = lo[e];
+                kf[4 + e] = hi[e];
+            }
+        }
+        s = mma<T>(kf, qf[ks], s);
+    }
+    return s;
+}
+
+// Validity of the KT keys from t0 on, of which n (<= KT) exist.
+template <int KT>
+__device__ __forceinline__ unsigned long long mask_bits(const uint8_t* m, int n) {
+    typedef unsigned u32x4_b __attribute__((ext_vector_type(4), aligned(1)));
+    unsigned long long bits = 0;
+    if (n >= KT) {
+#pragma unroll
+        for (int i = 0; i < KT / 16; i++) {
+            const u32x4_b w = *reinterpret_cast<const u32x4_b*>(m + 16 * i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const unsigned nz = ((((w[j] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[j]) >> 7) & 0x01010101u;
+                bits |= (unsigned long long)((nz * 0x01020408u) >> 24 & 0xfu) << (16 * i + 4 * j);
+            }
+        }
+    } else {
+        for (int i = 0; i < n; i++) bits |= (unsigned long long)(m[i] != 0) << i;
+    }
+    return bits;
+}
+
+// Tiles t0 .. te - 1, at most 64 of them, that hold a valid key, in order: lane i has the i-th one's
+// index and its keys' bits.
+struct TileWord {
+    int t, lo, hi;  // per lane
+    int n;          // the same in all
+};
+template <int KT>
+__device__ __forceinline__ TileWord tile_word(const uint8_t* mask, int len, int t0, int te, int lane) {
+    const int t = t0 + lane;
+    unsigned long long bits = 0ull;
+    if (t < te) {
+        const int n = len - t * KT < KT ? len - t * KT : KT;
+        if (mask) bits = mask_bits<KT>(mask + (int64_t)t * KT, n);
+        else bits = n == 64 ? ~0ull : (1ull << n) - 1ull;
+    }
+    const bool on = bits != 0ull;
+    const unsigned long long act = __ballot(on);
+    const int cnt = __popcll(act), below = __popcll(act & ((1ull << lane) - 1ull));
+    const int dest = 4 * (on ? below : cnt + (lane - below));
+    TileWord tw;
+    tw.t = __builtin_amdgcn_ds_permute(dest, t);
+    tw.lo = __builtin_amdgcn_ds_permute(dest, (int)(unsigned)bits);
+    tw.hi = __builtin_amdgcn_ds_permute(dest, (int)(unsigned)(bits >> 32));
+    tw.n = cnt;
+    return tw;
+}
+
+// A workgroup: QW wavefronts of 32 rows times KW groups that take the tiles in turn and are joined
+// through LDS.  Two ring slots of KW K and V tiles, moved HBM -> LDS by buffer_load_dwordx4 ... lds;
+// UNAL: through registers, for operands off a dword boundary or with rows too far apart for a window.
+template <typename T, int DH, int QW, int KW, bool UNAL>
+__global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(1, 2))) void cross_kernel(CrossArgs a,
+                                                                                                        int row_blocks) {
+    typedef typename Op8<T>::type V8;
+    constexpr int NW = QW * KW, KT = kTile<T>, KB = KT / 32, ROWB = DH * (int)sizeof(T), TILE = KT * ROWB;
+    constexpr int RPI = 1024 / ROWB, NI = KT / RPI, LPW = KW * NI / NW, DB = DH / 32, CH = ROWB / 16;
+    constexpr int RING = 4 * KW * TILE, PER = (DB * 16 + 2) * 64;
+    static_assert(LPW * NW == KW * NI, "a stage's loads split over the waves");
+    static_assert((KW - 1) * QW * PER * 4 <= RING, "the groups' results fit the rings");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[RING];
+    unsigned char* kring = smem;                  // [2][KW][TILE]
+    unsigned char* vring = smem + 2 * KW * TILE;  // [2][KW][TILE]
+
+    const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int qw = wave % QW, kw = wave / QW;
+    int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int rb = id % row_blocks;
+    id /= row_blocks;
+    const int sp = id % a.splits;
+    id /= a.splits;
+    const int hk = id % a.kv_heads, b = id / a.kv_heads;
+    int rows = a.rows;
+    if (a.q_len) {
+        const int n = a.q_len[b];
+        rows = n <= 0 ? 0 : (n < a.seq_q ? n : a.seq_q) * a.group;
+    }
+    const int row0 = rb * 32 * QW;
+    if (row0 >= rows) return;  // rows past the length stay as they were
+    int len = a.seq_kv;
+    if (a.kv_len) {
+        const int n = a.kv_len[b];
+        len = n < 0 ? 0 : n < len ? n : len;
+    }
+    const int nt = (len + KT - 1) / KT;
+    const int t_begin = (int)((int64_t)nt * sp / a.splits), t_end = (int)((int64_t)nt * (sp + 1) / a.splits);
+    const T* Kb = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
+    const T* Vb = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
+    const uint8_t* mb = a.mask ? a.mask + b * a.mask_stride : nullptr;
+    // c = 0 would turn a masked key's -inf into NaN; a tiny c gives the same exp2(0).
+    float c = a.scale * 1.4426950408889634f;
+    c = c == 0.f ? 1e-38f : c;
+    const float s_masked = c > 0.f ? -INFINITY : INFINITY;
+
+    const int row = row0 + 32 * qw + fr, rc = row < rows ? row : rows - 1;
+    const int tok = rc / a.group, head = hk * a.group + (rc - tok * a.group);
+    V8 qf[DH / 16];
+    {
+        typedef T Q8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+        const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + tok * a.qs[1] + head * a.qs[2] + 8 * fh;
+#pragma unroll
+        for (int ks = 0; ks < DH / 16; ks++) qf[ks] = __builtin_bit_cast(V8, *reinterpret_cast<const Q8*>(qp + 16 * ks));
+    }
+    f32x16 o[DB];
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[db][e] = 0.f;
+    float m = 0.f, l_run = 0.f;
+    bool unset = true;  // m is no reference yet: no tile so far, or only scores of -inf
+
+    // Load instruction ii of this wave in a stage: gi = wave LPW + ii -> group gi / NI, rows RPI
+    // (gi % NI) ..; lane -> row lane / CH, physical chunk lane % CH.
+    unsigned voK[LPW], voV[LPW];
+#pragma unroll
+    for (int ii = 0; ii < LPW; ii++) {
+        const int r = ((wave * LPW + ii) % NI) * RPI + lane / CH;
+        voK[ii] = (unsigned)(r * (a.ks[1] * (int)sizeof(T))) + (kswz<ROWB>(r, lane % CH) << 4);
+        voV[ii] = (unsigned)(r * (a.vs[1] * (int)sizeof(T))) + (vswz<T, ROWB>(r, lane % CH) << 4);
+    }
+
+    for (int t0 = t_begin; t0 < t_end; t0 += 64) {
+        const TileWord tw = tile_word<KT>(mb, len, t0, t_end, lane);
+        const int nact = tw.n, niter = (nact + KW - 1) / KW;
+        if (niter == 0) continue;  // the same for every wave
+        if (t0 > t_begin) {        // the rings are still being read
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            raw_barrier();
+        }
+        // The K and V tiles of step j into their ring slot.  Entries past the last are clamped to it,
+        // so every wave issues the same loads.
+        auto issue = [&](int j) {
+            const int slot = j & 1;
+#pragma unroll
+            for (int ii = 0; ii < LPW; ii++) {
+                const int gi = wave * LPW + ii, g = gi / NI;
+                int li = j * KW + g;
+                li = li < nact ? li : nact - 1;
+                const int t = __builtin_amdgcn_readlane(tw.t, li);
+                const int left = len - t * KT, n = left < KT ? left : KT;  // rows of the tile
+                const T* ksrc = Kb + (int64_t)t * KT * a.ks[1];
+                const T* vsrc = Vb + (int64_t)t * KT * a.vs[1];
+                unsigned char* kd = kring + (slot * KW + g) * TILE + (gi % NI) * 1024;
+                unsigned char* vd = vring + (slot * KW + g) * TILE + (gi % NI) * 1024;
+                if constexpr (UNAL) {
+                    typedef T E16 __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+                    const int r = (gi % NI) * RPI + lane / CH;
+                    u32x4 kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
+                    if (r < n) {
+                        const int per = 16 / (int)sizeof(T);
+                        kx = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(ksrc + r * a.ks[1] + kswz<ROWB>(r, lane % CH) * per));
+                        vx = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(vsrc + r * a.vs[1] + vswz<T, ROWB>(r, lane % CH) * per));
+                    }
+                    *reinterpret_cast<u32x4*>(kd + 16 * lane) = kx;
+                    *reinterpret_cast<u32x4*>(vd + 16 * lane) = vx;
+                } else {
+                    // Rows past the last key read as zero.
+                    buf_load_lds16(make_rsrc(ksrc, (unsigned)((n - 1) * a.ks[1] * (int)sizeof(T)) + ROWB), voK[ii], kd);
+                    buf_load_lds16(make_rsrc(vsrc, (unsigned)((n - 1) * a.vs[1] * (int)sizeof(T)) + ROWB), voV[ii], vd);
+                }
+            }
+        };
+        issue(0);
+        for (int j = 0; j < niter; j++) {
+            // This wave's loads of step j have landed, and its reads of the slot refilled next are done.
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            raw_barrier();
+            if (j + 1 < niter) issue(j + 1);
+            const int li = j * KW + kw;
+            if (li >= nact) continue;  // this group has no tile in the last step
+            const unsigned char* kt = kring + ((j & 1) * KW + kw) * TILE;
+            const unsigned char* vt = vring + ((j & 1) * KW + kw) * TILE;
+            f32x16 s[KB];
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) s[kb] = score_block<T, DH>(kt, kb, fr, fh, qf);
+            const unsigned word[2] = {(unsigned)__builtin_amdgcn_readlane(tw.lo, li),
+                                      (unsigned)__builtin_amdgcn_readlane(tw.hi, li)};
+            const bool thin = KB == 2 ? (word[0] & word[1]) != 0xffffffffu : word[0] != 0xffffffffu;
+            if (thin) {  // keys 32 kb + 8 g + 4 fh + i of this lane
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (!((word[kb] >> (4 * fh + 8 * (e >> 2) + (e & 3))) & 1u)) s[kb][e] = s_masked;
+            }
+            // Largest scaled score of the row over the tile, above the reference sub.
+            auto tile_max = [&](float sub) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) mx = fmaxf(mx, fmaf(s[kb][e], c, -sub));
+                return max_halves(mx);
+            };
+            if (__any(unset)) {
+                // (A row whose scores are all -inf so far adds nothing at any m, and must not keep one.)
+                const float t = tile_max(0.f);
+                if (unset && t != -INFINITY) {
+                    m = t;
+                    unset = false;
+                }
+            }
+            V8 pf[2 * KB];
+            auto exps = [&]() {
+                float sum = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float p = fast_exp2(fmaf(s[kb][e], c, -m));
+                        sum += p;
+                        pf[2 * kb + (e >> 3)][e & 7] = static_cast<T>(p);
+                    }
+                return sum;
+            };
+            float psum = exps();
+            const unsigned long long over = __ballot(!(psum <= kSumMax<T>));
+            if (over) {
+                // Lanes l and l ^ 32 hold one row's two key halves: either one asks for both.
+                const bool need = ((over >> lane) | (over >> (lane ^ 32))) & 1ull;
+                const float mx = tile_max(m);
+                const float nm = need ? m + mx : m, corr = fast_exp2(m - nm);
+                m = nm;
+#pragma unroll
+                for (int db = 0; db < DB; db++) o[db] *= corr;
+                l_run *= corr;
+                psum = exps();
+            }
+            l_run += psum;
+#pragma unroll
+            for (int g = 0; g < 2 * KB; g++) {
+#pragma unroll
+                for (int db = 0; db < DB; db++) {
+                    V8 vf = read_v<T, DH>(vt, g, db, lane);
+                    if (thin) {  // 0 times a masked value's NaN or infinity would not be 0
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (!((word[g >> 1] >> (16 * (g & 1) + 8 * (e >> 2) + 4 * fh + (e & 3))) & 1u)) vf[e] = static_cast<T>(0.f);
+                    }
+                    o[db] = mma<T>(vf, pf[g], o[db]);
+                }
+            }
+        }
+    }
+
+    // Join the key groups through LDS [group - 1][QW][16 DB + 2][64 lanes] in their order.
+    float m_run = unset ? -INFINITY : m;
+    if constexpr (KW > 1) {
+        float* comb = reinterpret_cast<float*>(smem) + lane;
+        __syncthreads();
+        if (kw > 0) {
+            float* cp = comb + ((kw - 1) * QW + qw) * PER;
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) cp[(16 * db + e) * 64] = o[db][e];
+            cp[16 * DB * 64] = m_run;
+            cp[(16 * DB + 1) * 64] = l_run;
+        }
+        __syncthreads();
+        if (kw > 0) return;
+#pragma unroll
+        for (int g = 1; g < KW; g++) {
+            const float* cp = comb + ((g - 1) * QW + qw) * PER;
+            const float m1 = cp[16 * DB * 64], l1 = cp[(16 * DB + 1) * 64];
+            const float mt = fmaxf(m_run, m1), mu = mt == -INFINITY ? 0.f : mt;
+            const float c0 = fast_exp2(m_run - mu), c1 = fast_exp2(m1 - mu);
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[db][e] = o[db][e] * c0 + cp[(16 * db + e) * 64] * c1;
+            l_run = l_run * c0 + l1 * c1;
+            m_run = mt;
+        }
+    }
+
+    // o[db][e] = O[row][32 db + 8 (e / 4) + 4 fh + e % 4].
+    const float l = sum_halves(l_run);
+    if (row >= rows) return;
+    if (a.splits > 1) {
+        const int64_t slot = ((int64_t)(b * a.kv_heads + hk) * a.splits + sp) * a.rows + row;
+        float* op = a.partial + slot * DH + 4 * fh;
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                *reinterpret_cast<float4*>(op + 32 * db + 8 * g) =
+                    make_float4(o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]);
+        float2* ml = reinterpret_cast<float2*>(a.partial + (int64_t)a.batch * a.kv_heads * a.splits * a.rows * DH);
+        if (fh == 0) ml[slot] = make_float2(m_run, l);
+        return;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    typedef T O4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    T* op = static_cast<T*>(a.out) + b * a.os[0] + tok * a.os[1] + head * a.os[2] + 4 * fh;
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            O4 v;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = static_cast<T>(o[db][4 * g + i] * inv);
+            *reinterpret_cast<O4*>(op + 32 * db + 8 * g) = v;
+        }
+}
+
+// The splits' results of a row joined: a wavefront per row, DH / 64 dimensions a lane.
+template <typename T, int DH>
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (w >= (int64_t)a.batch * a.kv_heads * a.rows) return;
+    const int row = (int)(w % a.rows), bh = (int)(w / a.rows), b = bh / a.kv_heads, hk = bh % a.kv_heads;
+    const int tok = row / a.group, head = hk * a.group + (row - tok * a.group);
+    if (a.q_len && tok >= a.q_len[b]) return;
+    const float2* ml = reinterpret_cast<const float2*>(a.partial + (int64_t)a.batch * a.kv_heads * a.splits * a.rows * DH);
+    constexpr int PER = DH / 64;
+    float o[PER], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; i++) o[i] = 0.f;
+    for (int s = 0; s < a.splits; s++) {
+        const int64_t slot = ((int64_t)bh * a.splits + s) * a.rows + row;
+        const float2 x = ml[slot];
+        const float mt = fmaxf(m, x.x), mu = mt == -INFINITY ? 0.f : mt;
+        const float c0 = fast_exp2(m - mu), c1 = fast_exp2(x.x - mu);
+#pragma unroll
+        for (int i = 0; i < PER; i++) o[i] = o[i] * c0 + a.partial[slot * DH + 64 * i + lane] * c1;
+        l = l * c0 + x.y * c1;
+        m = mt;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    T* op = static_cast<T*>(a.out) + b * a.os[0] + tok * a.os[1] + head * a.os[2];
+#pragma unroll
+    for (int i = 0; i < PER; i++) op[64 * i + lane] = static_cast<T>(o[i] * inv);
+}
+
+template <typename T, int DH, int QW, int KW, bool UNAL>
+int launch_cfg(const CrossArgs& a, hipStream_t st) {
+    const int rbs = (int)(((int64_t)a.rows + 32 * QW - 1) / (32 * QW));
+    const int64_t wgs = (int64_t)rbs * a.kv_heads * a.batch * a.splits;
+    const int64_t joins = ((int64_t)a.batch * a.kv_heads * a.rows + 3) / 4;
+    if (wgs > 0x7fffffffL || joins > 0x7fffffffL) return -1;
+    cross_kernel<T, DH, QW, KW, UNAL><<<(unsigned)wgs, 64 * QW * KW, 0, st>>>(a, rbs);
+    if (a.splits > 1) cross_join_kernel<T, DH><<<(unsigned)joins, 256, 0, st>>>(a);
+    return 0;
+}
+
+}  // namespace
+
+int cross_splits(int dtype, int batch, int kv_heads, int rows, int seq_kv, int head_dim) {
+    const int64_t wgs = (int64_t)((rows + 63) / 64) * batch * kv_heads;
+    const int tiles = (seq_kv + 63) / 64;
+    int64_t n = 512 / wgs;
+    n = n < tiles / 4 ? n : tiles / 4;
+    return n < 2 ? 1 : (int)(n < 64 ? n : 64);
+}
+
+template <typename T, int DH>
+int launch_cross(const CrossArgs& a, hipStream_t st) {
+    const int64_t es = sizeof(T);
+    // Windows of a tile's rows stay below 2^31 bytes, and the buffer-to-LDS loads take dword-aligned rows.
+    const bool unal = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 3) ||
+                      ((a.ks[0] | a.ks[1] | a.ks[2] | a.vs[0] | a.vs[1] | a.vs[2]) * es & 3) ||
+                      a.ks[1] * es > (1 << 24) || a.vs[1] * es > (1 << 24);
+    if (unal) return launch_cfg<T, DH, 2, 2, true>(a, st);
+    return launch_cfg<T, DH, 2, 2, false>(a, st);
+}
+
+template int launch_cross<bf16, 64>(const CrossArgs&, hipStream_t);
+template int launch_cross<bf16, 128>(const CrossArgs&, hipStream_t);
+template int launch_cross<f16, 64>(const CrossArgs&, hipStream_t);
+template int launch_cross<f16, 128>(const CrossArgs&, hipStream_t);
+template int launch_cross<float, 64>(const CrossArgs&, hipStream_t);
+template int launch_cross<float, 128>(const CrossArgs&, hipStream_t);
+
+}  // namespace irodori

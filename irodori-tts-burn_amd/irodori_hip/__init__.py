@@ -9,7 +9,8 @@ from .config import (CfgGuidanceMode, CodecConfig, DitConfig, EncoderConfig, Gui
                      InferenceBackendKind, IrodoriError, SamplerMethod, SamplerParams,
                      cfg_cpu_plumbing, cfg_full_rf, cfg_published_500m, cfg_tiny, codec_default, codec_tiny,
                      enc_speaker_default, enc_speaker_tiny, enc_text_default, enc_text_tiny)
-from .engine import HipDacVaeCodec, HipEncoder, HipInferenceEngine, ops
+from .engine import (CrossAttentionDesc, HipDacVaeCodec, HipEncoder, HipInferenceEngine, LinearDesc, RopeDesc,
+                     ops)
 from .inference import InferenceBuilder, InferenceEngine, ModelConfig, ModelWeights, SamplingRequest
 from .synthetic import (ROLE_COND, ROLE_NO_AUX, ROLE_NO_TEXT, ROLE_UNCOND, CodecWeights, ContextKV,
                         CtxProjWeights, DitWeights, EncoderWeights, make_context_kv, make_noise,
@@ -23,4 +24,5 @@ __all__ = [
     "EncoderConfig", "EncoderWeights", "enc_text_default", "enc_speaker_default", "enc_text_tiny",
     "enc_speaker_tiny", "CodecConfig", "CodecWeights", "HipDacVaeCodec", "codec_default",
     "codec_tiny", "InferenceBuilder", "InferenceEngine", "ModelConfig", "ModelWeights", "SamplingRequest",
+    "RopeDesc", "LinearDesc", "CrossAttentionDesc",
 ]

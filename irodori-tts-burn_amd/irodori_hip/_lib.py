@@ -123,6 +123,31 @@ class KernelTimesC(C.Structure):
                                           "wo_gemm_us", "w13_gemm_us", "w2_gemm_us", "final_us")]
 
 
+ROPE_LAYOUTS = {"interleaved": 0, "halves": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "by_parts": 3}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "sigmoid": 3, "tanh": 4, "gelu": 5, "gelu_tanh": 6}
+
+
+class RopeDescC(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "batch", "seq", "head_dim", "rot_dim", "q_heads", "k_heads",
+                                          "q_rot_heads", "k_rot_heads", "layout", "scaling", "inverse", "first_pos",
+                                          "reserved")] +
+                [(n, C.c_double) for n in ("theta", "factor", "trained_len", "beta_fast", "beta_slow", "amplitude")] +
+                [(n, C.c_int64 * 3) for n in ("q_strides", "q_out_strides", "k_strides", "k_out_strides")])
+
+
+class LinearDescC(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "out_dtype", "m", "n", "k", "activation", "gate_rows", "reserved")] +
+                [(n, C.c_int64) for n in ("ldx", "ldw", "ldy", "ldr")])
+
+
+class CrossAttentionDescC(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "batch", "seq_q", "seq_kv", "heads", "kv_heads", "head_dim")] +
+                [("scale", C.c_float)] +
+                [(n, C.c_int64 * 3) for n in ("q_strides", "k_strides", "v_strides", "out_strides")] +
+                [("mask_stride", C.c_int64)])
+
+
 # name -> (restype, argtypes): every symbol include/irodori_hip.h declares.
 _vp = C.c_void_p
 SIGNATURES = {
@@ -177,6 +202,12 @@ SIGNATURES = {
                                           C.c_int, C.c_int, C.c_float, _vp, _vp]),
     "irodori_op_joint_attention": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp]),
     "irodori_op_swiglu_mlp": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp]),
+    "irodori_op_rope": (C.c_int, [C.POINTER(RopeDescC), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "irodori_op_linear_workspace": (C.c_int, [C.POINTER(LinearDescC), C.POINTER(C.c_uint64)]),
+    "irodori_op_linear": (C.c_int, [C.POINTER(LinearDescC), _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_uint64, _vp]),
+    "irodori_op_cross_attention_workspace": (C.c_int, [C.POINTER(CrossAttentionDescC), C.POINTER(C.c_uint64)]),
+    "irodori_op_cross_attention": (C.c_int, [C.POINTER(CrossAttentionDescC), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                             C.c_uint64, _vp]),
     "irodori_op_mx_quantize": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp]),
     "irodori_op_gemm_fp8": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp]),
 }

@@ -531,6 +531,69 @@ class HipDacVaeCodec:
                                                     stream or None))
 
 
+_OP_DTYPES = {"f32": L.DTYPE_F32, "bf16": L.DTYPE_BF16, "f16": L.DTYPE_F16}
+
+
+def _choice(table, value, what: str) -> int:
+    if value not in table:
+        raise IrodoriError("Config", "%s must be one of %s, got %r" % (what, ", ".join(table), value))
+    return table[value]
+
+
+def _strides(given, seq: int, heads: int, dim: int):
+    """(batch, token, head) strides in elements; None: a contiguous [batch, seq, heads, dim]."""
+    if given is None:
+        given = (seq * heads * dim, heads * dim, dim)
+    if len(given) != 3:
+        raise IrodoriError("Shape", "strides are (batch, token, head), got %r" % (given,))
+    return (C.c_int64 * 3)(*given)
+
+
+class RopeDesc(L.RopeDescC):
+    """A call's shape for ops.rope (irodori_rope_desc), made once and kept: q [batch, seq, heads, head_dim]
+    and k [batch, seq, kv_heads, head_dim], contiguous unless strides say otherwise."""
+
+    def __init__(self, batch: int, seq: int, head_dim: int, *, heads: int, kv_heads: int = 0, dtype: str = "bf16",
+                 layout: str = "interleaved", rot_dim: int | None = None, rot_heads: int | None = None,
+                 rot_kv_heads: int | None = None, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                 trained_len: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0, amplitude: float = 1.0,
+                 inverse: bool = False, first_pos: int = 0, q_strides=None, q_out_strides=None, k_strides=None,
+                 k_out_strides=None):
+        super().__init__(_choice(_OP_DTYPES, dtype, "dtype"), batch, seq, head_dim,
+                         head_dim if rot_dim is None else rot_dim, heads, kv_heads,
+                         heads if rot_heads is None else rot_heads, kv_heads if rot_kv_heads is None else rot_kv_heads,
+                         _choice(L.ROPE_LAYOUTS, layout, "layout"), _choice(L.ROPE_SCALINGS, scaling, "scaling"),
+                         int(inverse), first_pos, 0, theta, factor, trained_len, beta_fast, beta_slow, amplitude,
+                         _strides(q_strides, seq, heads, head_dim), _strides(q_out_strides, seq, heads, head_dim),
+                         _strides(k_strides, seq, kv_heads, head_dim), _strides(k_out_strides, seq, kv_heads, head_dim))
+
+
+class LinearDesc(L.LinearDescC):
+    """A call's shape for ops.linear (irodori_linear_desc), made once and kept: x [m, k], w [n, k], y [m, n]."""
+
+    def __init__(self, m: int, n: int, k: int, *, dtype: str = "bf16", out_dtype: str | None = None,
+                 activation: str = "none", gate_rows: int = 0, ldx: int | None = None, ldw: int | None = None,
+                 ldy: int | None = None, ldr: int | None = None):
+        super().__init__(_choice(_OP_DTYPES, dtype, "dtype"), _choice(_OP_DTYPES, out_dtype or dtype, "out_dtype"), m, n, k,
+                         _choice(L.ACTIVATIONS, activation, "activation"), gate_rows, 0, k if ldx is None else ldx,
+                         k if ldw is None else ldw, n if ldy is None else ldy, n if ldr is None else ldr)
+
+
+class CrossAttentionDesc(L.CrossAttentionDescC):
+    """A call's shape for ops.cross_attention (irodori_cross_attention_desc), made once and kept:
+    q and out [batch, seq_q, heads, head_dim], k and v [batch, seq_kv, kv_heads, head_dim], contiguous
+    unless strides say otherwise; scale head_dim ** -0.5 by default."""
+
+    def __init__(self, batch: int, seq_q: int, seq_kv: int, heads: int, kv_heads: int, head_dim: int, *,
+                 dtype: str = "bf16", scale: float | None = None, q_strides=None, k_strides=None, v_strides=None,
+                 out_strides=None, mask_stride: int | None = None):
+        super().__init__(_choice(_OP_DTYPES, dtype, "dtype"), batch, seq_q, seq_kv, heads, kv_heads, head_dim,
+                         (head_dim ** -0.5 if head_dim > 0 else 0.0) if scale is None else scale,
+                         _strides(q_strides, seq_q, heads, head_dim), _strides(k_strides, seq_kv, kv_heads, head_dim),
+                         _strides(v_strides, seq_kv, kv_heads, head_dim), _strides(out_strides, seq_q, heads, head_dim),
+                         seq_kv if mask_stride is None else mask_stride)
+
+
 class ops:
     """Operator entry points (src/kernels analogues) on device pointers."""
 
@@ -565,3 +628,35 @@ class ops:
         64-dim operands limited to SDPA_SCRATCH_BYTES, the first call on a GPU outside capture."""
         _check(L.load().irodori_op_sdpa_noalloc(dtype, d_q, d_k, d_v, d_mask or None, batch, heads, seq_q,
                                                 seq_kv, head_dim, scale, d_out, stream or None))
+
+    @staticmethod
+    def rope(desc: RopeDesc, d_q, d_q_out, d_k=0, d_k_out=0, d_positions=0, d_lengths=0, stream: int = 0) -> None:
+        """Rotary positions of queries and keys (int32 positions [batch, seq], lengths [batch], or 0)."""
+        _check(L.load().irodori_op_rope(desc, d_q or None, d_q_out or None, d_k or None, d_k_out or None,
+                                        d_positions or None, d_lengths or None, stream or None))
+
+    @staticmethod
+    def linear_workspace(desc: LinearDesc) -> int:
+        n = C.c_uint64()
+        _check(L.load().irodori_op_linear_workspace(desc, n))
+        return n.value
+
+    @staticmethod
+    def linear(desc: LinearDesc, d_x, d_w, d_y, d_bias=0, d_gate=0, d_residual=0, d_workspace=0, workspace_bytes: int = 0,
+               stream: int = 0) -> None:
+        """y = residual + gate * act(x w^T + bias); bias and gate f32, each optional one 0."""
+        _check(L.load().irodori_op_linear(desc, d_x, d_w, d_bias or None, d_gate or None, d_residual or None, d_y,
+                                          d_workspace or None, workspace_bytes, stream or None))
+
+    @staticmethod
+    def cross_attention_workspace(desc: CrossAttentionDesc) -> int:
+        n = C.c_uint64()
+        _check(L.load().irodori_op_cross_attention_workspace(desc, n))
+        return n.value
+
+    @staticmethod
+    def cross_attention(desc: CrossAttentionDesc, d_q, d_k, d_v, d_out, d_mask=0, d_q_len=0, d_kv_len=0, d_workspace=0,
+                        workspace_bytes: int = 0, stream: int = 0) -> None:
+        """Attention of each query to its row's keys (mask uint8, lengths int32, each 0 for all)."""
+        _check(L.load().irodori_op_cross_attention(desc, d_q, d_k, d_v, d_mask or None, d_q_len or None, d_kv_len or None,
+                                                   d_out, d_workspace or None, workspace_bytes, stream or None))
