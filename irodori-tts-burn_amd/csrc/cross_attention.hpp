@@ -13,7 +13,7 @@ struct CrossArgs {
     void* out;
     const uint8_t* mask;          // [batch][mask_stride], nonzero = attend; may be null
     const int32_t *q_len, *kv_len;  // [batch]; may be null
-    float* partial;               // splits > 1: [batch kv_heads][split][rows][head_dim], then (m, l) of each row
+    float* partial;               // splits > 1: [kv_heads][splits + batch][rows][head_dim], then (m, l) of each row
     int64_t qs[3], ks[3], vs[3], os[3];  // batch, token, head strides in elements
     int64_t mask_stride;
     int batch, heads, kv_heads, group, seq_q, seq_kv, splits;
@@ -21,10 +21,10 @@ struct CrossArgs {
     float scale;
 };
 
-// Key splits of a launch, and the bytes of their partial results (0 where there is one).
-int cross_splits(int dtype, int batch, int kv_heads, int rows, int seq_kv, int head_dim);
+// Runs that the keys of a launch are split into (1: none), and the bytes of their partial results.
+int cross_splits(int batch, int kv_heads, int rows, int seq_kv);
 inline int64_t cross_partial_bytes(int splits, int batch, int kv_heads, int rows, int head_dim) {
-    return splits > 1 ? (int64_t)splits * batch * kv_heads * rows * (head_dim + 2) * 4 : 0;
+    return splits > 1 ? ((int64_t)splits + batch) * kv_heads * rows * (head_dim + 2) * 4 : 0;
 }
 
 // 0, or -1 where the grid would not fit one launch.

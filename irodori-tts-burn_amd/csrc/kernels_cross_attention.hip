@@ -41,6 +41,16 @@ __device__ __forceinline__ int vswz(int r, int c) {
     return ROWB == 128 ? c ^ (2 * ((r >> 1) & 3)) : c ^ (2 * (r & 7));
 }
 
+// Waits as builtins, which the compiler's own count of outstanding reads takes into account.
+__device__ __forceinline__ void wait_lds() {
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_all() {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
 // The 8 reduction elements of a lane.
 template <typename T>
 struct Op8 {
@@ -113,23 +123,19 @@ __device__ __forceinline__ f32x16 score_block(const unsigned char* kt, int kb, i
     return s;
 }
 
-// Validity of the KT keys from t0 on, of which n (<= KT) exist.
+// Validity of KT keys.
 template <int KT>
-__device__ __forceinline__ unsigned long long mask_bits(const uint8_t* m, int n) {
+__device__ __forceinline__ unsigned long long mask_bits(const uint8_t* m) {
     typedef unsigned u32x4_b __attribute__((ext_vector_type(4), aligned(1)));
     unsigned long long bits = 0;
-    if (n >= KT) {
 #pragma unroll
-        for (int i = 0; i < KT / 16; i++) {
-            const u32x4_b w = *reinterpret_cast<const u32x4_b*>(m + 16 * i);
+    for (int i = 0; i < KT / 16; i++) {
+        const u32x4_b w = *reinterpret_cast<const u32x4_b*>(m + 16 * i);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const unsigned nz = ((((w[j] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[j]) >> 7) & 0x01010101u;
-                bits |= (unsigned long long)((nz * 0x01020408u) >> 24 & 0xfu) << (16 * i + 4 * j);
-            }
+        for (int j = 0; j < 4; j++) {
+            const unsigned nz = ((((w[j] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[j]) >> 7) & 0x01010101u;
+            bits |= (unsigned long long)((nz * 0x01020408u) >> 24 & 0xfu) << (16 * i + 4 * j);
         }
-    } else {
-        for (int i = 0; i < n; i++) bits |= (unsigned long long)(m[i] != 0) << i;
     }
     return bits;
 }
@@ -142,12 +148,13 @@ struct TileWord {
 };
 template <int KT>
 __device__ __forceinline__ TileWord tile_word(const uint8_t* mask, int len, int t0, int te, int lane) {
-    const int t = t0 + lane;
+    const int t = t0 + lane, n = len - t * KT;  // keys from the lane's tile on
     unsigned long long bits = 0ull;
-    if (t < te) {
-        const int n = len - t * KT < KT ? len - t * KT : KT;
-        if (mask) bits = mask_bits<KT>(mask + (int64_t)t * KT, n);
-        else bits = n == 64 ? ~0ull : (1ull << n) - 1ull;
+    if (t < te && n >= KT) bits = mask ? mask_bits<KT>(mask + (int64_t)t * KT) : KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1ull;
+    const int part = len / KT, rest = len % KT;  // the tile that the keys end in: a byte a lane
+    if (rest && part >= t0 && part < te && part < t0 + 64) {
+        const unsigned long long b = __ballot(lane < rest && (!mask || mask[(int64_t)part * KT + (lane < rest ? lane : 0)]));
+        if (t == part) bits = b;
     }
     const bool on = bits != 0ull;
     const unsigned long long act = __ballot(on);
@@ -161,21 +168,41 @@ __device__ __forceinline__ TileWord tile_word(const uint8_t* mask, int len, int 
     return tw;
 }
 
+// Keys of batch row b.
+__device__ __forceinline__ int row_keys(const CrossArgs& a, int b) {
+    int n = a.seq_kv;
+    if (a.kv_len) n = a.kv_len[b];
+    return n < 0 ? 0 : n < a.seq_kv ? n : a.seq_kv;
+}
+// Key tiles of the 64 batch rows from b0 on, a lane each.
+template <int KT>
+__device__ __forceinline__ int lane_tiles(const CrossArgs& a, int b0, int lane) {
+    return b0 + lane < a.batch ? (row_keys(a, b0 + lane) + KT - 1) / KT : 0;
+}
+__device__ __forceinline__ int wave_sum(int v) {  // (beside the float one)
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+using irodori::wave_sum;
+
 // A workgroup: QW wavefronts of 32 rows times KW groups that take the tiles in turn and are joined
 // through LDS.  Two ring slots of KW K and V tiles, moved HBM -> LDS by buffer_load_dwordx4 ... lds;
 // UNAL: through registers, for operands off a dword boundary or with rows too far apart for a window.
-template <typename T, int DH, int QW, int KW, bool UNAL>
-__global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(1, 2))) void cross_kernel(CrossArgs a,
-                                                                                                        int row_blocks) {
+// Without splits it takes one batch row's keys.  With them, the tiles of all batch rows lie end to end
+// and each of a.splits workgroups of a key head and row block takes an equal run of them, of several
+// batch rows where they are short; the result for batch row b from workgroup w goes to slot w + b.
+template <typename T, int DH, int QW, int KW, int WPE, bool UNAL>
+__global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WPE))) void cross_kernel(CrossArgs a,
+                                                                                                       int row_blocks) {
     typedef typename Op8<T>::type V8;
     constexpr int NW = QW * KW, KT = kTile<T>, KB = KT / 32, ROWB = DH * (int)sizeof(T), TILE = KT * ROWB;
     constexpr int RPI = 1024 / ROWB, NI = KT / RPI, LPW = KW * NI / NW, DB = DH / 32, CH = ROWB / 16;
     constexpr int RING = 4 * KW * TILE, PER = (DB * 16 + 2) * 64;
-    static_assert(LPW * NW == KW * NI, "a stage's loads split over the waves");
+    static_assert(LPW * NW == KW * NI && NI % LPW == 0, "a wavefront's loads of a stage lie in one tile");
     static_assert((KW - 1) * QW * PER * 4 <= RING, "the groups' results fit the rings");
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[RING];
-    unsigned char* kring = smem;                  // [2][KW][TILE]
-    unsigned char* vring = smem + 2 * KW * TILE;  // [2][KW][TILE]
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[RING];  // K [2][KW][TILE], V [2][KW][TILE]
+    constexpr int VOFF = 2 * KW * TILE;
 
     const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -183,303 +210,400 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(1,
     int id = xcd_remap(blockIdx.x, gridDim.x);
     const int rb = id % row_blocks;
     id /= row_blocks;
-    const int sp = id % a.splits;
-    id /= a.splits;
-    const int hk = id % a.kv_heads, b = id / a.kv_heads;
-    int rows = a.rows;
-    if (a.q_len) {
-        const int n = a.q_len[b];
-        rows = n <= 0 ? 0 : (n < a.seq_q ? n : a.seq_q) * a.group;
+    const bool split = a.splits > 1;
+    int b, hk, w = 0;
+    int64_t at = 0, stop = 0;  // split: the run's next tile and its end, in all batch rows' tiles
+    if (split) {
+        w = id % a.splits;
+        hk = id / a.splits;
+        int64_t all = 0;
+        for (int i = 0; i < a.batch; i += 64) all += wave_sum(lane_tiles<KT>(a, i, lane));
+        at = all * w / a.splits;
+        stop = all * (w + 1) / a.splits;
+        b = 0;
+    } else {
+        hk = id % a.kv_heads;
+        b = id / a.kv_heads;
     }
-    const int row0 = rb * 32 * QW;
-    if (row0 >= rows) return;  // rows past the length stay as they were
-    int len = a.seq_kv;
-    if (a.kv_len) {
-        const int n = a.kv_len[b];
-        len = n < 0 ? 0 : n < len ? n : len;
-    }
-    const int nt = (len + KT - 1) / KT;
-    const int t_begin = (int)((int64_t)nt * sp / a.splits), t_end = (int)((int64_t)nt * (sp + 1) / a.splits);
-    const T* Kb = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
-    const T* Vb = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
-    const uint8_t* mb = a.mask ? a.mask + b * a.mask_stride : nullptr;
     // c = 0 would turn a masked key's -inf into NaN; a tiny c gives the same exp2(0).
     float c = a.scale * 1.4426950408889634f;
     c = c == 0.f ? 1e-38f : c;
-    const float s_masked = c > 0.f ? -INFINITY : INFINITY;
-
-    const int row = row0 + 32 * qw + fr, rc = row < rows ? row : rows - 1;
-    const int tok = rc / a.group, head = hk * a.group + (rc - tok * a.group);
-    V8 qf[DH / 16];
-    {
-        typedef T Q8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-        const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + tok * a.qs[1] + head * a.qs[2] + 8 * fh;
-#pragma unroll
-        for (int ks = 0; ks < DH / 16; ks++) qf[ks] = __builtin_bit_cast(V8, *reinterpret_cast<const Q8*>(qp + 16 * ks));
-    }
-    f32x16 o[DB];
-#pragma unroll
-    for (int db = 0; db < DB; db++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) o[db][e] = 0.f;
-    float m = 0.f, l_run = 0.f;
-    bool unset = true;  // m is no reference yet: no tile so far, or only scores of -inf
-
-    // Load instruction ii of this wave in a stage: gi = wave LPW + ii -> group gi / NI, rows RPI
-    // (gi % NI) ..; lane -> row lane / CH, physical chunk lane % CH.
+    const unsigned masked = __builtin_bit_cast(unsigned, c > 0.f ? -INFINITY : INFINITY);
+    // Load instruction ii of this wave in a stage: rows RPI (row0 + ii) .. of tile `tile` of the step's;
+    // lane -> row lane / CH, physical chunk lane % CH.
+    const int tile = wave * LPW / NI, part = wave * LPW % NI;
     unsigned voK[LPW], voV[LPW];
 #pragma unroll
     for (int ii = 0; ii < LPW; ii++) {
-        const int r = ((wave * LPW + ii) % NI) * RPI + lane / CH;
+        const int r = (part + ii) * RPI + lane / CH;
         voK[ii] = (unsigned)(r * (a.ks[1] * (int)sizeof(T))) + (kswz<ROWB>(r, lane % CH) << 4);
         voV[ii] = (unsigned)(r * (a.vs[1] * (int)sizeof(T))) + (vswz<T, ROWB>(r, lane % CH) << 4);
     }
 
-    for (int t0 = t_begin; t0 < t_end; t0 += 64) {
-        const TileWord tw = tile_word<KT>(mb, len, t0, t_end, lane);
-        const int nact = tw.n, niter = (nact + KW - 1) / KW;
-        if (niter == 0) continue;  // the same for every wave
-        if (t0 > t_begin) {        // the rings are still being read
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            raw_barrier();
+    int tiles = 0;  // split: those of the lane's batch row among the 64 around b
+    for (int64_t before = 0;; b++) {  // batch rows of the run
+        int t_begin = 0, t_end;
+        if (split) {
+            if (at >= stop) return;
+            if (b % 64 == 0) tiles = lane_tiles<KT>(a, b, lane);
+            t_end = __builtin_amdgcn_readlane(tiles, b & 63);
+            const int64_t after = before + t_end;
+            if (at >= after) {
+                before = after;
+                continue;
+            }
+            t_begin = (int)(at - before);
+            if (stop < after) t_end = (int)(stop - before);
+            at = before + t_end;
+            before = after;
         }
-        // The K and V tiles of step j into their ring slot.  Entries past the last are clamped to it,
-        // so every wave issues the same loads.
-        auto issue = [&](int j) {
-            const int slot = j & 1;
+        int rows = a.rows;
+        if (a.q_len) {
+            const int n = a.q_len[b];
+            rows = n <= 0 ? 0 : (n < a.seq_q ? n : a.seq_q) * a.group;
+        }
+        const int row0 = rb * 32 * QW;
+        if (row0 >= rows) {  // rows past the length stay as they were
+            if (split) continue;
+            return;
+        }
+        const int len = row_keys(a, b);
+        if (!split) t_end = (len + KT - 1) / KT;
+        const T* Kb = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[2];
+        const T* Vb = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[2];
+        const uint8_t* mb = a.mask ? a.mask + b * a.mask_stride : nullptr;
+        const int row = row0 + 32 * qw + fr, rc = row < rows ? row : rows - 1;
+        const int tok = rc / a.group, head = hk * a.group + (rc - tok * a.group);
+        V8 qf[DH / 16];
+        {
+            typedef T Q8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+            const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + tok * a.qs[1] + head * a.qs[2] + 8 * fh;
 #pragma unroll
-            for (int ii = 0; ii < LPW; ii++) {
-                const int gi = wave * LPW + ii, g = gi / NI;
-                int li = j * KW + g;
+            for (int ks = 0; ks < DH / 16; ks++) qf[ks] = __builtin_bit_cast(V8, *reinterpret_cast<const Q8*>(qp + 16 * ks));
+        }
+        f32x16 o[DB];
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[db][e] = 0.f;
+        float m = 0.f, l_run = 0.f;
+        bool unset = true;  // m is no reference yet: no tile so far, or only scores of -inf
+        bool first = true;  // any lane's unset
+
+        for (int t0 = t_begin; t0 < t_end; t0 += 64) {
+            const TileWord tw = tile_word<KT>(mb, len, t0, t_end, lane);
+            const int nact = tw.n, niter = (nact + KW - 1) / KW;
+            if (niter == 0) continue;  // the same for every wave
+            wait_lds();
+            raw_barrier();  // the rings may still be read
+            // This wave's share of the K and V tiles of step j into their ring slot.  Entries past the last
+            // are clamped to it, so every wave issues the same loads.
+            auto issue = [&](int j) {
+                int li = j * KW + tile;
                 li = li < nact ? li : nact - 1;
                 const int t = __builtin_amdgcn_readlane(tw.t, li);
                 const int left = len - t * KT, n = left < KT ? left : KT;  // rows of the tile
                 const T* ksrc = Kb + (int64_t)t * KT * a.ks[1];
                 const T* vsrc = Vb + (int64_t)t * KT * a.vs[1];
-                unsigned char* kd = kring + (slot * KW + g) * TILE + (gi % NI) * 1024;
-                unsigned char* vd = vring + (slot * KW + g) * TILE + (gi % NI) * 1024;
-                if constexpr (UNAL) {
-                    typedef T E16 __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-                    const int r = (gi % NI) * RPI + lane / CH;
-                    u32x4 kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
-                    if (r < n) {
-                        const int per = 16 / (int)sizeof(T);
-                        kx = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(ksrc + r * a.ks[1] + kswz<ROWB>(r, lane % CH) * per));
-                        vx = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(vsrc + r * a.vs[1] + vswz<T, ROWB>(r, lane % CH) * per));
+                unsigned char* dst = smem + ((j & 1) * KW + tile) * TILE + part * 1024;
+#pragma unroll
+                for (int ii = 0; ii < LPW; ii++) {
+                    if constexpr (UNAL) {
+                        typedef T E16 __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+                        constexpr int PE = 16 / (int)sizeof(T);
+                        const int r = (part + ii) * RPI + lane / CH;
+                        u32x4 kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
+                        if (r < n) {
+                            kx = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(ksrc + r * a.ks[1] + kswz<ROWB>(r, lane % CH) * PE));
+                            vx = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(vsrc + r * a.vs[1] + vswz<T, ROWB>(r, lane % CH) * PE));
+                        }
+                        *reinterpret_cast<u32x4*>(dst + ii * 1024 + 16 * lane) = kx;
+                        *reinterpret_cast<u32x4*>(dst + VOFF + ii * 1024 + 16 * lane) = vx;
+                    } else {
+                        // Rows past the last key read as zero.
+                        buf_load_lds16(make_rsrc(ksrc, (unsigned)((n - 1) * a.ks[1] * (int)sizeof(T)) + ROWB), voK[ii], dst + ii * 1024);
+                        buf_load_lds16(make_rsrc(vsrc, (unsigned)((n - 1) * a.vs[1] * (int)sizeof(T)) + ROWB), voV[ii], dst + VOFF + ii * 1024);
                     }
-                    *reinterpret_cast<u32x4*>(kd + 16 * lane) = kx;
-                    *reinterpret_cast<u32x4*>(vd + 16 * lane) = vx;
-                } else {
-                    // Rows past the last key read as zero.
-                    buf_load_lds16(make_rsrc(ksrc, (unsigned)((n - 1) * a.ks[1] * (int)sizeof(T)) + ROWB), voK[ii], kd);
-                    buf_load_lds16(make_rsrc(vsrc, (unsigned)((n - 1) * a.vs[1] * (int)sizeof(T)) + ROWB), voV[ii], vd);
                 }
-            }
-        };
-        issue(0);
-        for (int j = 0; j < niter; j++) {
-            // This wave's loads of step j have landed, and its reads of the slot refilled next are done.
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            raw_barrier();
-            if (j + 1 < niter) issue(j + 1);
-            const int li = j * KW + kw;
-            if (li >= nact) continue;  // this group has no tile in the last step
-            const unsigned char* kt = kring + ((j & 1) * KW + kw) * TILE;
-            const unsigned char* vt = vring + ((j & 1) * KW + kw) * TILE;
-            f32x16 s[KB];
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++) s[kb] = score_block<T, DH>(kt, kb, fr, fh, qf);
-            const unsigned word[2] = {(unsigned)__builtin_amdgcn_readlane(tw.lo, li),
-                                      (unsigned)__builtin_amdgcn_readlane(tw.hi, li)};
-            const bool thin = KB == 2 ? (word[0] & word[1]) != 0xffffffffu : word[0] != 0xffffffffu;
-            if (thin) {  // keys 32 kb + 8 g + 4 fh + i of this lane
-#pragma unroll
-                for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (!((word[kb] >> (4 * fh + 8 * (e >> 2) + (e & 3))) & 1u)) s[kb][e] = s_masked;
-            }
-            // Largest scaled score of the row over the tile, above the reference sub.
-            auto tile_max = [&](float sub) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) mx = fmaxf(mx, fmaf(s[kb][e], c, -sub));
-                return max_halves(mx);
             };
-            if (__any(unset)) {
-                // (A row whose scores are all -inf so far adds nothing at any m, and must not keep one.)
-                const float t = tile_max(0.f);
-                if (unset && t != -INFINITY) {
-                    m = t;
-                    unset = false;
+            issue(0);
+            for (int j = 0; j < niter; j++) {
+                // This wave's loads of step j have landed; the masked rows among its V rows become zero (0 times
+                // a masked value's NaN or infinity would not be 0).
+                wait_all();
+                if (mb) {
+                    int li = j * KW + tile;
+                    li = li < nact ? li : nact - 1;
+                    const unsigned lo = (unsigned)__builtin_amdgcn_readlane(tw.lo, li), hi = (unsigned)__builtin_amdgcn_readlane(tw.hi, li);
+                    if ((KB == 2 ? lo & hi : lo) != 0xffffffffu) {
+                        unsigned char* dst = smem + VOFF + ((j & 1) * KW + tile) * TILE + part * 1024 + 16 * lane;
+#pragma unroll
+                        for (int ii = 0; ii < LPW; ii++) {
+                            const int r = (part + ii) * RPI + lane / CH;
+                            if (!(((r < 32 ? lo : hi) >> (r & 31)) & 1u)) *reinterpret_cast<u32x4*>(dst + ii * 1024) = u32x4{0, 0, 0, 0};
+                        }
+                        wait_lds();
+                    }
+                }
+                raw_barrier();
+                if (j + 1 < niter) issue(j + 1);
+                const int li = j * KW + kw;
+                if (li >= nact) continue;  // this group has no tile in the last step
+                const unsigned char* kt = smem + ((j & 1) * KW + kw) * TILE;
+                const unsigned char* vt = kt + VOFF;
+                f32x16 s[KB];
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++) s[kb] = score_block<T, DH>(kt, kb, fr, fh, qf);
+                const unsigned word[2] = {(unsigned)__builtin_amdgcn_readlane(tw.lo, li),
+                                          (unsigned)__builtin_amdgcn_readlane(tw.hi, li)};
+                if ((KB == 2 ? word[0] & word[1] : word[0]) != 0xffffffffu) {  // keys 32 kb + 8 g + 4 fh + i of this lane
+#pragma unroll
+                    for (int kb = 0; kb < KB; kb++) {
+                        const int wd = (int)(word[kb] >> (4 * fh));
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const unsigned on = (unsigned)__builtin_amdgcn_sbfe(wd, 8 * (e >> 2) + (e & 3), 1);  // all ones or none
+                            const float x = s[kb][e];  // (a bit_cast of the vector's element itself takes element 0)
+                            s[kb][e] = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, x) & on) | (masked & ~on));
+                        }
+                    }
+                }
+                // Largest of f(score) of the row over the tile.
+                auto tile_max = [&](auto f) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) mx = fmaxf(mx, f(s[kb][e]));
+                    return max_halves(mx);
+                };
+                if (first) {
+                    // (A row whose scores are all -inf so far adds nothing at any m, and must not keep one.)
+                    const float t = tile_max([&](float x) { return x * c; });
+                    if (unset && t != -INFINITY) {
+                        m = t;
+                        unset = false;
+                    }
+                    first = __any(unset);
+                }
+                // The scores become their distances f(s) from the reference, which alone stay live.
+                V8 pf[2 * KB];
+                auto exps = [&](auto f) {
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            s[kb][e] = f(s[kb][e]);
+                            const float p = fast_exp2(s[kb][e]);
+                            pf[2 * kb + (e >> 3)][e & 7] = static_cast<T>(p);
+                            if (!std::is_same<T, bf16>::value) sum[e & 3] += p;
+                        }
+                    if constexpr (std::is_same<T, bf16>::value) {
+                        // Two rounded elements an instruction (455 us where 32 additions take 470 at 32 x 750 x 4100
+                        // keys of 20 heads; f16's like instruction loses, 492).
+                        typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+                        for (int g = 0; g < 2 * KB; g++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                sum[i] = __builtin_amdgcn_fdot2_f32_bf16(B2{pf[g][2 * i], pf[g][2 * i + 1]}, B2{1.f, 1.f}, sum[i], false);
+                    }
+                    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                };
+                float psum = exps([&](float x) { return fmaf(x, c, -m); });
+                const unsigned long long over = __ballot(!(psum <= kSumMax<T>));
+                if (over) {
+                    // Lanes l and l ^ 32 hold one row's two key halves: either one asks for both.
+                    const bool need = ((over >> lane) | (over >> (lane ^ 32))) & 1ull;
+                    const float mx = tile_max([](float x) { return x; });
+                    const float shift = need ? mx : 0.f, corr = fast_exp2(-shift);
+                    m += shift;
+#pragma unroll
+                    for (int db = 0; db < DB; db++) o[db] *= corr;
+                    l_run *= corr;
+                    psum = exps([&](float x) { return x - shift; });
+                }
+                l_run += psum;
+#pragma unroll
+                for (int g = 0; g < 2 * KB; g++)
+#pragma unroll
+                    for (int db = 0; db < DB; db++) o[db] = mma<T>(read_v<T, DH>(vt, g, db, lane), pf[g], o[db]);
+            }
+        }
+
+        // Join the key groups through LDS [group - 1][QW][16 DB + 2][64 lanes] in their order.
+        float m_run = unset ? -INFINITY : m;
+        if constexpr (KW > 1) {
+            float* comb = reinterpret_cast<float*>(smem) + lane;
+            __syncthreads();
+            if (kw > 0) {
+                float* cp = comb + ((kw - 1) * QW + qw) * PER;
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) cp[(16 * db + e) * 64] = o[db][e];
+                cp[16 * DB * 64] = m_run;
+                cp[(16 * DB + 1) * 64] = l_run;
+            }
+            __syncthreads();
+            if (kw == 0) {
+#pragma unroll
+                for (int g = 1; g < KW; g++) {
+                    const float* cp = comb + ((g - 1) * QW + qw) * PER;
+                    const float m1 = cp[16 * DB * 64], l1 = cp[(16 * DB + 1) * 64];
+                    const float mt = fmaxf(m_run, m1), mu = mt == -INFINITY ? 0.f : mt;
+                    const float c0 = fast_exp2(m_run - mu), c1 = fast_exp2(m1 - mu);
+#pragma unroll
+                    for (int db = 0; db < DB; db++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[db][e] = o[db][e] * c0 + cp[(16 * db + e) * 64] * c1;
+                    l_run = l_run * c0 + l1 * c1;
+                    m_run = mt;
                 }
             }
-            V8 pf[2 * KB];
-            auto exps = [&]() {
-                float sum = 0.f;
+        }
+
+        // o[db][e] = O[row][32 db + 8 (e / 4) + 4 fh + e % 4].
+        const float l = sum_halves(l_run);
+        if (kw == 0 && row < rows) {
+            if (split) {
+                const int64_t slot = ((int64_t)hk * (a.splits + a.batch) + w + b) * a.rows + row;
+                float* op = a.partial + slot * DH + 4 * fh;
 #pragma unroll
-                for (int kb = 0; kb < KB; kb++)
+                for (int db = 0; db < DB; db++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float p = fast_exp2(fmaf(s[kb][e], c, -m));
-                        sum += p;
-                        pf[2 * kb + (e >> 3)][e & 7] = static_cast<T>(p);
+                    for (int g = 0; g < 4; g++)
+                        *reinterpret_cast<float4*>(op + 32 * db + 8 * g) =
+                            make_float4(o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]);
+                float2* ml = reinterpret_cast<float2*>(a.partial + (int64_t)a.kv_heads * (a.splits + a.batch) * a.rows * DH);
+                if (fh == 0) ml[slot] = make_float2(m_run, l);
+            } else {
+                const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+                typedef T O4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+                T* op = static_cast<T*>(a.out) + b * a.os[0] + tok * a.os[1] + head * a.os[2] + 4 * fh;
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        O4 v;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) v[i] = static_cast<T>(o[db][4 * g + i] * inv);
+                        *reinterpret_cast<O4*>(op + 32 * db + 8 * g) = v;
                     }
-                return sum;
-            };
-            float psum = exps();
-            const unsigned long long over = __ballot(!(psum <= kSumMax<T>));
-            if (over) {
-                // Lanes l and l ^ 32 hold one row's two key halves: either one asks for both.
-                const bool need = ((over >> lane) | (over >> (lane ^ 32))) & 1ull;
-                const float mx = tile_max(m);
-                const float nm = need ? m + mx : m, corr = fast_exp2(m - nm);
-                m = nm;
-#pragma unroll
-                for (int db = 0; db < DB; db++) o[db] *= corr;
-                l_run *= corr;
-                psum = exps();
-            }
-            l_run += psum;
-#pragma unroll
-            for (int g = 0; g < 2 * KB; g++) {
-#pragma unroll
-                for (int db = 0; db < DB; db++) {
-                    V8 vf = read_v<T, DH>(vt, g, db, lane);
-                    if (thin) {  // 0 times a masked value's NaN or infinity would not be 0
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (!((word[g >> 1] >> (16 * (g & 1) + 8 * (e >> 2) + 4 * fh + (e & 3))) & 1u)) vf[e] = static_cast<T>(0.f);
-                    }
-                    o[db] = mma<T>(vf, pf[g], o[db]);
-                }
             }
         }
+        if (!split) return;
     }
-
-    // Join the key groups through LDS [group - 1][QW][16 DB + 2][64 lanes] in their order.
-    float m_run = unset ? -INFINITY : m;
-    if constexpr (KW > 1) {
-        float* comb = reinterpret_cast<float*>(smem) + lane;
-        __syncthreads();
-        if (kw > 0) {
-            float* cp = comb + ((kw - 1) * QW + qw) * PER;
-#pragma unroll
-            for (int db = 0; db < DB; db++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) cp[(16 * db + e) * 64] = o[db][e];
-            cp[16 * DB * 64] = m_run;
-            cp[(16 * DB + 1) * 64] = l_run;
-        }
-        __syncthreads();
-        if (kw > 0) return;
-#pragma unroll
-        for (int g = 1; g < KW; g++) {
-            const float* cp = comb + ((g - 1) * QW + qw) * PER;
-            const float m1 = cp[16 * DB * 64], l1 = cp[(16 * DB + 1) * 64];
-            const float mt = fmaxf(m_run, m1), mu = mt == -INFINITY ? 0.f : mt;
-            const float c0 = fast_exp2(m_run - mu), c1 = fast_exp2(m1 - mu);
-#pragma unroll
-            for (int db = 0; db < DB; db++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) o[db][e] = o[db][e] * c0 + cp[(16 * db + e) * 64] * c1;
-            l_run = l_run * c0 + l1 * c1;
-            m_run = mt;
-        }
-    }
-
-    // o[db][e] = O[row][32 db + 8 (e / 4) + 4 fh + e % 4].
-    const float l = sum_halves(l_run);
-    if (row >= rows) return;
-    if (a.splits > 1) {
-        const int64_t slot = ((int64_t)(b * a.kv_heads + hk) * a.splits + sp) * a.rows + row;
-        float* op = a.partial + slot * DH + 4 * fh;
-#pragma unroll
-        for (int db = 0; db < DB; db++)
-#pragma unroll
-            for (int g = 0; g < 4; g++)
-                *reinterpret_cast<float4*>(op + 32 * db + 8 * g) =
-                    make_float4(o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]);
-        float2* ml = reinterpret_cast<float2*>(a.partial + (int64_t)a.batch * a.kv_heads * a.splits * a.rows * DH);
-        if (fh == 0) ml[slot] = make_float2(m_run, l);
-        return;
-    }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    typedef T O4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    T* op = static_cast<T*>(a.out) + b * a.os[0] + tok * a.os[1] + head * a.os[2] + 4 * fh;
-#pragma unroll
-    for (int db = 0; db < DB; db++)
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            O4 v;
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = static_cast<T>(o[db][4 * g + i] * inv);
-            *reinterpret_cast<O4*>(op + 32 * db + 8 * g) = v;
-        }
 }
 
-// The splits' results of a row joined: a wavefront per row, DH / 64 dimensions a lane.
+// The runs' results of a row joined: a wavefront per row.  Lane i holds the weight exp2(m_i - M) of run i,
+// 64 at a time; a lane then sums DH / 64 dimensions, four runs' loads in flight.
 template <typename T, int DH>
-__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (w >= (int64_t)a.batch * a.kv_heads * a.rows) return;
-    const int row = (int)(w % a.rows), bh = (int)(w / a.rows), b = bh / a.kv_heads, hk = bh % a.kv_heads;
+__global__ __launch_bounds__(64) void cross_join_kernel(CrossArgs a) {
+    const int lane = threadIdx.x;
+    const int row = (int)(blockIdx.x % (unsigned)a.rows), bh = (int)(blockIdx.x / (unsigned)a.rows);
+    const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
     const int tok = row / a.group, head = hk * a.group + (row - tok * a.group);
     if (a.q_len && tok >= a.q_len[b]) return;
-    const float2* ml = reinterpret_cast<const float2*>(a.partial + (int64_t)a.batch * a.kv_heads * a.splits * a.rows * DH);
+    int64_t all = 0, before = 0;
+    int mine = 0;
+    for (int x = 0; x < a.batch; x += 64) {
+        const int n = lane_tiles<kTile<T>>(a, x, lane);
+        all += wave_sum(n);
+        before += wave_sum(x + lane < b ? n : 0);
+        if (b - x >= 0 && b - x < 64) mine = __builtin_amdgcn_readlane(n, b - x);
+    }
+    // Run w holds tiles all w / splits .. all (w + 1) / splits - 1: those from w0 to w1 have some of row b's.
+    int w0 = 0, w1 = -1;
+    if (mine > 0) {
+        w0 = (int)(((before + 1) * a.splits + all - 1) / all) - 1;
+        w1 = (int)(((before + mine) * a.splits + all - 1) / all) - 1;
+    }
+    const int64_t slot0 = ((int64_t)hk * (a.splits + a.batch) + b) * a.rows + row;  // run w's is w rows further
+    const float2* ml = reinterpret_cast<const float2*>(a.partial + (int64_t)a.kv_heads * (a.splits + a.batch) * a.rows * DH);
     constexpr int PER = DH / 64;
     float o[PER], m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER; i++) o[i] = 0.f;
-    for (int s = 0; s < a.splits; s++) {
-        const int64_t slot = ((int64_t)bh * a.splits + s) * a.rows + row;
-        const float2 x = ml[slot];
-        const float mt = fmaxf(m, x.x), mu = mt == -INFINITY ? 0.f : mt;
-        const float c0 = fast_exp2(m - mu), c1 = fast_exp2(x.x - mu);
-#pragma unroll
-        for (int i = 0; i < PER; i++) o[i] = o[i] * c0 + a.partial[slot * DH + 64 * i + lane] * c1;
-        l = l * c0 + x.y * c1;
+    for (int j = 0; j < PER; j++) o[j] = 0.f;
+    for (int x = w0; x <= w1; x += 64) {
+        const int n = w1 + 1 - x < 64 ? w1 + 1 - x : 64;
+        const float2 v = lane < n ? ml[slot0 + (int64_t)(x + lane) * a.rows] : make_float2(-INFINITY, 0.f);
+        const float mt = fmaxf(m, wave_max(v.x)), mu = mt == -INFINITY ? 0.f : mt;
+        const float c0 = fast_exp2(m - mu), weight = fast_exp2(v.x - mu);
+        l = l * c0 + wave_sum(v.y * weight);
         m = mt;
+#pragma unroll
+        for (int j = 0; j < PER; j++) o[j] *= c0;
+        const float* p = a.partial + (slot0 + (int64_t)x * a.rows) * DH + lane;
+        for (int i = 0; i < n; i += 4) {
+            float f[4][PER];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int j = 0; j < PER; j++) f[u][j] = i + u < n ? p[(int64_t)(i + u) * a.rows * DH + 64 * j] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), (i + u) & 63));
+#pragma unroll
+                for (int j = 0; j < PER; j++)
+                    if (i + u < n) o[j] = fmaf(f[u][j], c, o[j]);
+            }
+        }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     T* op = static_cast<T*>(a.out) + b * a.os[0] + tok * a.os[1] + head * a.os[2];
 #pragma unroll
-    for (int i = 0; i < PER; i++) op[64 * i + lane] = static_cast<T>(o[i] * inv);
+    for (int j = 0; j < PER; j++) op[64 * j + lane] = static_cast<T>(o[j] * inv);
 }
 
-template <typename T, int DH, int QW, int KW, bool UNAL>
+template <typename T, int DH, int QW, int KW, int WPE, bool UNAL>
 int launch_cfg(const CrossArgs& a, hipStream_t st) {
     const int rbs = (int)(((int64_t)a.rows + 32 * QW - 1) / (32 * QW));
-    const int64_t wgs = (int64_t)rbs * a.kv_heads * a.batch * a.splits;
-    const int64_t joins = ((int64_t)a.batch * a.kv_heads * a.rows + 3) / 4;
+    const int64_t wgs = (int64_t)rbs * a.kv_heads * (a.splits > 1 ? a.splits : a.batch);
+    const int64_t joins = (int64_t)a.batch * a.kv_heads * a.rows;
     if (wgs > 0x7fffffffL || joins > 0x7fffffffL) return -1;
-    cross_kernel<T, DH, QW, KW, UNAL><<<(unsigned)wgs, 64 * QW * KW, 0, st>>>(a, rbs);
-    if (a.splits > 1) cross_join_kernel<T, DH><<<(unsigned)joins, 256, 0, st>>>(a);
+    cross_kernel<T, DH, QW, KW, WPE, UNAL><<<(unsigned)wgs, 64 * QW * KW, 0, st>>>(a, rbs);
+    if (a.splits > 1) cross_join_kernel<T, DH><<<(unsigned)joins, 64, 0, st>>>(a);
     return 0;
 }
 
 }  // namespace
 
-int cross_splits(int dtype, int batch, int kv_heads, int rows, int seq_kv, int head_dim) {
-    const int64_t wgs = (int64_t)((rows + 63) / 64) * batch * kv_heads;
-    const int tiles = (seq_kv + 63) / 64;
-    int64_t n = 512 / wgs;
-    n = n < tiles / 4 ? n : tiles / 4;
-    return n < 2 ? 1 : (int)(n < 64 ? n : 64);
+// 64-row workgroups of a launch that does not split its keys.
+static int64_t row_groups(int batch, int kv_heads, int rows) { return ((int64_t)rows + 63) / 64 * kv_heads * batch; }
+
+// One workgroup a CU: at 1 x 16 heads x 1 x 16400 keys (bf16, 64-dim) 4 / 8 / 16 / 32 / 64 runs a head take 45 / 28 / 23 /
+// 25 / 31 us, unsplit 141; at 8 x 4 key heads x 1 x 8200 (128-dim) 16 / 32 / 64 take 72 / 43 / 33, unsplit 125.  A run
+// has two tiles at least, and the split has to save more than the joining kernel's 5 us: about 8 tiles of a
+// workgroup's time.
+int cross_splits(int batch, int kv_heads, int rows, int seq_kv) {
+    const int64_t tiles = (seq_kv + 63) / 64, per_batch = row_groups(1, kv_heads, rows);
+    int64_t n = 256 / per_batch;
+    n = n < batch * tiles / 2 ? n : batch * tiles / 2;
+    return n > batch && tiles * (n - batch) > 8 * n ? (int)n : 1;
 }
 
 template <typename T, int DH>
 int launch_cross(const CrossArgs& a, hipStream_t st) {
-    const int64_t es = sizeof(T);
+    constexpr int64_t es = sizeof(T);
+    constexpr bool F32 = sizeof(T) == 4;
     // Windows of a tile's rows stay below 2^31 bytes, and the buffer-to-LDS loads take dword-aligned rows.
     const bool unal = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 3) ||
                       ((a.ks[0] | a.ks[1] | a.ks[2] | a.vs[0] | a.vs[1] | a.vs[2]) * es & 3) ||
                       a.ks[1] * es > (1 << 24) || a.vs[1] * es > (1 << 24);
-    if (unal) return launch_cfg<T, DH, 2, 2, true>(a, st);
-    return launch_cfg<T, DH, 2, 2, false>(a, st);
+    constexpr int SMALL = DH == 64 ? 2 : 1;  // wavefronts per SIMD, of two (one) workgroups a CU
+    if (unal) return launch_cfg<T, DH, 2, 2, SMALL, true>(a, st);
+    // f32 in one block of 32 rows is bound by the matrix cores, most of whose rows are padding: a group on every SIMD
+    // (38 against 51 us at 8 x 4 key heads x 1 x 8200; at 128-dim the rings do not fit).
+    if constexpr (F32 && DH == 64) {
+        if (a.rows <= 32) return launch_cfg<T, DH, 1, 4, 1, false>(a, st);
+    }
+    // Where 64 rows a workgroup with two key groups take more than the one round that fits the chip, 128 rows
+    // with one: at 750 queries x 1381 keys x 16 heads (bf16, 64-dim) 21.4 against 27.1 us for 2 batch rows, 34.6 against
+    // 32.7 for 4, 59 against 47 for 8; 10 heads of 128 dimensions 26.9 / 39.4, 51.8 / 41.3 and 102 / 54.
+    if (a.splits > 1 || row_groups(a.batch, a.kv_heads, a.rows) <= 256 * SMALL) return launch_cfg<T, DH, 2, 2, SMALL, false>(a, st);
+    return launch_cfg<T, DH, 4, 1, DH == 64 && !F32 ? 3 : 2, false>(a, st);
 }
 
 template int launch_cross<bf16, 64>(const CrossArgs&, hipStream_t);
