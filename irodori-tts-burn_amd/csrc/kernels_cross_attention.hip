@@ -168,6 +168,16 @@ __device__ __forceinline__ TileWord tile_word(const uint8_t* mask, int len, int 
     return tw;
 }
 
+// s + a + b in f32.
+__device__ __forceinline__ float add_pair(bf16 a, bf16 b, float s) {
+    typedef bf16 P2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(P2{a, b}, P2{1.f, 1.f}, s, false);
+}
+__device__ __forceinline__ float add_pair(f16 a, f16 b, float s) {
+    typedef f16 P2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(P2{a, b}, P2{1.f, 1.f}, s, false);
+}
+
 // Keys of batch row b.
 __device__ __forceinline__ int row_keys(const CrossArgs& a, int b) {
     int n = a.seq_kv;
@@ -291,21 +301,14 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
         bool first = true;  // any lane's unset
 
         for (int t0 = t_begin; t0 < t_end; t0 += 64) {
-            const TileWord tw = tile_word<KT>(mb, len, t0, t_end, lane);
-            const int nact = tw.n, niter = (nact + KW - 1) / KW;
-            if (niter == 0) continue;  // the same for every wave
             wait_lds();
             raw_barrier();  // the rings may still be read
-            // This wave's share of the K and V tiles of step j into their ring slot.  Entries past the last
-            // are clamped to it, so every wave issues the same loads.
-            auto issue = [&](int j) {
-                int li = j * KW + tile;
-                li = li < nact ? li : nact - 1;
-                const int t = __builtin_amdgcn_readlane(tw.t, li);
+            // This wave's share of K and V tile t into ring slot `slot`.
+            auto load = [&](int t, int slot) {
                 const int left = len - t * KT, n = left < KT ? left : KT;  // rows of the tile
                 const T* ksrc = Kb + (int64_t)t * KT * a.ks[1];
                 const T* vsrc = Vb + (int64_t)t * KT * a.vs[1];
-                unsigned char* dst = smem + ((j & 1) * KW + tile) * TILE + part * 1024;
+                unsigned char* dst = smem + (slot * KW + tile) * TILE + part * 1024;
 #pragma unroll
                 for (int ii = 0; ii < LPW; ii++) {
                     if constexpr (UNAL) {
@@ -326,17 +329,37 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
                     }
                 }
             };
-            issue(0);
+            // Few rows: the first step's tiles are loaded under the mask's latency, on the guess that they hold a
+            // key (14.7 -> 13.7 us at 750 queries x 631 masked keys x 16 heads; many rows want the registers).
+            constexpr bool GUESS = KW > 1;
+            const int guess = t0 + tile < t_end ? t0 + tile : t_end - 1;
+            if (GUESS && mb) load(guess, 0);
+            const TileWord tw = tile_word<KT>(mb, len, t0, t_end, lane);
+            const int nact = tw.n, niter = (nact + KW - 1) / KW;
+            // The tile of step j that this wave has a share of; entries past the last are clamped to it, so
+            // every wave issues the same loads.
+            auto mine = [&](int j) {
+                const int li = j * KW + tile;
+                return li < nact ? li : nact - 1;
+            };
+            if (niter == 0) {  // the same for every wave
+                if (GUESS) wait_all();
+                continue;
+            }
+            if (!GUESS || !mb || __builtin_amdgcn_readlane(tw.t, mine(0)) != guess) {
+                if (GUESS && mb) wait_all();
+                load(__builtin_amdgcn_readlane(tw.t, mine(0)), 0);
+            }
             for (int j = 0; j < niter; j++) {
                 // This wave's loads of step j have landed; the masked rows among its V rows become zero (0 times
                 // a masked value's NaN or infinity would not be 0).
+                const int slot = j & 1;
                 wait_all();
                 if (mb) {
-                    int li = j * KW + tile;
-                    li = li < nact ? li : nact - 1;
+                    const int li = mine(j);
                     const unsigned lo = (unsigned)__builtin_amdgcn_readlane(tw.lo, li), hi = (unsigned)__builtin_amdgcn_readlane(tw.hi, li);
                     if ((KB == 2 ? lo & hi : lo) != 0xffffffffu) {
-                        unsigned char* dst = smem + VOFF + ((j & 1) * KW + tile) * TILE + part * 1024 + 16 * lane;
+                        unsigned char* dst = smem + VOFF + (slot * KW + tile) * TILE + part * 1024 + 16 * lane;
 #pragma unroll
                         for (int ii = 0; ii < LPW; ii++) {
                             const int r = (part + ii) * RPI + lane / CH;
@@ -346,10 +369,10 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
                     }
                 }
                 raw_barrier();
-                if (j + 1 < niter) issue(j + 1);
+                if (j + 1 < niter) load(__builtin_amdgcn_readlane(tw.t, mine(j + 1)), slot ^ 1);
+                const unsigned char* kt = smem + (slot * KW + kw) * TILE;
                 const int li = j * KW + kw;
                 if (li >= nact) continue;  // this group has no tile in the last step
-                const unsigned char* kt = smem + ((j & 1) * KW + kw) * TILE;
                 const unsigned char* vt = kt + VOFF;
                 f32x16 s[KB];
 #pragma unroll
@@ -397,17 +420,14 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
                             s[kb][e] = f(s[kb][e]);
                             const float p = fast_exp2(s[kb][e]);
                             pf[2 * kb + (e >> 3)][e & 7] = static_cast<T>(p);
-                            if (!std::is_same<T, bf16>::value) sum[e & 3] += p;
+                            if (sizeof(T) == 4) sum[e & 3] += p;
                         }
-                    if constexpr (std::is_same<T, bf16>::value) {
-                        // Two rounded elements an instruction (455 us where 32 additions take 470 at 32 x 750 x 4100
-                        // keys of 20 heads; f16's like instruction loses, 492).
-                        typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+                    if constexpr (sizeof(T) == 2) {
+                        // As the P V product takes them (so the weights add up to one), two an instruction.
 #pragma unroll
                         for (int g = 0; g < 2 * KB; g++)
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                sum[i] = __builtin_amdgcn_fdot2_f32_bf16(B2{pf[g][2 * i], pf[g][2 * i + 1]}, B2{1.f, 1.f}, sum[i], false);
+                            for (int i = 0; i < 4; i++) sum[i] = add_pair(pf[g][2 * i], pf[g][2 * i + 1], sum[i]);
                     }
                     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 };

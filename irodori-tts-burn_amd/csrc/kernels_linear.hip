@@ -121,9 +121,14 @@ __device__ __forceinline__ void load_cols(const T* p, int n, float (&f)[C]) {
     }
 }
 
-// Columns n .. n + C - 1 (those below N) of row m of Y from their sums.
+// Columns n .. n + C - 1 (those below N) of row m of the residual.
 template <typename TO, int C>
-__device__ __forceinline__ void finish(const LinearArgs& a, int m, int n, float (&v)[C]) {
+__device__ __forceinline__ void load_residual(const LinearArgs& a, int m, int n, float (&f)[C]) {
+    load_cols(static_cast<const TO*>(a.residual) + (int64_t)m * a.ldr + n, a.N - n, f);
+}
+// The same columns of Y from their sums, and from the residual's values where they are loaded already.
+template <typename TO, int C>
+__device__ __forceinline__ void finish(const LinearArgs& a, int m, int n, float (&v)[C], const float* residual = nullptr) {
     constexpr int E = C < 16 / (int)sizeof(TO) ? C : 16 / sizeof(TO);
     typedef TO OE __attribute__((ext_vector_type(E), aligned(sizeof(TO))));
     const int left = a.N - n;
@@ -140,9 +145,9 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int m, int n, float 
         for (int i = 0; i < C; i++) v[i] *= f[i];
     }
     if (a.residual) {
-        load_cols(static_cast<const TO*>(a.residual) + (int64_t)m * a.ldr + n, left, f);
+        if (!residual) load_residual<TO>(a, m, n, f);
 #pragma unroll
-        for (int i = 0; i < C; i++) v[i] += f[i];
+        for (int i = 0; i < C; i++) v[i] += residual ? residual[i] : f[i];
     }
     TO* y = static_cast<TO*>(a.y) + (int64_t)m * a.ldy + n;
     if (left >= C) {
@@ -280,6 +285,14 @@ void linear_kernel(LinearArgs a) {
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
 
+    // One block a wavefront: its residual comes under the products (11.6 -> 11.1 us at 1500 x 1024 x 1024).
+    constexpr bool EARLY = FM * FN == 1;
+    [[maybe_unused]] float early[16];
+    if constexpr (EARLY) {
+        const int m = m0 + wm * TM + fr, n = n0 + wn * TN + 16 * fh;
+        if (a.residual && wk == 0 && m < a.M && n < a.N) load_residual<TO>(a, m, n, early);
+    }
+
     // Two sets of fragments: a step's are read while the step before multiplies.  Before a slice's last
     // step the next slice is waited for and its first fragments read, so that the barrier's and the LDS's
     // latency hide behind that step; the slot that every wave has read by then is filled again.
@@ -405,7 +418,7 @@ void linear_kernel(LinearArgs a) {
             float v[16];
 #pragma unroll
             for (int e = 0; e < 16; e++) v[e] = acc[i][j][e];
-            finish<TO>(a, m, n, v);
+            finish<TO>(a, m, n, v, EARLY ? early : nullptr);
         }
     }
 }
@@ -524,16 +537,24 @@ int launch_tiles(const LinearArgs& a, hipStream_t st) {
 
 namespace {
 
-// The tiles a launch takes: of these, the one whose busiest CU is done first, by the microseconds of a
-// tile (f + a K) measured over M from 24 to 12 000 at N = 1024, 1280 and 5632, K = 1024 and 3680.  E.g. at
-// 1500 x 1024 x 1024 in bf16, 32 x 32 / 64 x 64 / 128 x 64 / 128 x 128 / 256 x 256 tiles take 13.6 / 9.8 / 10.0 /
-// 12.0 / 29.9 us, at 64 x 1024 x 1024 4.9 / 6.4 / 8.5 / 10.6 / 24.6, at 24000 x 5632 x 1024 the last two 345 / 322.
+// The tiles a launch takes: of these, the one whose busiest CU is done first, by the microseconds of a tile
+// (f + a K) measured over M from 32 to 12 000 at N = 333, 1024, 1280 and 5632, K = 512, 1024 and 3680.  Two tiles
+// on a CU overlap where they wait for memory (half: rounds count by halves); one alone may take longer than one of
+// many.  E.g. in bf16 with 32 x 32 / 64 x 64 / 128 x 64 / 128 x 128 / 256 x 256 tiles: 256 x 1024 x 1024 6.8 / 6.7 / 9.0 /
+// 11.3 / 29 us, 1500 x 1024 x 1024 13.0 / 8.5 / 9.5 / 11.8 / 30, 12000 x 5632 x 1024 436 / 262 / 207 / 168 / 183, 24000 x 5632
+// x 1024 the last two 345 / 322.
 struct TileCost {
     int bm, bn;
     float f, a;
+    bool half;
+    float alone;
 };
-constexpr TileCost kTiles16[] = {{32, 32, 0.25f, 0.0014f}, {64, 64, 0.35f, 0.0036f}, {128, 64, 0.3f, 0.006f}, {128, 128, 1.15f, 0.0085f}, {256, 256, 8.f, 0.0264f}};
-constexpr TileCost kTiles32[] = {{32, 32, 0.45f, 0.00425f}, {64, 64, 1.1f, 0.016f}, {128, 128, 4.5f, 0.059f}};
+constexpr TileCost kTiles16[] = {{32, 32, 0.25f, 0.0014f, false, 1.f},
+                                 {64, 64, 0.38f, 0.0036f, true, 1.f},
+                                 {128, 64, 0.3f, 0.006f, true, 1.f},
+                                 {128, 128, 1.15f, 0.0085f, false, 1.35f},
+                                 {256, 256, 8.f, 0.0264f, false, 1.f}};
+constexpr TileCost kTiles32[] = {{32, 32, 0.45f, 0.00425f, false, 1.f}, {64, 64, 0.7f, 0.0162f, false, 1.f}, {128, 128, 4.5f, 0.059f, false, 1.f}};
 template <int N>
 int best_tiles(const TileCost (&t)[N], const LinearArgs& a) {
     constexpr int CUS = 256;
@@ -541,7 +562,8 @@ int best_tiles(const TileCost (&t)[N], const LinearArgs& a) {
     double least = 0.;
     for (int i = 0; i < N; i++) {
         const int64_t n = ((int64_t)(a.M + t[i].bm - 1) / t[i].bm) * ((a.N + t[i].bn - 1) / t[i].bn);
-        const double c = (double)((n + CUS - 1) / CUS) * (t[i].f + t[i].a * a.K);
+        const double rounds = n <= CUS ? 1. : t[i].half ? (double)((2 * n + CUS - 1) / CUS) / 2. : (double)((n + CUS - 1) / CUS);
+        const double c = rounds * (t[i].f + t[i].a * a.K) * (n <= CUS ? t[i].alone : 1.f);
         if (i == 0 || c < least) {
             least = c;
             best = i;
@@ -554,7 +576,7 @@ int best_tiles(const TileCost (&t)[N], const LinearArgs& a) {
 
 template <typename T, typename TO>
 int launch_linear(const LinearArgs& a, hipStream_t st) {
-    // One new token or a few: 3.2 against 4.9 us with 32 x 32 tiles at 1 x 1024 x 512 (bf16).
+    // One new token or a few: 4.1 against 6.2 us with 32 x 32 tiles at 16 x 1024 x 1024 (bf16), 5.0 and 4.9 at 32 rows.
     if (a.M <= 16) return launch_rows<T, TO, 1, 8>(a, st);
     // The buffer-to-LDS loads take dword-aligned rows, and windows of a tile's rows below 2^31 bytes.
     constexpr int64_t ES = sizeof(T), FAR = (int64_t)1 << 22;
@@ -564,13 +586,13 @@ int launch_linear(const LinearArgs& a, hipStream_t st) {
     if constexpr (sizeof(T) == 4) {
         switch (best_tiles(kTiles32, a)) {
             case 0: return launch_tiles<T, TO, 32, 32, 1, 1, 4, 256, 2, true>(a, st);
-            case 1: return launch_tiles<T, TO, 64, 64, 2, 2, 2, 128, 4, true>(a, st);
+            case 1: return launch_tiles<T, TO, 64, 64, 2, 2, 2, 256, 2, true>(a, st);
             default: return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, true>(a, st);
         }
     } else {
         switch (best_tiles(kTiles16, a)) {
             case 0: return launch_tiles<T, TO, 32, 32, 1, 1, 4, 256, 3, true>(a, st);
-            case 1: return launch_tiles<T, TO, 64, 64, 2, 2, 2, 128, 4, true>(a, st);
+            case 1: return launch_tiles<T, TO, 64, 64, 2, 2, 2, 256, 2, true>(a, st);
             case 2: return launch_tiles<T, TO, 128, 64, 4, 2, 1, 128, 3, true>(a, st);
             case 3: return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, true>(a, st);
             default: return launch_tiles<T, TO, 256, 256, 2, 4, 1, 128, 2, true>(a, st);
