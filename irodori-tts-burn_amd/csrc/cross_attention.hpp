@@ -22,7 +22,7 @@ struct CrossArgs {
 };
 
 // Runs that the keys of a launch are split into (1: none), and the bytes of their partial results.
-int cross_splits(int batch, int kv_heads, int rows, int seq_kv);
+int cross_splits(bool f32, int batch, int kv_heads, int rows, int seq_kv, int head_dim);
 inline int64_t cross_partial_bytes(int splits, int batch, int kv_heads, int rows, int head_dim) {
     return splits > 1 ? ((int64_t)splits + batch) * kv_heads * rows * (head_dim + 2) * 4 : 0;
 }

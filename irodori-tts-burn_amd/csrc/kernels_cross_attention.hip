@@ -518,7 +518,7 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
 }
 
 // The runs' results of a row joined: a wavefront per row.  Lane i holds the weight exp2(m_i - M) of run i,
-// 64 at a time; a lane then sums DH / 64 dimensions, four runs' loads in flight.
+// 64 at a time; a lane then sums DH / 64 dimensions.
 template <typename T, int DH>
 __global__ __launch_bounds__(64) void cross_join_kernel(CrossArgs a) {
     const int lane = threadIdx.x;
@@ -548,6 +548,16 @@ __global__ __launch_bounds__(64) void cross_join_kernel(CrossArgs a) {
     for (int j = 0; j < PER; j++) o[j] = 0.f;
     for (int x = w0; x <= w1; x += 64) {
         const int n = w1 + 1 - x < 64 ? w1 + 1 - x : 64;
+        const float* p = a.partial + (slot0 + (int64_t)x * a.rows) * DH + lane;
+        constexpr int U = 8;  // runs in flight, the first of them with the weights
+        float f[U][PER];
+        auto load = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < PER; j++) f[u][j] = i + u < n ? p[(int64_t)(i + u) * a.rows * DH + 64 * j] : 0.f;
+        };
+        load(0);
         const float2 v = lane < n ? ml[slot0 + (int64_t)(x + lane) * a.rows] : make_float2(-INFINITY, 0.f);
         const float mt = fmaxf(m, wave_max(v.x)), mu = mt == -INFINITY ? 0.f : mt;
         const float c0 = fast_exp2(m - mu), weight = fast_exp2(v.x - mu);
@@ -555,15 +565,10 @@ __global__ __launch_bounds__(64) void cross_join_kernel(CrossArgs a) {
         m = mt;
 #pragma unroll
         for (int j = 0; j < PER; j++) o[j] *= c0;
-        const float* p = a.partial + (slot0 + (int64_t)x * a.rows) * DH + lane;
-        for (int i = 0; i < n; i += 4) {
-            float f[4][PER];
+        for (int i = 0; i < n; i += U) {
+            if (i > 0) load(i);
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-#pragma unroll
-                for (int j = 0; j < PER; j++) f[u][j] = i + u < n ? p[(int64_t)(i + u) * a.rows * DH + 64 * j] : 0.f;
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
+            for (int u = 0; u < U; u++) {
                 const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), (i + u) & 63));
 #pragma unroll
                 for (int j = 0; j < PER; j++)
@@ -593,13 +598,13 @@ int launch_cfg(const CrossArgs& a, hipStream_t st) {
 // 64-row workgroups of a launch that does not split its keys.
 static int64_t row_groups(int batch, int kv_heads, int rows) { return ((int64_t)rows + 63) / 64 * kv_heads * batch; }
 
-// One workgroup a CU: at 1 x 16 heads x 1 x 16400 keys (bf16, 64-dim) 4 / 8 / 16 / 32 / 64 runs a head take 45 / 28 / 23 /
-// 25 / 31 us, unsplit 141; at 8 x 4 key heads x 1 x 8200 (128-dim) 16 / 32 / 64 take 72 / 43 / 33, unsplit 125.  A run
-// has two tiles at least, and the split has to save more than the joining kernel's 5 us: about 8 tiles of a
-// workgroup's time.
-int cross_splits(int batch, int kv_heads, int rows, int seq_kv) {
+// As many workgroups as run at once: at 1 x 16 heads x 1 x 16400 keys (bf16, 64-dim) 4 / 8 / 16 / 32 / 64 runs a head
+// take 45 / 28 / 23 / 25 / 31 us, unsplit 141; at 8 x 4 key heads x 1 x 8200 ragged keys (128-dim) 64 / 96 / 128 / 192 take
+// 30.6 / 27.3 / 27.2 / 34.3, unsplit 125.  A run has two tiles at least, and the split has to save more than the
+// joining kernel's 5 us: about 8 tiles of a workgroup's time.
+int cross_splits(bool f32, int batch, int kv_heads, int rows, int seq_kv, int head_dim) {
     const int64_t tiles = (seq_kv + 63) / 64, per_batch = row_groups(1, kv_heads, rows);
-    int64_t n = 256 / per_batch;
+    int64_t n = (head_dim == 128 && !f32 ? 512 : 256) / per_batch;
     n = n < batch * tiles / 2 ? n : batch * tiles / 2;
     return n > batch && tiles * (n - batch) > 8 * n ? (int)n : 1;
 }
@@ -618,6 +623,11 @@ int launch_cross(const CrossArgs& a, hipStream_t st) {
     // (38 against 51 us at 8 x 4 key heads x 1 x 8200; at 128-dim the rings do not fit).
     if constexpr (F32 && DH == 64) {
         if (a.rows <= 32) return launch_cfg<T, DH, 1, 4, 1, false>(a, st);
+    }
+    // Runs of 128-dim heads in two workgroups a CU, which hide each other's ends, rather than one with two
+    // key groups (27.2 against 30.0 us at 8 x 4 key heads x 1 x 8200; 64-dim heads fit two a CU either way).
+    if constexpr (!F32 && DH == 128) {
+        if (a.splits > 1) return launch_cfg<T, DH, 2, 1, 1, false>(a, st);
     }
     // Where 64 rows a workgroup with two key groups take more than the one round that fits the chip, 128 rows
     // with one: at 750 queries x 1381 keys x 16 heads (bf16, 64-dim) 21.4 against 27.1 us for 2 batch rows, 34.6 against

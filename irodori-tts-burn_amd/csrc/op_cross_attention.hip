@@ -30,7 +30,8 @@ int check_cross(const irodori_cross_attention_desc* dp) {
 }
 
 int splits_of(const irodori_cross_attention_desc& d) {
-    return cross_splits(d.batch, d.kv_heads, d.seq_q * (d.heads / d.kv_heads), d.seq_kv);
+    return cross_splits(d.dtype == IRODORI_DTYPE_F32, d.batch, d.kv_heads, d.seq_q * (d.heads / d.kv_heads), d.seq_kv,
+                        d.head_dim);
 }
 int64_t bytes_of(const irodori_cross_attention_desc& d, int splits) {
     return cross_partial_bytes(splits, d.batch, d.kv_heads, d.seq_q * (d.heads / d.kv_heads), d.head_dim);
