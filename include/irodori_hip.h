@@ -508,7 +508,7 @@ int irodori_op_gemm_fp8(const uint8_t* a, const uint8_t* a_scale, const uint8_t*
 #define IRODORI_ROPE_BY_PARTS 3
 typedef struct irodori_rope_desc {
     int32_t dtype;
-    int32_t batch, seq;
+    int32_t batch, seq;  /* seq <= 2^30 */
     int32_t head_dim;    /* even, <= 1024 */
     int32_t rot_dim;     /* even, 2 .. min(head_dim, 512) */
     int32_t q_heads, k_heads;          /* either may be 0; at most 16384 */
@@ -541,7 +541,7 @@ int irodori_op_rope(const irodori_rope_desc* desc, const void* q, void* q_out, c
 #define IRODORI_ACT_GELU_TANH 6 /* its tanh approximation */
 typedef struct irodori_linear_desc {
     int32_t dtype, out_dtype;
-    int32_t m, n, k;
+    int32_t m, n, k;             /* at most 2^28 */
     int32_t activation;
     int32_t gate_rows;           /* rows that share a row of the gate; 0 without one */
     int32_t reserved;
@@ -565,7 +565,7 @@ int irodori_op_linear(const irodori_linear_desc* desc, const void* x, const void
  * many keys are split over the keys and joined in f32, through the workspace. */
 typedef struct irodori_cross_attention_desc {
     int32_t dtype;
-    int32_t batch, seq_q, seq_kv;
+    int32_t batch, seq_q, seq_kv; /* seq_q * heads / kv_heads <= 2^28, seq_kv <= 2^29 */
     int32_t heads, kv_heads;     /* heads a multiple of kv_heads */
     int32_t head_dim;
     float scale;

@@ -235,9 +235,9 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
         hk = id % a.kv_heads;
         b = id / a.kv_heads;
     }
-    // c = 0 would turn a masked key's -inf into NaN; a tiny c gives the same exp2(0).
+    // c = 0 would turn a masked key's -inf into NaN; the smallest normal gives the same exp2(0).
     float c = a.scale * 1.4426950408889634f;
-    c = c == 0.f ? 1e-38f : c;
+    c = fabsf(c) < 1.1754944e-38f ? 1.1754944e-38f : c;
     const unsigned masked = __builtin_bit_cast(unsigned, c > 0.f ? -INFINITY : INFINITY);
     // Load instruction ii of this wave in a stage: rows RPI (row0 + ii) .. of tile `tile` of the step's;
     // lane -> row lane / CH, physical chunk lane % CH.
@@ -558,9 +558,13 @@ __global__ __launch_bounds__(64) void cross_join_kernel(CrossArgs a) {
                 for (int j = 0; j < PER; j++) f[u][j] = i + u < n ? p[(int64_t)(i + u) * a.rows * DH + 64 * j] : 0.f;
         };
         load(0);
-        const float2 v = lane < n ? ml[slot0 + (int64_t)(x + lane) * a.rows] : make_float2(-INFINITY, 0.f);
+        // (Where the batch has fewer tiles than runs, some runs are empty and wrote nothing.)
+        const int64_t w = x + lane;
+        const bool wrote = lane < n && all * w / a.splits < all * (w + 1) / a.splits;
+        const float2 v = wrote ? ml[slot0 + w * a.rows] : make_float2(-INFINITY, 0.f);
         const float mt = fmaxf(m, wave_max(v.x)), mu = mt == -INFINITY ? 0.f : mt;
-        const float c0 = fast_exp2(m - mu), weight = fast_exp2(v.x - mu);
+        const float c0 = fast_exp2(m - mu), weight = wrote ? fast_exp2(v.x - mu) : 0.f;
+        const unsigned long long there = __ballot(wrote);
         l = l * c0 + wave_sum(v.y * weight);
         m = mt;
 #pragma unroll
@@ -572,7 +576,7 @@ __global__ __launch_bounds__(64) void cross_join_kernel(CrossArgs a) {
                 const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), (i + u) & 63));
 #pragma unroll
                 for (int j = 0; j < PER; j++)
-                    if (i + u < n) o[j] = fmaf(f[u][j], c, o[j]);
+                    if (i + u < n && (there >> (i + u) & 1)) o[j] = fmaf(f[u][j], c, o[j]);
             }
         }
     }

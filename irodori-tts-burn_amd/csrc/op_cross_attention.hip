@@ -17,9 +17,9 @@ int check_cross(const irodori_cross_attention_desc* dp) {
     IRO_REQUIRE(d.head_dim == 64 || d.head_dim == 128, IRODORI_ERR_SHAPE,
                 "irodori_op_cross_attention: head_dim must be 64 or 128");
     IRO_REQUIRE(d.heads % d.kv_heads == 0, IRODORI_ERR_SHAPE, "irodori_op_cross_attention: heads must be a multiple of kv_heads");
-    IRO_REQUIRE((int64_t)d.seq_q * (d.heads / d.kv_heads) <= 1 << 28 && d.seq_kv <= 1 << 30, IRODORI_ERR_SHAPE,
-                "irodori_op_cross_attention: more than 2^28 rows of a key head or 2^30 keys");
-    IRO_REQUIRE(std::isfinite(d.scale), IRODORI_ERR_CONFIG, "irodori_op_cross_attention: scale must be finite");
+    IRO_REQUIRE((int64_t)d.seq_q * (d.heads / d.kv_heads) <= 1 << 28 && d.seq_kv <= 1 << 29, IRODORI_ERR_SHAPE,
+                "irodori_op_cross_attention: more than 2^28 rows of a key head or 2^29 keys");
+    IRO_REQUIRE(std::fabs(d.scale) <= 1e38f, IRODORI_ERR_CONFIG, "irodori_op_cross_attention: scale must be at most 1e38 in magnitude");
     const int64_t qn[3] = {d.batch, d.seq_q, d.heads}, kn[3] = {d.batch, d.seq_kv, d.kv_heads};
     IRO_REQUIRE(strides_readable(qn, d.q_strides) && strides_readable(kn, d.k_strides) && strides_readable(kn, d.v_strides),
                 IRODORI_ERR_SHAPE, "irodori_op_cross_attention: a negative or too large stride");

@@ -155,8 +155,10 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     }
 }
 
-// Turns per position of each pair: theta^(-2p / rot) / 2 pi, scaled.
-void make_turns(const irodori_rope_desc& d, double* turns) {
+// Turns per position of each pair: theta^(-2p / rot) / 2 pi, scaled.  False where one is not a number below
+// kMaxTurns (2^31 positions of it still have 2^-2 of a turn's precision in float64).
+constexpr double kMaxTurns = 1048576.;
+bool make_turns(const irodori_rope_desc& d, double* turns) {
     const int n = d.rot_dim / 2;
     double theta = d.theta;
     if (d.scaling == IRODORI_ROPE_NTK) theta *= std::pow(d.factor, d.rot_dim / (d.rot_dim - 2.0));
@@ -171,8 +173,10 @@ void make_turns(const irodori_rope_desc& d, double* turns) {
             const double keep = std::min(1.0, std::max(0.0, (whole - d.beta_slow) / (d.beta_fast - d.beta_slow)));
             t *= keep + (1.0 - keep) / d.factor;
         }
+        if (!(t < kMaxTurns)) return false;
         turns[p] = t;
     }
+    return true;
 }
 
 int check_side(const irodori_rope_desc& d, const char* name, const void* x, const void* y, int heads, int rot_heads,
@@ -208,7 +212,7 @@ int check_rope(const irodori_rope_desc* dp) {
     IRO_REQUIRE(d.layout == IRODORI_ROPE_INTERLEAVED || d.layout == IRODORI_ROPE_HALVES, IRODORI_ERR_CONFIG,
                 "irodori_op_rope: unknown layout");
     IRO_REQUIRE(std::isfinite(d.theta) && d.theta > 0, IRODORI_ERR_CONFIG, "irodori_op_rope: theta must be positive");
-    IRO_REQUIRE(std::isfinite(d.amplitude), IRODORI_ERR_CONFIG, "irodori_op_rope: amplitude must be finite");
+    IRO_REQUIRE(std::fabs(d.amplitude) <= 1e38, IRODORI_ERR_CONFIG, "irodori_op_rope: amplitude must be at most 1e38 in magnitude");
     IRO_REQUIRE(d.scaling >= IRODORI_ROPE_UNSCALED && d.scaling <= IRODORI_ROPE_BY_PARTS, IRODORI_ERR_CONFIG,
                 "irodori_op_rope: unknown scaling");
     if (d.scaling != IRODORI_ROPE_UNSCALED)
@@ -220,7 +224,8 @@ int check_rope(const irodori_rope_desc* dp) {
                         std::isfinite(d.beta_fast) && d.beta_fast > d.beta_slow,
                     IRODORI_ERR_CONFIG,
                     "irodori_op_rope: scaling by parts needs a positive trained_len and beta_fast above beta_slow");
-    IRO_REQUIRE(d.first_pos <= INT32_MAX - d.seq, IRODORI_ERR_SHAPE, "irodori_op_rope: positions past 2^31");
+    IRO_REQUIRE(d.seq <= 1 << 30 && d.first_pos <= INT32_MAX - d.seq, IRODORI_ERR_SHAPE,
+                "irodori_op_rope: more than 2^30 tokens, or positions past 2^31");
     return IRODORI_OK;
 }
 
@@ -275,8 +280,6 @@ int irodori_op_rope(const irodori_rope_desc* desc, const void* q, void* q_out, c
     IRO_REQUIRE(d.head_dim % 2 == 0, IRODORI_ERR_SHAPE, "irodori_op_rope: head_dim must be even");
     IRO_REQUIRE(aligned_to(positions, 4) && aligned_to(lengths, 4), IRODORI_ERR_INVALID_ARG,
                 "irodori_op_rope: positions or lengths are not aligned");
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    IRO_TRY(check_op_stream(st, "irodori_op_rope"));
     RopeArgs a;
     auto side = [](const void* x, void* y, const int64_t* xs, const int64_t* ys, int heads, int rot) {
         return RopeSide{x, y, {xs[0], xs[1], xs[2]}, {ys[0], ys[1], ys[2]}, heads, rot};
@@ -291,7 +294,9 @@ int irodori_op_rope(const irodori_rope_desc* desc, const void* q, void* q_out, c
     a.pairs = d.rot_dim / 2;
     a.amplitude = (float)d.amplitude;
     a.sin_sign = d.inverse ? -1.f : 1.f;
-    make_turns(d, a.turns);
+    IRO_REQUIRE(make_turns(d, a.turns), IRODORI_ERR_CONFIG, "irodori_op_rope: theta and the scaling give a frequency that is too large");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    IRO_TRY(check_op_stream(st, "irodori_op_rope"));
     if (d.dtype == IRODORI_DTYPE_BF16) return launch_width<bf16>(d, a, st);
     if (d.dtype == IRODORI_DTYPE_F16) return launch_width<f16>(d, a, st);
     return launch_width<float>(d, a, st);

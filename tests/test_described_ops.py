@@ -56,11 +56,12 @@ def test_description_sizes_match_the_header():
     (dict(rot_dim=0), "Shape", "rot_dim"), (dict(rot_dim=63), "Shape", "rot_dim"), (dict(rot_dim=66), "Shape", "rot_dim"),
     (dict(head_dim=1024, rot_dim=514), "Shape", "rot_dim"), (dict(rot_heads=5), "Shape", "rot_heads"),
     (dict(rot_kv_heads=-1), "Shape", "rot_heads"), (dict(theta=0.0), "Config", "theta"), (dict(theta=float("nan")), "Config", "theta"),
-    (dict(amplitude=float("inf")), "Config", "amplitude"), (dict(scaling="linear", factor=0.0), "Config", "factor"),
+    (dict(amplitude=float("inf")), "Config", "amplitude"), (dict(amplitude=-1e300), "Config", "amplitude"),
+    (dict(scaling="linear", factor=1e-30), "Config", "frequency"), (dict(theta=1e-300), "Config", "frequency"), (dict(scaling="linear", factor=0.0), "Config", "factor"),
     (dict(scaling="ntk", factor=2.0, rot_dim=2), "Config", "rot_dim"),
     (dict(scaling="by_parts", factor=2.0), "Config", "trained_len"),
     (dict(scaling="by_parts", factor=2.0, trained_len=100.0, beta_fast=1.0), "Config", "beta_fast"),
-    (dict(first_pos=2 ** 31 - 3), "Shape", "2^31"),
+    (dict(first_pos=2 ** 31 - 3), "Shape", "2^31"), (dict(seq=2 ** 30 + 1), "Shape", "2^30"),
     (dict(q_strides=(-1, 256, 64)), "Shape", "stride"), (dict(k_out_strides=(640, 128, 32)), "Shape", "overlap"),
     (dict(q_out_strides=(0, 256, 64)), "Shape", "overlap"),
 ])
@@ -114,8 +115,8 @@ def test_linear_refuses_pointers_and_codes():
 @pytest.mark.parametrize("kw,kind,text", [
     (dict(batch=0), "Shape", "positive"), (dict(seq_q=0), "Shape", "positive"), (dict(seq_kv=0), "Shape", "positive"),
     (dict(heads=3), "Shape", "multiple"), (dict(kv_heads=0), "Shape", "positive"), (dict(head_dim=96), "Shape", "head_dim"),
-    (dict(scale=float("nan")), "Config", "scale"), (dict(seq_q=2 ** 28, heads=4, kv_heads=2), "Shape", "2^28"),
-    (dict(seq_kv=2 ** 30 + 1), "Shape", "2^30"), (dict(k_strides=(-64, 128, 64)), "Shape", "stride"),
+    (dict(scale=float("nan")), "Config", "scale"), (dict(scale=-3e38), "Config", "scale"), (dict(seq_q=2 ** 28, heads=4, kv_heads=2), "Shape", "2^28"),
+    (dict(seq_kv=2 ** 29 + 1), "Shape", "2^29"), (dict(k_strides=(-64, 128, 64)), "Shape", "stride"),
     (dict(out_strides=(768, 256, 63)), "Shape", "overlap"), (dict(mask_stride=-1), "Shape", "mask_stride"),
 ])
 def test_cross_attention_refusals(kw, kind, text):

@@ -360,6 +360,28 @@ def test_cross_attention_lengths_masks_and_what_they_hide(dtype, sq):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens", [[1], [130], [0, 3, 0], [5000, 1, 0, 700, 64], [0] * 70 + [200] + [0] * 9 + [4999, 1], [65] * 90])
+def test_cross_attention_split_over_short_rows(dtype, d, lens):
+    """A description of many keys, split, of which the rows hold few: runs that are empty, that end
+    inside a row and that span several; more rows than a wavefront has lanes."""
+    b, sq, skv, h, hk = len(lens), 2, 5000, 4, 2
+    desc = ih.CrossAttentionDesc(b, sq, skv, h, hk, d, dtype=dtype)
+    assert ih.ops.cross_attention_workspace(desc) > 0
+    q = randn(1, b, sq, h, d, dtype=dtype)
+    k, v = (randn(i, 1, skv, hk, d, dtype=dtype).expand(b, skv, hk, d) for i in (2, 3))  # (one set of states)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    mask = (torch.rand(b, skv, generator=torch.Generator().manual_seed(3)) < 0.5).to(torch.uint8).cuda()
+    q_len = torch.tensor([i % 3 for i in range(b)], dtype=torch.int32, device="cuda")
+    for kw in (dict(), dict(mask=mask, q_len=q_len)):
+        out = torch.full((b, sq, h, d), CANARY, dtype=TYPE[dtype], device="cuda")
+        run_cross(q, k, v, out, dtype, kv_len=n, **kw)
+        check_cross(out, q, k, v, dtype, kv_len=n, **kw)
+        for i in range(b):
+            assert (out[i, int(q_len[i]) if kw else sq:] == CANARY).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("pad,offset", [(2, 0), (1, 1), (3, 0)])
 def test_cross_attention_strides_and_alignment(dtype, d, pad, offset):
     b, sq, skv, h, hk = 2, 40, 150, 4, 2
@@ -397,7 +419,7 @@ def test_cross_attention_scores_that_grow(dtype, sq, skv):
     out = torch.empty(b, sq, h, d, dtype=TYPE[dtype], device="cuda")
     run_cross(q, k, v, out, dtype, scale=0.5)
     check_cross(out, q, k, v, dtype, scale=0.5)
-    for scale in (0.0, -0.5, 2.0 ** -10, 15.0):
+    for scale in (0.0, -0.5, 2.0 ** -10, 15.0, 1e-42):
         run_cross(q, k, v, out, dtype, scale=scale)
         check_cross(out, q, k, v, dtype, scale=scale, what="scale %g" % scale)
 
@@ -556,3 +578,56 @@ def test_half_block_captured_and_on_another_stream(dtype):
         other(c, states, kv_len)
     torch.cuda.synchronize()
     assert torch.equal(a, want) and torch.equal(c, want)
+
+
+CHILD = """
+import torch
+import irodori_hip as ih
+
+def captured(name, call, *outs):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(torch.cuda.current_stream().cuda_stream)
+    got = []
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        got.append([o.clone() for o in outs])
+    for o in outs:
+        o.zero_()
+    call(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    for rep in got:
+        for a, o in zip(rep, outs):
+            assert o.float().abs().sum() > 0 and torch.equal(a, o), name
+    print(name, flush=True)
+
+t = lambda *s: torch.randn(*s, device="cuda").to(torch.bfloat16)
+for m, n, k in ((3, 64, 64), (40, 64, 64), (600, 512, 128), (12000, 5632, 1024), (40, 64, 33)):
+    x, w, y = t(m, k), t(n, k), t(m, n)
+    d = ih.LinearDesc(m, n, k)
+    captured("linear %d" % m, lambda s: ih.ops.linear(d, x.data_ptr(), w.data_ptr(), y.data_ptr(), stream=s), y)
+q, qo = t(2, 9, 4, 64), t(2, 9, 4, 64)
+rd = ih.RopeDesc(2, 9, 64, heads=4)
+captured("rope", lambda s: ih.ops.rope(rd, q.data_ptr(), qo.data_ptr(), stream=s), qo)
+for sq, skv, dim in ((1, 9000, 128), (70, 90, 128), (2000, 90, 128), (1, 9000, 64), (9000, 90, 64)):
+    q, o, kv = t(1, sq, 8, dim), t(1, sq, 8, dim), t(1, skv, 8, dim)
+    cd = ih.CrossAttentionDesc(1, sq, skv, 8, 8, dim)
+    nb = ih.ops.cross_attention_workspace(cd)
+    ws = torch.empty(max(nb, 1), dtype=torch.uint8, device="cuda")
+    captured("cross %d %d" % (sq, dim), lambda s: ih.ops.cross_attention(cd, q.data_ptr(), kv.data_ptr(), kv.data_ptr(), o.data_ptr(),
+             d_workspace=ws.data_ptr(), workspace_bytes=nb, stream=s), o)
+print("captures ok")
+"""
+
+
+def test_first_calls_may_be_captured():
+    # A fresh process, whose first call of each kernel is under capture.
+    import os
+    import subprocess
+    import sys
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(ih.__file__)))
+    r = subprocess.run([sys.executable, "-W", "ignore", "-c", CHILD], env=env, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "captures ok" in r.stdout, r.stdout + r.stderr
