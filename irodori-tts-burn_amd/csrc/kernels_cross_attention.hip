@@ -12,7 +12,7 @@
 //                    matrix core's operand; its rounding averages out over the keys as V's own does);
 //                    V^T comes from the row-major tile, 16-bit by the transposing LDS read.
 // A tile that the mask empties is never loaded; in a tile that it thins, the masked scores are -inf and
-// the masked values zero, whatever their memory holds.
+// the masked values, which are not loaded, zero.
 #include <type_traits>
 
 #include "attn_util.hpp"
@@ -168,6 +168,11 @@ __device__ __forceinline__ TileWord tile_word(const uint8_t* mask, int len, int 
     return tw;
 }
 
+// a where on is all ones, b where it is 0: one instruction (the expression itself becomes a compare and a select).
+__device__ __forceinline__ float bit_select(int on, float a, float b) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_bitop3_b32((unsigned)on, __builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b),
+                                                                 0xCA));
+}
 // s + a + b in f32.
 __device__ __forceinline__ float add_pair(bf16 a, bf16 b, float s) {
     typedef bf16 P2 __attribute__((ext_vector_type(2)));
@@ -238,7 +243,7 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
     // c = 0 would turn a masked key's -inf into NaN; the smallest normal gives the same exp2(0).
     float c = a.scale * 1.4426950408889634f;
     c = fabsf(c) < 1.1754944e-38f ? 1.1754944e-38f : c;
-    const unsigned masked = __builtin_bit_cast(unsigned, c > 0.f ? -INFINITY : INFINITY);
+    const float masked = c > 0.f ? -INFINITY : INFINITY;  // the score that vanishes
     // Load instruction ii of this wave in a stage: rows RPI (row0 + ii) .. of tile `tile` of the step's;
     // lane -> row lane / CH, physical chunk lane % CH.
     const int tile = wave * LPW / NI, part = wave * LPW % NI;
@@ -303,73 +308,62 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
         for (int t0 = t_begin; t0 < t_end; t0 += 64) {
             wait_lds();
             raw_barrier();  // the rings may still be read
-            // This wave's share of K and V tile t into ring slot `slot`.
-            auto load = [&](int t, int slot) {
+            // This wave's share of K tile t, and of V tile t without its masked rows (0 times a masked value's NaN or
+            // infinity would not be 0), into ring slot `slot`.  Rows past the last key and those left out read as zero.
+            auto load = [&](const T* base, const int64_t token, const unsigned (&vo)[LPW], int off, int t, int slot, auto kept) {
                 const int left = len - t * KT, n = left < KT ? left : KT;  // rows of the tile
-                const T* ksrc = Kb + (int64_t)t * KT * a.ks[1];
-                const T* vsrc = Vb + (int64_t)t * KT * a.vs[1];
-                unsigned char* dst = smem + (slot * KW + tile) * TILE + part * 1024;
+                const T* src = base + (int64_t)t * KT * token;
+                unsigned char* dst = smem + off + (slot * KW + tile) * TILE + part * 1024;
 #pragma unroll
                 for (int ii = 0; ii < LPW; ii++) {
+                    const int r = (part + ii) * RPI + lane / CH;
                     if constexpr (UNAL) {
                         typedef T E16 __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-                        constexpr int PE = 16 / (int)sizeof(T);
-                        const int r = (part + ii) * RPI + lane / CH;
-                        u32x4 kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
-                        if (r < n) {
-                            kx = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(ksrc + r * a.ks[1] + kswz<ROWB>(r, lane % CH) * PE));
-                            vx = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(vsrc + r * a.vs[1] + vswz<T, ROWB>(r, lane % CH) * PE));
-                        }
-                        *reinterpret_cast<u32x4*>(dst + ii * 1024 + 16 * lane) = kx;
-                        *reinterpret_cast<u32x4*>(dst + VOFF + ii * 1024 + 16 * lane) = vx;
+                        u32x4 x = {0, 0, 0, 0};
+                        if (r < n && kept(r)) x = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(src + vo[ii] / sizeof(T)));
+                        *reinterpret_cast<u32x4*>(dst + ii * 1024 + 16 * lane) = x;
                     } else {
-                        // Rows past the last key read as zero.
-                        buf_load_lds16(make_rsrc(ksrc, (unsigned)((n - 1) * a.ks[1] * (int)sizeof(T)) + ROWB), voK[ii], dst + ii * 1024);
-                        buf_load_lds16(make_rsrc(vsrc, (unsigned)((n - 1) * a.vs[1] * (int)sizeof(T)) + ROWB), voV[ii], dst + VOFF + ii * 1024);
+                        buf_load_lds16(make_rsrc(src, (unsigned)((n - 1) * token * (int)sizeof(T)) + ROWB), kept(r) ? vo[ii] : 0x80000000u,
+                                       dst + ii * 1024);
                     }
                 }
             };
-            // Few rows: the first step's tiles are loaded under the mask's latency, on the guess that they hold a
-            // key (14.7 -> 13.7 us at 750 queries x 631 masked keys x 16 heads; many rows want the registers).
+            auto load_k = [&](int t, int slot) { load(Kb, a.ks[1], voK, 0, t, slot, [](int) { return true; }); };
+            auto load_v = [&](int t, int slot, unsigned lo, unsigned hi) {
+                load(Vb, a.vs[1], voV, VOFF, t, slot, [&](int r) { return !mb || (((r < 32 ? lo : hi) >> (r & 31)) & 1u); });
+            };
+            // Few rows: the first step's K is loaded under the mask's latency, on the guess that its tiles hold a
+            // key (many rows want the registers).
             constexpr bool GUESS = KW > 1;
             const int guess = t0 + tile < t_end ? t0 + tile : t_end - 1;
-            if (GUESS && mb) load(guess, 0);
+            if (GUESS && mb) load_k(guess, 0);
             const TileWord tw = tile_word<KT>(mb, len, t0, t_end, lane);
             const int nact = tw.n, niter = (nact + KW - 1) / KW;
-            // The tile of step j that this wave has a share of; entries past the last are clamped to it, so
-            // every wave issues the same loads.
-            auto mine = [&](int j) {
-                const int li = j * KW + tile;
-                return li < nact ? li : nact - 1;
-            };
             if (niter == 0) {  // the same for every wave
                 if (GUESS) wait_all();
                 continue;
             }
-            if (!GUESS || !mb || __builtin_amdgcn_readlane(tw.t, mine(0)) != guess) {
-                if (GUESS && mb) wait_all();
-                load(__builtin_amdgcn_readlane(tw.t, mine(0)), 0);
+            // Step j's tile that this wave has a share of; entries past the last are clamped to it, so every
+            // wave issues the same loads.
+            auto load_step = [&](int j, int slot, bool k) {
+                int li = j * KW + tile;
+                li = li < nact ? li : nact - 1;
+                const int t = __builtin_amdgcn_readlane(tw.t, li);
+                if (k) load_k(t, slot);
+                load_v(t, slot, (unsigned)__builtin_amdgcn_readlane(tw.lo, li), (unsigned)__builtin_amdgcn_readlane(tw.hi, li));
+            };
+            bool guessed = false;
+            if (GUESS && mb) {
+                guessed = __builtin_amdgcn_readlane(tw.t, tile < nact ? tile : nact - 1) == guess;
+                if (!guessed) wait_all();
             }
+            load_step(0, 0, !guessed);
             for (int j = 0; j < niter; j++) {
-                // This wave's loads of step j have landed; the masked rows among its V rows become zero (0 times
-                // a masked value's NaN or infinity would not be 0).
+                // This wave's loads of step j have landed, and its reads of the slot refilled next are done.
                 const int slot = j & 1;
                 wait_all();
-                if (mb) {
-                    const int li = mine(j);
-                    const unsigned lo = (unsigned)__builtin_amdgcn_readlane(tw.lo, li), hi = (unsigned)__builtin_amdgcn_readlane(tw.hi, li);
-                    if ((KB == 2 ? lo & hi : lo) != 0xffffffffu) {
-                        unsigned char* dst = smem + VOFF + (slot * KW + tile) * TILE + part * 1024 + 16 * lane;
-#pragma unroll
-                        for (int ii = 0; ii < LPW; ii++) {
-                            const int r = (part + ii) * RPI + lane / CH;
-                            if (!(((r < 32 ? lo : hi) >> (r & 31)) & 1u)) *reinterpret_cast<u32x4*>(dst + ii * 1024) = u32x4{0, 0, 0, 0};
-                        }
-                        wait_lds();
-                    }
-                }
                 raw_barrier();
-                if (j + 1 < niter) load(__builtin_amdgcn_readlane(tw.t, mine(j + 1)), slot ^ 1);
+                if (j + 1 < niter) load_step(j + 1, slot ^ 1, true);
                 const unsigned char* kt = smem + (slot * KW + kw) * TILE;
                 const int li = j * KW + kw;
                 if (li >= nact) continue;  // this group has no tile in the last step
@@ -385,9 +379,7 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
                         const int wd = (int)(word[kb] >> (4 * fh));
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            const unsigned on = (unsigned)__builtin_amdgcn_sbfe(wd, 8 * (e >> 2) + (e & 3), 1);  // all ones or none
-                            const float x = s[kb][e];  // (a bit_cast of the vector's element itself takes element 0)
-                            s[kb][e] = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, x) & on) | (masked & ~on));
+                            s[kb][e] = bit_select(__builtin_amdgcn_sbfe(wd, 8 * (e >> 2) + (e & 3), 1), s[kb][e], masked);
                         }
                     }
                 }
