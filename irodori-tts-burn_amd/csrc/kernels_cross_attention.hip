@@ -592,7 +592,7 @@ int launch_cfg(const CrossArgs& a, hipStream_t st) {
     const int rbs = (int)(((int64_t)a.rows + 32 * QW - 1) / (32 * QW));
     const int64_t wgs = (int64_t)rbs * a.kv_heads * (a.splits > 1 ? a.splits : a.batch);
     const int64_t joins = (int64_t)a.batch * a.kv_heads * a.rows;
-    if (wgs > 0x7fffffffL || joins > 0x7fffffffL) return -1;
+    if (wgs > UINT32_MAX / (64 * QW * KW) || (a.splits > 1 && joins > UINT32_MAX / 64)) return -1;
     cross_kernel<T, DH, QW, KW, WPE, UNAL><<<(unsigned)wgs, 64 * QW * KW, 0, st>>>(a, rbs);
     if (a.splits > 1) cross_join_kernel<T, DH><<<(unsigned)joins, 64, 0, st>>>(a);
     return 0;

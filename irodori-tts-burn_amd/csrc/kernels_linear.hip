@@ -531,15 +531,18 @@ __global__ __launch_bounds__(64 * NW) void linear_rows_kernel(LinearArgs a) {
 template <typename T, typename TO, int MT, int NW>
 int launch_rows(const LinearArgs& a, hipStream_t st) {
     static_assert(MT <= NW, "a thread per four sums");
-    linear_rows_kernel<T, TO, MT, NW><<<(a.N + 15) / 16, 64 * NW, 0, st>>>(a);
+    const int64_t wgs = ((int64_t)a.N + 15) / 16;
+    if (wgs * (64 * NW) > UINT32_MAX) return -1;
+    linear_rows_kernel<T, TO, MT, NW><<<(unsigned)wgs, 64 * NW, 0, st>>>(a);
     return 0;
 }
 
 template <typename T, typename TO, int BM, int BN, int WM, int WN, int WK, int RB, int STAGES, bool ASYNC>
 int launch_tiles(const LinearArgs& a, hipStream_t st) {
+    constexpr int THREADS = 64 * WM * WN * WK;
     const int64_t wgs = (int64_t)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-    if (wgs > 0x7fffffffL) return -1;
-    linear_kernel<T, TO, BM, BN, WM, WN, WK, RB, STAGES, ASYNC><<<(unsigned)wgs, 64 * WM * WN * WK, 0, st>>>(a);
+    if (wgs * THREADS > UINT32_MAX) return -1;
+    linear_kernel<T, TO, BM, BN, WM, WN, WK, RB, STAGES, ASYNC><<<(unsigned)wgs, THREADS, 0, st>>>(a);
     return 0;
 }
 

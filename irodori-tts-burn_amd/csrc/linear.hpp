@@ -17,7 +17,7 @@ struct LinearArgs {
     int M, N, K, act, gate_rows;
 };
 
-// 0, or -1 where the grid would not fit one launch.
+// 0, or -1 where the grid would not fit one launch (2^32 threads).
 template <typename T, typename TO>
 int launch_linear(const LinearArgs& a, hipStream_t st);
 

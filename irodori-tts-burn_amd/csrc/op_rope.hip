@@ -250,7 +250,7 @@ int launch(const irodori_rope_desc& d, RopeArgs& a, hipStream_t st) {
     a.div_units = ceil_inv(a.units);
     a.div_heads = ceil_inv(a.heads);
     const int64_t wgs = (int64_t)d.batch * a.tok_blocks * a.head_blocks;
-    IRO_REQUIRE(wgs <= INT32_MAX, IRODORI_ERR_SHAPE, "irodori_op_rope: too many tokens for one launch");
+    IRO_REQUIRE(wgs <= UINT32_MAX / 256, IRODORI_ERR_SHAPE, "irodori_op_rope: too many tokens for one launch");
     rope_kernel<T, V, HALVES><<<(unsigned)wgs, 256, 0, st>>>(a);
     return check_launch("rope");
 }

@@ -139,3 +139,16 @@ def test_cross_attention_refuses_pointers_and_workspaces():
                dict(workspace_bytes=need)):
         refused("InvalidArg", "workspace", lambda: ih.ops.cross_attention(d, P, P, P, P, **kw))
     assert L.load().irodori_op_cross_attention_workspace(d, None) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("text,call", [
+    ("tokens", lambda: ih.ops.rope(rope_desc(batch=1024, seq=2 ** 30), P, 2 * P, 3 * P, 4 * P)),
+    ("tokens", lambda: ih.ops.rope(rope_desc(batch=4096, seq=2 ** 18, dtype="bf16"), P, 2 * P, 3 * P, 4 * P)),
+    ("tiles", lambda: ih.ops.linear(linear_desc(m=1, n=2 ** 28, k=1), P, 2 * P, 3 * P)),
+    ("tiles", lambda: ih.ops.linear(linear_desc(m=2 ** 28, n=2 ** 28, k=1), P, 2 * P, 3 * P)),
+    ("rows", lambda: ih.ops.cross_attention(cross_desc(batch=2 ** 20, seq_q=4096, heads=16, kv_heads=16), P, 2 * P, 3 * P, 4 * P)),
+    ("rows", lambda: ih.ops.cross_attention(cross_desc(batch=2 ** 17, seq_q=4096, heads=16, kv_heads=2), P, 2 * P, 3 * P, 4 * P)),
+])
+def test_more_work_than_a_launch_holds_is_refused(text, call):
+    # A launch has at most 2^32 - 1 threads in one dimension.
+    refused("Shape", text + " for one launch", call)
