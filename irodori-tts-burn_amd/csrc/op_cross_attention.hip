@@ -70,6 +70,7 @@ int irodori_op_cross_attention(const irodori_cross_attention_desc* desc, const v
     const int64_t need = bytes_of(d, splits);
     IRO_REQUIRE(need == 0 || (workspace && workspace_bytes >= (uint64_t)need && aligned_to(workspace, 16)), IRODORI_ERR_INVALID_ARG,
                 "irodori_op_cross_attention: this shape takes a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
+    IRO_REQUIRE(out != q && out != k && out != v, IRODORI_ERR_INVALID_ARG, "irodori_op_cross_attention: out is an input");
     hipStream_t st = static_cast<hipStream_t>(stream);
     IRO_TRY(check_op_stream(st, "irodori_op_cross_attention"));
     CrossArgs a;

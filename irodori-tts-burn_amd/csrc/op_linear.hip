@@ -52,6 +52,7 @@ int irodori_op_linear(const irodori_linear_desc* desc, const void* x, const void
                 IRODORI_ERR_INVALID_ARG, "irodori_op_linear: an argument is not aligned to its element type");
     IRO_REQUIRE(!gate == !d.gate_rows, IRODORI_ERR_INVALID_ARG,
                 "irodori_op_linear: a gate and a positive gate_rows go together");
+    IRO_REQUIRE(y != x && y != w, IRODORI_ERR_INVALID_ARG, "irodori_op_linear: y is an input");
     IRO_REQUIRE(residual != y || d.m == 1 || d.ldr == d.ldy, IRODORI_ERR_SHAPE,
                 "irodori_op_linear: y onto its residual needs ldr == ldy");
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -280,6 +280,9 @@ int irodori_op_rope(const irodori_rope_desc* desc, const void* q, void* q_out, c
     const irodori_rope_desc& d = *desc;
     if (d.q_heads) IRO_TRY(check_side(d, "q", q, q_out, d.q_heads, d.q_rot_heads, d.q_strides, d.q_out_strides));
     if (d.k_heads) IRO_TRY(check_side(d, "k", k, k_out, d.k_heads, d.k_rot_heads, d.k_strides, d.k_out_strides));
+    if (d.q_heads && d.k_heads)
+        IRO_REQUIRE(q_out != k_out && q_out != k && k_out != q, IRODORI_ERR_INVALID_ARG,
+                    "irodori_op_rope: one side's output is the other side's tensor");
     IRO_REQUIRE(d.head_dim % 2 == 0, IRODORI_ERR_SHAPE, "irodori_op_rope: head_dim must be even");
     IRO_REQUIRE(aligned_to(positions, 4) && aligned_to(lengths, 4), IRODORI_ERR_INVALID_ARG,
                 "irodori_op_rope: positions or lengths are not aligned");

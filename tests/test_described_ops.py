@@ -152,3 +152,13 @@ def test_cross_attention_refuses_pointers_and_workspaces():
 def test_more_work_than_a_launch_holds_is_refused(text, call):
     # A launch has at most 2^32 - 1 threads in one dimension.
     refused("Shape", text + " for one launch", call)
+
+
+def test_outputs_that_are_inputs_are_refused():
+    d = cross_desc()
+    for at in (P, 2 * P, 3 * P):
+        refused("InvalidArg", "out is an input", lambda: ih.ops.cross_attention(d, P, 2 * P, 3 * P, at))
+    for at in (P, 2 * P):
+        refused("InvalidArg", "y is an input", lambda: ih.ops.linear(linear_desc(), P, 2 * P, at))
+    for args in ((P, 2 * P, 3 * P, 2 * P), (P, 3 * P, 3 * P, 4 * P), (P, P, 3 * P, P)):
+        refused("InvalidArg", "other side's", lambda: ih.ops.rope(rope_desc(), *args))
