@@ -212,7 +212,7 @@ using irodori::wave_sum;
 
 // A workgroup: QW wavefronts of 32 rows times KW groups that take the tiles in turn and are joined
 // through LDS.  Two ring slots of KW K and V tiles, moved HBM -> LDS by buffer_load_dwordx4 ... lds;
-// UNAL: through registers, for operands off a dword boundary or with rows too far apart for a window.
+// UNAL: through registers, for operands off a dword boundary, with rows too far apart for a window or overlapping.
 // Without splits it takes one batch row's keys.  With them, the tiles of all batch rows lie end to end
 // and each of a.splits workgroups of a key head and row block takes an equal run of them, of several
 // batch rows where they are short; the result for batch row b from workgroup w goes to slot w + b.
@@ -618,10 +618,11 @@ template <typename T, int DH>
 int launch_cross(const CrossArgs& a, hipStream_t st) {
     constexpr int64_t es = sizeof(T);
     constexpr bool F32 = sizeof(T) == 4;
-    // Windows of a tile's rows stay below 2^31 bytes, and the buffer-to-LDS loads take dword-aligned rows.
+    // Windows of a tile's rows stay below 2^31 bytes, and the buffer-to-LDS loads take dword-aligned rows.  Values
+    // whose rows overlap (a stride of 0) have rows past the last key inside the window, where they would not read as zero.
     const bool unal = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 3) ||
                       ((a.ks[0] | a.ks[1] | a.ks[2] | a.vs[0] | a.vs[1] | a.vs[2]) * es & 3) ||
-                      a.ks[1] * es > (1 << 24) || a.vs[1] * es > (1 << 24);
+                      a.ks[1] * es > (1 << 24) || a.vs[1] * es > (1 << 24) || (a.vs[1] < DH && a.seq_kv > 1);
     constexpr int SMALL = DH == 64 ? 2 : 1;  // wavefronts per SIMD, of two (one) workgroups a CU
     if (unal) return launch_cfg<T, DH, 2, 2, SMALL, true>(a, st);
     // f32 in one block of 32 rows is bound by the matrix cores, most of whose rows are padding: a group on every SIMD

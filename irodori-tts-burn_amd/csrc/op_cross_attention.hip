@@ -77,8 +77,10 @@ int irodori_op_cross_attention(const irodori_cross_attention_desc* desc, const v
     a.q = q; a.k = k; a.v = v; a.out = out;
     a.mask = mask; a.q_len = q_len; a.kv_len = kv_len;
     a.partial = static_cast<float*>(workspace);
-    for (int i = 0; i < 3; i++) {
-        a.qs[i] = d.q_strides[i]; a.ks[i] = d.k_strides[i]; a.vs[i] = d.v_strides[i]; a.os[i] = d.out_strides[i];
+    const int qn[3] = {d.batch, d.seq_q, d.heads}, kn[3] = {d.batch, d.seq_kv, d.kv_heads};
+    for (int i = 0; i < 3; i++) {  // (the stride of a dimension of one says nothing)
+        a.qs[i] = qn[i] > 1 ? d.q_strides[i] : 0; a.os[i] = qn[i] > 1 ? d.out_strides[i] : 0;
+        a.ks[i] = kn[i] > 1 ? d.k_strides[i] : 0; a.vs[i] = kn[i] > 1 ? d.v_strides[i] : 0;
     }
     a.mask_stride = d.mask_stride;
     a.batch = d.batch; a.heads = d.heads; a.kv_heads = d.kv_heads; a.group = d.heads / d.kv_heads;

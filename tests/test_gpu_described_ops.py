@@ -469,6 +469,35 @@ def test_cross_attention_broadcast_keys():
     check_cross(wide, q, k, v, "bf16")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,sq,skv", [(64, 5, 37), (64, 300, 70), (128, 40, 33), (64, 1, 3001)])
+def test_cross_attention_one_value_for_all_keys(dtype, d, sq, skv):
+    # A token stride of 0: every key's value is the same row, and so is the result, infinities included.
+    q, k = randn(1, 2, sq, 2, d, dtype=dtype), randn(2, 2, skv, 2, d, dtype=dtype)
+    row = randn(3, 2, 1, 2, d, dtype=dtype)
+    row[0, 0, 1, 3], row[1, 0, 0, 9] = float("inf"), float("-inf")
+    out = torch.empty_like(q)
+    run_cross(q, k, row.expand(2, skv, 2, d), out, dtype)
+    want = row.expand(2, sq, 2, d)
+    finite = want.isfinite()
+    assert torch.equal(out[~finite], want[~finite])
+    # The weights' sum is off by its own roundings alone: those of skv f32 additions on both sides.
+    tol = (2 * skv * F + 2.0 ** -20 + u(dtype) * (1 + 2.0 ** -6)) * want.double().abs() + tiny(dtype)
+    close(out[finite], want.double()[finite], tol[finite], "one value")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_cross_attention_strides_of_single_dimensions(dtype):
+    # One key, one token, one head or one batch row: that dimension's stride may be anything.
+    q, k, v = (randn(i, 1, 1, 1, 64, dtype=dtype) for i in (1, 2, 3))
+    for odd in (-1, 1, 2 ** 62):
+        desc = ih.CrossAttentionDesc(1, 1, 1, 1, 1, 64, dtype=dtype, q_strides=(odd,) * 3, k_strides=(odd,) * 3, v_strides=(odd,) * 3,
+                                     out_strides=(odd,) * 3)
+        out = torch.empty_like(q)
+        ih.ops.cross_attention(desc, ptr(q), ptr(k), ptr(v), ptr(out), stream=stream())
+        assert torch.equal(out, v)
+
+
 # ---- the half block they make up ----------------------------------------------------------------
 class HalfBlock:
     """x + g * (cross(rope(norm(x) Wq + bq), states Wk, states Wv) Wo), each step one operator."""
