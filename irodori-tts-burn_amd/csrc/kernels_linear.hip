@@ -4,8 +4,9 @@
 //
 // The product is formed transposed: W rows are the A operand and X rows the B operand of the
 // 32x32 matrix-core step, and the A operand's row 8g + 4f + c is W's row 16f + 4g + c of the block, so
-// a lane's 16 accumulators are 16 neighbouring columns of one row of Y: 16-byte loads of the bias, the
-// gate and the residual, 16-byte stores.
+// a lane's 16 accumulators are 16 neighbouring columns of one row of Y.  Two or four neighbouring lanes, a
+// row each, then exchange 16-byte pieces, so that one load of the residual or one store of Y has them side by side
+// in a row: the caches take a request a row from four lanes, not one a lane.
 //
 // Measured a call, host side included (the operator's floor in brackets):
 //   1 x 1024 x 512 bf16, silu            7.3 us [0.2]   the launch; 3.4 us of kernel
@@ -45,9 +46,17 @@ __device__ __forceinline__ void mma(f32x16& acc, const LFrag<T>& a, const LFrag<
     }
 }
 
-// W's row within a 32-row block that operand row r takes, and the other way round.
-__device__ __forceinline__ int w_row(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
-__device__ __forceinline__ int operand_row(int w) { return 8 * ((w >> 2) & 3) + 4 * ((w >> 4) & 1) + (w & 3); }
+// W's row that operand row r of block i takes, and the operand row of W's row w: blocks by themselves (16 columns of Y a
+// lane), or in pairs, whose 64 rows give a lane 32 columns.
+template <bool PAIR>
+__device__ __forceinline__ int w_row(int i, int r) {
+    const int f = (r >> 2) & 1, row = 4 * (r >> 3) + (r & 3);
+    return PAIR ? 64 * (i >> 1) + 32 * f + 16 * (i & 1) + row : 32 * i + 16 * f + row;
+}
+template <bool PAIR>
+__device__ __forceinline__ int operand_row(int w) {
+    return 8 * ((w >> 2) & 3) + 4 * ((w >> (PAIR ? 5 : 4)) & 1) + (w & 3);
+}
 // LDS rows of RB bytes (128 or 256); a 16-byte chunk c of the row that operand row r reads sits at this
 // place: 16 operand rows at one chunk spread over all banks.
 template <int RB>
@@ -113,7 +122,7 @@ __device__ __forceinline__ void activate(float (&v)[N], int act) {
     }
 }
 
-// C elements at p as f32: whole vectors, or one by one with those past the last (n of them) repeated.
+// C elements at p as f32 (n of them there: the others are zero).
 template <int C, typename T>
 __device__ __forceinline__ void load_cols(const T* p, int n, float (&f)[C]) {
     constexpr int E = C < 16 / (int)sizeof(T) ? C : 16 / sizeof(T);
@@ -127,18 +136,13 @@ __device__ __forceinline__ void load_cols(const T* p, int n, float (&f)[C]) {
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < C; i++) f[i] = static_cast<float>(p[i < n ? i : n - 1]);
+        for (int i = 0; i < C; i++) f[i] = i < n ? static_cast<float>(p[i]) : 0.f;
     }
 }
 
-// Columns n .. n + C - 1 (those below N) of row m of the residual.
+// Columns n .. n + C - 1 (those below N) of row m of Y from their sums.
 template <typename TO, int C>
-__device__ __forceinline__ void load_residual(const LinearArgs& a, int m, int n, float (&f)[C]) {
-    load_cols(static_cast<const TO*>(a.residual) + (int64_t)m * a.ldr + n, a.N - n, f);
-}
-// The same columns of Y from their sums, and from the residual's values where they are loaded already.
-template <typename TO, int C>
-__device__ __forceinline__ void finish(const LinearArgs& a, int m, int n, float (&v)[C], const float* residual = nullptr) {
+__device__ __forceinline__ void finish(const LinearArgs& a, int m, int n, float (&v)[C]) {
     constexpr int E = C < 16 / (int)sizeof(TO) ? C : 16 / sizeof(TO);
     typedef TO OE __attribute__((ext_vector_type(E), aligned(sizeof(TO))));
     const int left = a.N - n;
@@ -155,9 +159,9 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int m, int n, float 
         for (int i = 0; i < C; i++) v[i] *= f[i];
     }
     if (a.residual) {
-        if (!residual) load_residual<TO>(a, m, n, f);
+        load_cols(static_cast<const TO*>(a.residual) + (int64_t)m * a.ldr + n, left, f);
 #pragma unroll
-        for (int i = 0; i < C; i++) v[i] += residual ? residual[i] : f[i];
+        for (int i = 0; i < C; i++) v[i] += f[i];
     }
     TO* y = static_cast<TO*>(a.y) + (int64_t)m * a.ldy + n;
     if (left >= C) {
@@ -172,6 +176,117 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int m, int n, float 
 #pragma unroll
         for (int i = 0; i < C; i++)
             if (i < left) y[i] = static_cast<TO>(v[i]);
+    }
+}
+
+// Pieces of 16 bytes exchanged among Q neighbouring lanes: piece s of lane t becomes piece t of lane s.
+template <int Q>
+__device__ __forceinline__ void exchange(u32x4 (&p)[Q], int lane) {
+    auto step = [&](auto bit, auto perm) {
+        constexpr int b = decltype(bit)::value;
+        const bool up = lane & b;
+#pragma unroll
+        for (int s = 0; s < Q; s++) {
+            if (s & b) continue;
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                const unsigned x = p[s][d], y = p[s | b][d];
+                const unsigned px = __builtin_amdgcn_update_dpp(0u, x, decltype(perm)::value, 0xf, 0xf, true);
+                const unsigned py = __builtin_amdgcn_update_dpp(0u, y, decltype(perm)::value, 0xf, 0xf, true);
+                p[s][d] = up ? py : x;
+                p[s | b][d] = up ? y : px;
+            }
+        }
+    };
+    step(std::integral_constant<int, 1>{}, std::integral_constant<int, 0xb1>{});  // lane ^ 1
+    if constexpr (Q == 4) step(std::integral_constant<int, 2>{}, std::integral_constant<int, 0x4e>{});  // lane ^ 2
+}
+// Columns of Y in 16 bytes, and how many lanes exchange where each has C columns of a row.
+template <typename TO>
+constexpr int kPiece = 16 / (int)sizeof(TO);
+template <typename TO, int C>
+constexpr int kLanes = C / kPiece<TO> < 4 ? C / kPiece<TO> : 4;
+
+// One exchange's worth of the residual, exchanged: piece s is that of row m + s at column n (those in Y; WHOLE: all columns are).
+template <typename TO, bool WHOLE, int Q>
+__device__ __forceinline__ void load_pieces(const LinearArgs& a, int m, int n, u32x4 (&p)[Q]) {
+    constexpr int E = kPiece<TO>;
+    typedef TO OE __attribute__((ext_vector_type(E), aligned(sizeof(TO))));
+#pragma unroll
+    for (int s = 0; s < Q; s++) {
+        p[s] = u32x4{0u, 0u, 0u, 0u};
+        if (m + s >= a.M || (!WHOLE && n >= a.N)) continue;
+        const TO* r = static_cast<const TO*>(a.residual) + (int64_t)(m + s) * a.ldr + n;
+        OE o;
+        if (WHOLE || n + E <= a.N) {
+            o = *reinterpret_cast<const OE*>(r);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = n + e < a.N ? r[e] : static_cast<TO>(0.f);
+        }
+        p[s] = __builtin_bit_cast(u32x4, o);
+    }
+}
+// C columns of Y from n on, rows m0 + lane % 32, from their sums; by a whole wavefront.  WHOLE: all the columns are in Y.
+template <typename TO, bool WHOLE, int C>
+__device__ __forceinline__ void finish_block(const LinearArgs& a, int m0, int n, int lane, float (&v)[C], const u32x4* residual = nullptr) {
+    constexpr int E = kPiece<TO>, Q = kLanes<TO, C>;
+    typedef TO OE __attribute__((ext_vector_type(E), aligned(sizeof(TO))));
+    const int m = m0 + (lane & 31), t = lane & (Q - 1), mq = m - t, left = WHOLE ? C : a.N - n;
+    if (left > 0) {
+        float f[C];
+        if (a.bias) {
+            load_cols(a.bias + n, left, f);
+#pragma unroll
+            for (int i = 0; i < C; i++) v[i] += f[i];
+        }
+        activate(v, a.act);
+        if (a.gate) {
+            load_cols(a.gate + (int64_t)((m < a.M ? m : a.M - 1) / a.gate_rows) * a.N + n, left, f);
+#pragma unroll
+            for (int i = 0; i < C; i++) v[i] *= f[i];
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < C / (Q * E); g++) {
+        const int nt = n + (g * Q + t) * E;  // of this lane's pieces in the exchanged order
+        u32x4 p[Q];
+        if (a.residual) {
+            if (residual) {
+#pragma unroll
+                for (int s = 0; s < Q; s++) p[s] = residual[s];
+            } else {
+                load_pieces<TO, WHOLE>(a, mq, nt, p);
+            }
+            exchange(p, lane);
+#pragma unroll
+            for (int s = 0; s < Q; s++) {
+                const OE o = __builtin_bit_cast(OE, p[s]);
+#pragma unroll
+                for (int e = 0; e < E; e++) v[(g * Q + s) * E + e] += static_cast<float>(o[e]);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < Q; s++) {
+            OE o;
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = static_cast<TO>(v[(g * Q + s) * E + e]);
+            p[s] = __builtin_bit_cast(u32x4, o);
+        }
+        exchange(p, lane);
+#pragma unroll
+        for (int s = 0; s < Q; s++) {
+            if (mq + s >= a.M || (!WHOLE && nt >= a.N)) continue;
+            TO* y = static_cast<TO*>(a.y) + (int64_t)(mq + s) * a.ldy + nt;
+            const OE o = __builtin_bit_cast(OE, p[s]);
+            if (WHOLE || nt + E <= a.N) {
+                *reinterpret_cast<OE*>(y) = o;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (nt + e < a.N) y[e] = o[e];
+            }
+        }
     }
 }
 
@@ -208,6 +323,8 @@ void linear_kernel(LinearArgs a) {
     constexpr int NW = WM * WN * WK, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
     constexpr int ROWS = BM + BN, STAGE = ROWS * RB, BK = RB / sizeof(T), KS = BK / 16, RC = RB / 16;
     constexpr int RPI = 64 / RC, LPW = ROWS / RPI / NW;  // rows a load instruction fills, instructions per wave per slice
+    constexpr bool PAIR = FN % 2 == 0 && sizeof(TO) == 2;
+    constexpr int C = PAIR ? 32 : 16;  // neighbouring columns of Y a lane ends with
     static_assert(LPW * RPI * NW == ROWS && BN % RPI == 0 && KS % WK == 0, "slices split over the waves");
     static_assert(WK == 1 || (WK - 1) * BM * BN * 4 <= STAGES * STAGE, "the k groups' sums fit the ring");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * STAGE];
@@ -230,7 +347,7 @@ void linear_kernel(LinearArgs a) {
     // lane -> row lane / RC, physical chunk lane % RC, which holds the row's chunk `chunk`.
     auto chunk = [&](int i) {
         const int r = (wave * LPW + i) * RPI + lane / RC;
-        return lswz<RB>(r < BN ? operand_row(r & 31) : r, lane % RC);
+        return lswz<RB>(r < BN ? operand_row<PAIR>(r) : r, lane % RC);
     };
     [[maybe_unused]] __amdgpu_buffer_rsrc_t rX, rW;
     [[maybe_unused]] unsigned voff[LPW];
@@ -297,10 +414,11 @@ void linear_kernel(LinearArgs a) {
 
     // One block a wavefront: its residual comes under the products (11.6 -> 11.1 us at 1500 x 1024 x 1024).
     constexpr bool EARLY = FM * FN == 1;
-    [[maybe_unused]] float early[16];
+    [[maybe_unused]] u32x4 early[kLanes<TO, C>];
     if constexpr (EARLY) {
-        const int m = m0 + wm * TM + fr, n = n0 + wn * TN + 16 * fh;
-        if (a.residual && wk == 0 && m < a.M && n < a.N) load_residual<TO>(a, m, n, early);
+        constexpr int Q = kLanes<TO, C>;
+        const int t = lane & (Q - 1);
+        if (a.residual && wk == 0) load_pieces<TO, false>(a, m0 + wm * TM + fr - t, n0 + wn * TN + 16 * fh + t * kPiece<TO>, early);
     }
 
     // Two sets of fragments: a step's are read while the step before multiplies.  Before a slice's last
@@ -312,7 +430,7 @@ void linear_kernel(LinearArgs a) {
         const unsigned char* st = smem + kt % STAGES * STAGE;
         const int ks = s * WK + wk;
 #pragma unroll
-        for (int i = 0; i < FN; i++) fw[set][i] = read_frag<T, RB>(st + (wn * TN + 32 * i + w_row(fr)) * RB, fr, ks, fh);
+        for (int i = 0; i < FN; i++) fw[set][i] = read_frag<T, RB>(st + (wn * TN + w_row<PAIR>(i, fr)) * RB, fr, ks, fh);
 #pragma unroll
         for (int j = 0; j < FM; j++) fx[set][j] = read_frag<T, RB>(st + (BN + wm * TM + 32 * j + fr) * RB, fr, ks, fh);
     };
@@ -416,21 +534,21 @@ void linear_kernel(LinearArgs a) {
 
     if (WK > 1 && wk > 0) return;
 
-    // acc[i][j][e] = Y[m0 + wm TM + 32 j + fr][n0 + wn TN + 32 i + 16 fh + e].
+    // Lane (fr, fh) has of row m0 + wm TM + 32 j + fr the columns from n0 + wn TN + 2 C i + C fh on, C / 16 blocks' sums.
+    auto finish_all = [&](auto whole) {
 #pragma unroll
-    for (int j = 0; j < FM; j++) {
-        const int m = m0 + wm * TM + 32 * j + fr;
-        if (m >= a.M) continue;
+        for (int j = 0; j < FM; j++)
 #pragma unroll
-        for (int i = 0; i < FN; i++) {
-            const int n = n0 + wn * TN + 32 * i + 16 * fh;
-            if (n >= a.N) continue;
-            float v[16];
+            for (int i = 0; i < FN * 16 / C; i++) {
+                float v[C];
 #pragma unroll
-            for (int e = 0; e < 16; e++) v[e] = acc[i][j][e];
-            finish<TO>(a, m, n, v, EARLY ? early : nullptr);
-        }
-    }
+                for (int e = 0; e < C; e++) v[e] = acc[i * (C / 16) + e / 16][j][e % 16];
+                finish_block<TO, decltype(whole)::value>(a, m0 + wm * TM + 32 * j, n0 + wn * TN + 2 * C * i + C * fh, lane, v,
+                                                         EARLY ? early : nullptr);
+            }
+    };
+    if (rows_n == BN) finish_all(std::true_type{});
+    else finish_all(std::false_type{});
 }
 
 // ---- few rows ---------------------------------------------------------------------------------
@@ -551,32 +669,36 @@ int launch_tiles(const LinearArgs& a, hipStream_t st) {
 namespace {
 
 // The tiles a launch takes: of these, the one whose busiest CU is done first, by the microseconds of a tile
-// (f + a K) measured over M from 32 to 12 000 at N = 333, 1024, 1280 and 5632, K = 512, 1024 and 3680.  Two tiles
-// on a CU overlap where they wait for memory (half: rounds count by halves); one alone may take longer than one of
-// many.  E.g. in bf16 with 32 x 32 / 64 x 64 / 128 x 64 / 128 x 128 / 256 x 256 tiles: 256 x 1024 x 1024 6.8 / 6.7 / 9.0 /
-// 11.3 / 29 us, 1500 x 1024 x 1024 13.0 / 8.5 / 9.5 / 11.8 / 30, 12000 x 5632 x 1024 436 / 262 / 207 / 168 / 183, 24000 x 5632
-// x 1024 the last two 345 / 322.
+// (f + a K) fitted to all tiles' times over M from 32 to 69 694 at N = 333, 1024, 1280 and 5632 and K = 32, 512, 1024 and 3680
+// (the choice loses 0.7 % on the best of them on average, 11 % at most).  Two tiles on a CU overlap where they wait
+// (half: rounds count by halves); one alone may take longer than one of many.  E.g. in bf16 with 32 x 32 / 64 x 64 / 128 x 64 /
+// 128 x 128 / 256 x 256 tiles: 256 x 1024 x 1024 5.5 / 6.0 / 8.9 / 10.4 / 27 us, 1500 x 1024 x 1024 14.1 / 9.1 / 9.9 / 11.1 / 27,
+// 12000 x 5632 x 1024 - / 244 / 195 / 150 / 162, 24000 x 5632 x 1024 the last two 295 / 281 (with silu 304 / 301, with gelu
+// 356 / 371), 12000 x 5632 x 32 - / 85 / 47 / 34 / 42.
 struct TileCost {
     int bm, bn;
-    float f, a;
+    float f, a, act;  // act: one exponential and one reciprocal an element
     bool half;
     float alone;
 };
-constexpr TileCost kTiles16[] = {{32, 32, 0.25f, 0.0014f, false, 1.f},
-                                 {64, 64, 0.38f, 0.0036f, true, 1.f},
-                                 {128, 64, 0.3f, 0.006f, true, 1.f},
-                                 {128, 128, 1.15f, 0.0085f, false, 1.35f},
-                                 {256, 256, 8.f, 0.0264f, false, 1.f}};
-constexpr TileCost kTiles32[] = {{32, 32, 0.45f, 0.00425f, false, 1.f}, {64, 64, 0.7f, 0.0162f, false, 1.f}, {128, 128, 4.5f, 0.059f, false, 1.f}};
+constexpr TileCost kTiles16[] = {{32, 32, 0.25f, 0.0014f, 0.03f, true, 1.f},
+                                 {64, 64, 0.32f, 0.0036f, 0.12f, false, 1.f},
+                                 {128, 64, 0.43f, 0.0136f, 0.25f, false, 1.f},
+                                 {128, 128, 1.2f, 0.0075f, 0.5f, true, 1.2f},
+                                 {256, 256, 14.3f, 0.0155f, 2.8f, false, 1.f}};
+constexpr TileCost kTiles32[] = {{32, 32, 0.43f, 0.0046f, 0.03f, false, 1.f},
+                                 {64, 64, 0.97f, 0.0161f, 0.12f, false, 1.f},
+                                 {128, 128, 2.74f, 0.0606f, 0.5f, true, 1.f}};
 template <int N>
 int best_tiles(const TileCost (&t)[N], const LinearArgs& a) {
     constexpr int CUS = 256;
+    const float act = a.act == IRODORI_ACT_NONE || a.act == IRODORI_ACT_RELU ? 0.f : a.act == IRODORI_ACT_GELU ? 4.f : 1.f;
     int best = 0;
     double least = 0.;
     for (int i = 0; i < N; i++) {
         const int64_t n = ((int64_t)(a.M + t[i].bm - 1) / t[i].bm) * ((a.N + t[i].bn - 1) / t[i].bn);
         const double rounds = n <= CUS ? 1. : t[i].half ? (double)((2 * n + CUS - 1) / CUS) / 2. : (double)((n + CUS - 1) / CUS);
-        const double c = rounds * (t[i].f + t[i].a * a.K) * (n <= CUS ? t[i].alone : 1.f);
+        const double c = rounds * (t[i].f + t[i].a * a.K + t[i].act * act) * (n <= CUS ? t[i].alone : 1.f);
         if (i == 0 || c < least) {
             least = c;
             best = i;
