@@ -15,13 +15,13 @@
 // the masked values, which are not loaded, zero.
 //
 // Measured a call, host side included (the operator's floor in brackets):
-//   8 x 1 token over 8200 ragged keys, 16 heads on 4 of 128 (bf16)   27.2 us [19.5]  memory: the runs stream at 4.3 TB/s for
-//                                        22 us, the joining launch takes 5
-//   2 x 101 over 37 keys, 16 heads of 64 (f32)    8.1 [0.4]   one chain: mask, tile, 4096 cycles of f32 matrix core, join
-//   2 x 750 over 631 masked keys, 16 heads of 64 (bf16)   15.5 [1.7]  192 workgroups, a chain of five steps of about 1.4 us
+//   8 x 1 token over 8200 ragged keys, 16 heads on 4 of 128 (bf16)   26.4 us [19.5]  memory: the runs stream at 4.5 TB/s for
+//                                        21 us, the joining launch takes 5
+//   2 x 101 over 37 keys, 16 heads of 64 (f32)    8.2 [0.4]   one chain: mask, tile, 4096 cycles of f32 matrix core, join
+//   2 x 750 over 631 masked keys, 16 heads of 64 (bf16)   14.8 [1.7]  384 workgroups, a chain of five steps of about 1.2 us
 //                                        (softmax on the VALU, then the products) between 4 us of loads and 2 of joining
-//   32 x 750 over 4100 ragged keys, 20 heads of 64 (f16)  460 [219]   VALU 64 % and matrix cores 42 % of the cycles, at the
-//                                        1.7 GHz that the card's power leaves; 128-dim heads 830 TFLOP/s (bf16)
+//   32 x 750 over 4100 ragged keys, 20 heads of 64 (f16)  455 [219]   VALU 64 % and matrix cores 43 % of the cycles, at the
+//                                        1.7 GHz that the card's power leaves; 128-dim heads 855 TFLOP/s (bf16)
 #include <type_traits>
 
 #include "attn_util.hpp"

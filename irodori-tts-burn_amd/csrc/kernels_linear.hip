@@ -4,18 +4,19 @@
 //
 // The product is formed transposed: W rows are the A operand and X rows the B operand of the
 // 32x32 matrix-core step, and the A operand's row 8g + 4f + c is W's row 16f + 4g + c of the block, so
-// a lane's 16 accumulators are 16 neighbouring columns of one row of Y.  Two or four neighbouring lanes, a
+// a lane ends with 16 neighbouring columns of one row of Y (of two blocks together 32).  Two or four neighbouring lanes, a
 // row each, then exchange 16-byte pieces, so that one load of the residual or one store of Y has them side by side
-// in a row: the caches take a request a row from four lanes, not one a lane.
+// in a row: the caches take one request from four lanes, not four (12000 x 5632 x 1024 into f32 171 against 214 us,
+// 69694 x 1280 x 32 in f16 40 against 66).
 //
 // Measured a call, host side included (the operator's floor in brackets):
 //   1 x 1024 x 512 bf16, silu            7.3 us [0.2]   the launch; 3.4 us of kernel
 //   4 x 3680 x 1280 f16, gelu            7.3 [1.9]      the launch; W at 2.0 TB/s in 4.7 us of kernel
 //   253 x 1280 x 1280 f32, gelu          16.7 [5.4]     f32 matrix cores: 320 tiles on 256 CUs, two on the busiest
-//   1500 x 1024 x 1024 bf16 -> f32, gate, residual  11.9 [3.6]  a chain of 8 slices from L2 with 384 tiles, then 12 MB of
+//   1500 x 1024 x 1024 bf16 -> f32, gate, residual  10.9 [3.6]  a chain of 8 slices from L2 with 384 tiles, then 12 MB of
 //                                        residual and output
-//   24000 x 5632 x 1024 bf16, silu       306 [192]      the card's power (278 us on zeros) and, per 256 x 256 tile, 11 of
-//                                        36 us before the first and after the last slice; a library product of
+//   24000 x 5632 x 1024 bf16, silu       306 [192]      the card's power (272 us on zeros) and, per 256 x 256 tile, 9 of
+//                                        35 us before the first and after the last slice; a library product of
 //                                        the same operands takes 318
 #include <type_traits>
 
