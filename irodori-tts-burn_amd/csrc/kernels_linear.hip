@@ -16,7 +16,7 @@
 //   1500 x 1024 x 1024 bf16 -> f32, gate, residual  10.9 [3.6]  a chain of 8 slices from L2 with 384 tiles, then 12 MB of
 //                                        residual and output
 //   24000 x 5632 x 1024 bf16, silu       306 [192]      the card's power (272 us on zeros) and, per 256 x 256 tile, 9 of
-//                                        35 us before the first and after the last slice; a library product of
+//                                        37 us before the first and after the last slice; a library product of
 //                                        the same operands takes 318
 #include <type_traits>
 
@@ -413,7 +413,7 @@ void linear_kernel(LinearArgs a) {
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
 
-    // One block a wavefront: its residual comes under the products (11.6 -> 11.1 us at 1500 x 1024 x 1024).
+    // One block a wavefront: its residual comes under the products (9.6 -> 9.4 us at 1500 x 1024 x 1024).
     constexpr bool EARLY = FM * FN == 1;
     [[maybe_unused]] u32x4 early[kLanes<TO, C>];
     if constexpr (EARLY) {
@@ -712,15 +712,15 @@ int best_tiles(const TileCost (&t)[N], const LinearArgs& a) {
 
 template <typename T, typename TO>
 int launch_linear(const LinearArgs& a, hipStream_t st) {
-    // One new token or a few: 4.1 against 6.2 us with 32 x 32 tiles at 16 x 1024 x 1024 (bf16), 5.0 and 4.9 at 32 rows.
+    // One new token or a few: 4.0 against 5.0 to 6.2 us with 32 x 32 tiles at 16 x 1024 x 1024 (bf16).
     if (a.M <= 16) return launch_rows<T, TO, 1, 8>(a, st);
     // The buffer-to-LDS loads take dword-aligned rows, and windows of a tile's rows below 2^31 bytes.
     constexpr int64_t ES = sizeof(T), FAR = (int64_t)1 << 22;
     const bool async = !((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx * ES | a.ldw * ES) & 3) &&
                        a.ldx * ES <= FAR && a.ldw * ES <= FAR && a.K * ES <= FAR;
     if (!async) {
-        // Through registers (16-bit rows an odd number of elements apart): 64 x 64 against 128 x 128 tiles 13.0 / 25.6 us at
-        // 500 x 1024 x 1001 (32 tiles of 128), 60.5 / 37.7 at 2000 x 2816 (352), 1046 / 565 at 20000 x 5632.
+        // Through registers (16-bit rows an odd number of elements apart): 64 x 64 against 128 x 128 tiles 12.5 / 24.6 us at
+        // 500 x 1024 x 1001 (32 tiles of 128), 56 / 37 at 2000 x 2816 (352), 786 / 552 at 20000 x 5632.
         if (((int64_t)a.M + 127) / 128 * ((a.N + 127) / 128) < 128) return launch_tiles<T, TO, 64, 64, 2, 2, 2, 128, 2, false>(a, st);
         return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, false>(a, st);
     }
