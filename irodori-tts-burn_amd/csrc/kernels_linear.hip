@@ -670,26 +670,26 @@ int launch_tiles(const LinearArgs& a, hipStream_t st) {
 namespace {
 
 // The tiles a launch takes: of these, the one whose busiest CU is done first, by the microseconds of a tile
-// (f + a K) fitted to all tiles' times over M from 32 to 69 694 at N = 333, 1024, 1280 and 5632 and K = 32, 512, 1024 and 3680
-// (the choice loses 0.7 % on the best of them on average, 11 % at most).  Two tiles on a CU overlap where they wait
-// (half: rounds count by halves); one alone may take longer than one of many.  E.g. in bf16 with 32 x 32 / 64 x 64 / 128 x 64 /
-// 128 x 128 / 256 x 256 tiles: 256 x 1024 x 1024 5.5 / 6.0 / 8.9 / 10.4 / 27 us, 1500 x 1024 x 1024 14.1 / 9.1 / 9.9 / 11.1 / 27,
-// 12000 x 5632 x 1024 - / 244 / 195 / 150 / 162, 24000 x 5632 x 1024 the last two 295 / 281 (with silu 304 / 301, with gelu
-// 356 / 371), 12000 x 5632 x 32 - / 85 / 47 / 34 / 42.
+// (f + a K) fitted to all tiles' times at 288 sizes (16-bit) and 202 (f32): M from 20 to 69 694, N from 333 to 5632, K from 32 to
+// 3680.  The choice loses 1.3 % on the best of them on average, 23 % at most (0.1 % and 11 % in f32).  Tiles that share a CU
+// overlap where they wait (rounds count in parts); one a CU may take longer than one of many.  E.g. in bf16 with
+// 32 x 32 / 64 x 64 / 128 x 64 / 128 x 128 / 256 x 256 tiles: 256 x 1024 x 1024 5.5 / 6.0 / 8.9 / 10.4 / 27 us, 1500 x 1024 x 1024
+// 14.1 / 9.1 / 9.9 / 11.1 / 27, 12000 x 5632 x 1024 - / 244 / 195 / 150 / 162, 24000 x 5632 x 1024 the last two 295 / 281 (with silu
+// 304 / 301, with gelu 356 / 371), 12000 x 5632 x 32 - / 85 / 47 / 34 / 42.
 struct TileCost {
     int bm, bn;
     float f, a, act;  // act: one exponential and one reciprocal an element
-    bool half;
+    int parts;
     float alone;
 };
-constexpr TileCost kTiles16[] = {{32, 32, 0.25f, 0.0014f, 0.03f, true, 1.f},
-                                 {64, 64, 0.32f, 0.0036f, 0.12f, false, 1.f},
-                                 {128, 64, 0.43f, 0.0136f, 0.25f, false, 1.f},
-                                 {128, 128, 1.2f, 0.0075f, 0.5f, true, 1.2f},
-                                 {256, 256, 14.3f, 0.0155f, 2.8f, false, 1.f}};
-constexpr TileCost kTiles32[] = {{32, 32, 0.43f, 0.0046f, 0.03f, false, 1.f},
-                                 {64, 64, 0.97f, 0.0161f, 0.12f, false, 1.f},
-                                 {128, 128, 2.74f, 0.0606f, 0.5f, true, 1.f}};
+constexpr TileCost kTiles16[] = {{32, 32, 0.65f, 0.0022f, 0.03f, 4, 1.1f},
+                                 {64, 64, 0.9f, 0.0055f, 0.12f, 2, 1.f},
+                                 {128, 64, 2.4f, 0.0047f, 0.25f, 1, 1.4f},
+                                 {128, 128, 0.45f, 0.0095f, 0.5f, 2, 1.6f},
+                                 {256, 256, 7.4f, 0.022f, 3.1f, 1, 1.f}};
+constexpr TileCost kTiles32[] = {{32, 32, 0.54f, 0.0042f, 0.03f, 1, 1.f},
+                                 {64, 64, 1.18f, 0.0154f, 0.12f, 1, 1.f},
+                                 {128, 128, 1.93f, 0.0596f, 0.5f, 1, 1.f}};
 template <int N>
 int best_tiles(const TileCost (&t)[N], const LinearArgs& a) {
     constexpr int CUS = 256;
@@ -698,8 +698,8 @@ int best_tiles(const TileCost (&t)[N], const LinearArgs& a) {
     double least = 0.;
     for (int i = 0; i < N; i++) {
         const int64_t n = ((int64_t)(a.M + t[i].bm - 1) / t[i].bm) * ((a.N + t[i].bn - 1) / t[i].bn);
-        const double rounds = n <= CUS ? 1. : t[i].half ? (double)((2 * n + CUS - 1) / CUS) / 2. : (double)((n + CUS - 1) / CUS);
-        const double c = rounds * (t[i].f + t[i].a * a.K + t[i].act * act) * (n <= CUS ? t[i].alone : 1.f);
+        const double rounds = n <= CUS ? t[i].alone : (double)((n * t[i].parts + CUS - 1) / CUS) / t[i].parts;
+        const double c = rounds * (t[i].f + t[i].a * a.K + t[i].act * act);
         if (i == 0 || c < least) {
             least = c;
             best = i;
