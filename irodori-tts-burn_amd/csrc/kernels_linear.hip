@@ -720,8 +720,9 @@ int launch_linear(const LinearArgs& a, hipStream_t st) {
                        a.ldx * ES <= FAR && a.ldw * ES <= FAR && a.K * ES <= FAR;
     if (!async) {
         // Through registers (16-bit rows an odd number of elements apart): 64 x 64 against 128 x 128 tiles 12.5 / 24.6 us at
-        // 500 x 1024 x 1001 (32 tiles of 128), 56 / 37 at 2000 x 2816 (352), 786 / 552 at 20000 x 5632.
-        if (((int64_t)a.M + 127) / 128 * ((a.N + 127) / 128) < 128) return launch_tiles<T, TO, 64, 64, 2, 2, 2, 128, 2, false>(a, st);
+        // 500 x 1024 x 1001 (32 tiles of 128), 24.4 / 33.9 at 1536 x 2048 (192), 36.9 / 26.3 at 2048 x 2048 (256), 786 / 552 at
+        // 20000 x 5632.
+        if (((int64_t)a.M + 127) / 128 * ((a.N + 127) / 128) < 200) return launch_tiles<T, TO, 64, 64, 2, 2, 2, 128, 2, false>(a, st);
         return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, false>(a, st);
     }
     if constexpr (sizeof(T) == 4) {

@@ -254,6 +254,29 @@ def test_linear_strides_and_alignment(dtype, m, n, k, pad, offset):
     assert (flat[kept] == CANARY).all()
 
 
+@pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("m,n,k,pad", [(1003, 1283, 1288, 8), (403, 2819, 2824, 8), (1501, 1291, 128, 8), (2101, 2051, 72, 8),
+                                       (1501, 5635, 3688, 8), (1902, 1801, 136, 3), (901, 1030, 136, 3)])
+def test_linear_edges_of_large_tiles(dtype, out, m, n, k, pad):
+    """Tiles of every size that end past the last row and inside a lane's columns, everything after the product
+    with them, onto the residual; the columns between rows keep what they hold."""
+    def rows(seed, r, c, dt):
+        flat = torch.full((r, c + pad), math.nan, dtype=TYPE[dt], device="cuda")
+        v = flat[:, :c]
+        v.copy_(randn(seed, r, c, dtype=dt))
+        return flat, v
+    _, x = rows(1, m, k, dtype)
+    _, w = rows(2, n, k, dtype)
+    w.mul_(k ** -0.5)
+    bias, gate = randn(3, n), randn(5, -(-m // 7), n)
+    flat, y = rows(4, m, n, out)
+    flat[:, n:] = CANARY
+    ref = linear_ref(x, w, out, "silu", bias, gate, 7, y.clone())
+    run_linear(x, w, y, dtype, out, "silu", bias=bias, gate=gate, gate_rows=7, residual=y)
+    close(y, *ref, "edges")
+    assert (flat[:, n:] == CANARY).all()
+
+
 def test_linear_broadcast_rows_and_specials():
     # A stride of 0 repeats one row of x and of the residual; infinities and NaN reach their own rows only.
     w = randn(2, 48, 64, dtype="bf16")
