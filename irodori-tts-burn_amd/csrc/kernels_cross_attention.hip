@@ -639,7 +639,7 @@ int launch_cross(const CrossArgs& a, hipStream_t st) {
     // whose rows overlap (a stride of 0) have rows past the last key inside the window, where they would not read as zero.
     const bool unal = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 3) ||
                       ((a.ks[0] | a.ks[1] | a.ks[2] | a.vs[0] | a.vs[1] | a.vs[2]) * es & 3) ||
-                      a.ks[1] * es > (1 << 24) || a.vs[1] * es > (1 << 24) || (a.vs[1] < DH && a.seq_kv > 1);
+                      a.ks[1] * es > (1 << 24) || a.vs[1] * es > (1 << 24) || a.vs[1] < DH;
     constexpr int SMALL = DH == 64 ? 2 : 1;  // wavefronts per SIMD, of two (one) workgroups a CU
     if (unal) return launch_cfg<T, DH, 2, 2, SMALL, true>(a, st);
     // f32 in one block of 32 rows is bound by the matrix cores, most of whose rows are padding: a group on every SIMD

@@ -82,6 +82,9 @@ int irodori_op_cross_attention(const irodori_cross_attention_desc* desc, const v
         a.qs[i] = qn[i] > 1 ? d.q_strides[i] : 0; a.os[i] = qn[i] > 1 ? d.out_strides[i] : 0;
         a.ks[i] = kn[i] > 1 ? d.k_strides[i] : 0; a.vs[i] = kn[i] > 1 ? d.v_strides[i] : 0;
     }
+    // A tile's rows past a single key lie behind it, outside its window: at stride 0 each would read as that key, and
+    // a weight of 0 times an infinite value is not 0.
+    if (d.seq_kv == 1) a.ks[1] = a.vs[1] = d.head_dim;
     a.mask_stride = d.mask_stride;
     a.batch = d.batch; a.heads = d.heads; a.kv_heads = d.kv_heads; a.group = d.heads / d.kv_heads;
     a.seq_q = d.seq_q; a.seq_kv = d.seq_kv; a.splits = splits;

@@ -521,6 +521,28 @@ def test_cross_attention_strides_of_single_dimensions(dtype):
         assert torch.equal(out, v)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq", [1, 70])
+@pytest.mark.parametrize("masked", [False, True])
+def test_cross_attention_single_key(dtype, d, sq, masked):
+    """One key: its weight is 1, and the result its value, infinities and NaN among them."""
+    b, h = 3, 2
+    q, k, v = randn(1, b, sq, h, d, dtype=dtype), randn(2, b, 1, h, d, dtype=dtype), randn(3, b, 1, h, d, dtype=dtype)
+    for i, x in enumerate((math.inf, -math.inf, math.nan)):
+        v[:, 0, 1, 7 * i] = x
+    mask = torch.tensor([[1], [255], [0]], dtype=torch.uint8, device="cuda") if masked else None
+    out = torch.full((b, sq, h, d), CANARY, dtype=TYPE[dtype], device="cuda")
+    run_cross(q, k, v, out, dtype, mask=mask)
+    want = v.expand(b, sq, h, d).clone()
+    if masked:
+        want[2] = 0
+    special = ~want.isfinite()
+    assert torch.equal(out[special].nan_to_num(CANARY), want[special].nan_to_num(CANARY))
+    # The product with the weight, the reciprocal of the same weight and their product: F each, then the type's rounding.
+    close(out[~special], want.double()[~special], (4 * F + u(dtype) * (1 + 4 * F)) * want.double().abs()[~special] + tiny(dtype), "one key")
+
+
 # ---- the half block they make up ----------------------------------------------------------------
 class HalfBlock:
     """x + g * (cross(rope(norm(x) Wq + bq), states Wk, states Wv) Wo), each step one operator."""
