@@ -68,8 +68,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     const int s0 = tb * a.tokens, h0 = hb * a.heads;
     int len = a.seq;
     if (a.lengths) {
-        const int n = a.lengths[b];
-        len = n < len ? n : len;
+        const int n = a.lengths[b];  // (below 0 none: len - s0 must not leave 32 bits)
+        len = n < 0 ? 0 : n < len ? n : len;
     }
     const int nt = len - s0 < a.tokens ? len - s0 : a.tokens;
     if (nt <= 0) return;  // rows past the length stay as they were

@@ -164,6 +164,24 @@ def test_rope_gradient_is_the_inverse_flag():
     assert abs(diff - dx[1, 4, 1, 3].double()) <= 64 * F * 8 * g.abs().max().double() * x.abs().max().double()
 
 
+def test_rope_lengths_below_zero():
+    # Lengths of any sign, the lowest number among them: rows without a token stay as they were, the rows beside them too.
+    b, s, h, d = 5, 2051, 3, 64
+    lens = [-1, -2 ** 31, 2051, 1 - 2 ** 31, 2 ** 31 - 1]
+    x = randn(3, b, s, h, d)
+    flat = torch.full((b * s * h * d + 4096,), CANARY, device="cuda")
+    y = flat[:b * s * h * d].view(b, s, h, d)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ih.ops.rope(ih.RopeDesc(b, s, d, heads=h, dtype="f32"), ptr(x), ptr(y), d_lengths=ptr(n), stream=stream())
+    ref, mag = rope_ref(x, torch.arange(s, device="cuda").expand(b, s), rope_freq(64), "interleaved", h)
+    for row in range(b):
+        if lens[row] < 0:
+            assert (y[row] == CANARY).all()
+        else:
+            close(y[row], ref[row], rope_tol(ref[row], mag[row], "f32"))
+    assert (flat[b * s * h * d:] == CANARY).all()
+
+
 # ---- linear layer -----------------------------------------------------------------------------
 ACTS = {
     "none": lambda z: z, "relu": torch.relu, "silu": torch.nn.functional.silu, "sigmoid": torch.sigmoid, "tanh": torch.tanh,
