@@ -270,12 +270,13 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
     // Load instruction ii of this wave in a stage: rows RPI (row0 + ii) .. of tile `tile` of the step's;
     // lane -> row lane / CH, physical chunk lane % CH.
     const int tile = wave * LPW / NI, part = wave * LPW % NI;
-    unsigned voK[LPW], voV[LPW];
+    typedef typename std::conditional<UNAL, int64_t, unsigned>::type Off;  // (a window's stay below 2^31)
+    Off voK[LPW], voV[LPW];
 #pragma unroll
     for (int ii = 0; ii < LPW; ii++) {
         const int r = (part + ii) * RPI + lane / CH;
-        voK[ii] = (unsigned)(r * (a.ks[1] * (int)sizeof(T))) + (kswz<ROWB>(r, lane % CH) << 4);
-        voV[ii] = (unsigned)(r * (a.vs[1] * (int)sizeof(T))) + (vswz<T, ROWB>(r, lane % CH) << 4);
+        voK[ii] = (Off)(r * (a.ks[1] * (int)sizeof(T))) + (kswz<ROWB>(r, lane % CH) << 4);
+        voV[ii] = (Off)(r * (a.vs[1] * (int)sizeof(T))) + (vswz<T, ROWB>(r, lane % CH) << 4);
     }
 
     int tiles = 0;  // split: those of the lane's batch row among the 64 around b
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
             raw_barrier();  // the rings may still be read
             // This wave's share of K tile t, and of V tile t without its masked rows (0 times a masked value's NaN or
             // infinity would not be 0), into ring slot `slot`.  Rows past the last key and those left out read as zero.
-            auto load = [&](const T* base, const int64_t token, const unsigned (&vo)[LPW], int off, int t, int slot, auto kept) {
+            auto load = [&](const T* base, const int64_t token, const Off (&vo)[LPW], int off, int t, int slot, auto kept) {
                 const int left = len - t * KT, n = left < KT ? left : KT;  // rows of the tile
                 const T* src = base + (int64_t)t * KT * token;
                 unsigned char* dst = smem + off + (slot * KW + tile) * TILE + part * 1024;
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
                     if constexpr (UNAL) {
                         typedef T E16 __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
                         u32x4 x = {0, 0, 0, 0};
-                        if (r < n && kept(r)) x = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(src + vo[ii] / sizeof(T)));
+                        if (r < n && kept(r)) x = __builtin_bit_cast(u32x4, *reinterpret_cast<const E16*>(src + vo[ii] / (int)sizeof(T)));
                         *reinterpret_cast<u32x4*>(dst + ii * 1024 + 16 * lane) = x;
                     } else {
                         buf_load_lds16(make_rsrc(src, (unsigned)((n - 1) * token * (int)sizeof(T)) + ROWB), kept(r) ? vo[ii] : 0x80000000u,

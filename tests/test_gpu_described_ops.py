@@ -561,6 +561,20 @@ def test_cross_attention_single_key(dtype, d, sq, masked):
     close(out[~special], want.double()[~special], (4 * F + u(dtype) * (1 + 4 * F)) * want.double().abs()[~special] + tiny(dtype), "one key")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_cross_attention_keys_far_apart(dtype):
+    # Keys 2^26 elements apart: inside one tile their byte offsets pass 2^32.
+    skv, step = 40, 1 << 26
+    flat = torch.empty((skv - 1) * step + 256, dtype=TYPE[dtype], device="cuda")
+    kv = flat.as_strided((1, skv, 4, 64), (0, step, 64, 1))
+    kv.copy_(randn(1, 1, skv, 4, 64, dtype=dtype))
+    k, v = kv[:, :, :2], kv[:, :, 2:]
+    for sq in (1, 66):
+        q, out = randn(2, 1, sq, 2, 64, dtype=dtype), torch.empty(1, sq, 2, 64, dtype=TYPE[dtype], device="cuda")
+        run_cross(q, k, v, out, dtype)
+        check_cross(out, q, k, v, dtype)
+
+
 # ---- the half block they make up ----------------------------------------------------------------
 class HalfBlock:
     """x + g * (cross(rope(norm(x) Wq + bq), states Wk, states Wv) Wo), each step one operator."""
