@@ -106,7 +106,8 @@ __device__ __forceinline__ typename Op8<T>::type read_v(const unsigned char* til
 
 // N operands read from LDS and used, in their order.  In the 16-bit forms two are read ahead of the products; the compiler
 // by itself reads one at a time, each with its full latency (483 against 464 us at 32 x 750 x 4100 x 20 heads).
-template <typename T, int N, typename R, typename U>
+// FENCE: in this order also in f32, where the compiler would hold as many as it can.
+template <typename T, int N, bool FENCE = sizeof(T) == 2, typename R, typename U>
 __device__ __forceinline__ void read_ahead(R read, U use) {
     constexpr int CH = sizeof(T) == 2 ? 2 : 1;
     static_assert(N % CH == 0, "whole chunks");
@@ -115,11 +116,11 @@ __device__ __forceinline__ void read_ahead(R read, U use) {
     for (int i = 0; i < CH; i++) f[0][i] = read(i);
 #pragma unroll
     for (int c = 0; c < N / CH; c++) {
-        if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
         if (c + 1 < N / CH)
 #pragma unroll
             for (int i = 0; i < CH; i++) f[(c + 1) & 1][i] = read((c + 1) * CH + i);
-        if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < CH; i++) use(c * CH + i, f[c & 1][i]);
     }
@@ -195,6 +196,12 @@ __device__ __forceinline__ TileWord tile_word(const uint8_t* mask, int len, int 
 __device__ __forceinline__ float bit_select(int on, float a, float b) {
     return __builtin_bit_cast(float, __builtin_amdgcn_bitop3_b32((unsigned)on, __builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b),
                                                                  0xCA));
+}
+// a b rounded by itself, not inside a multiply-add.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+    const float p = a * b;
+    return p;
 }
 // s + a + b in f32.
 __device__ __forceinline__ float add_pair(bf16 a, bf16 b, float s) {
@@ -392,54 +399,56 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
                 const int li = j * KW + kw;
                 if (li >= nact) continue;  // this group has no tile in the last step
                 const unsigned char* vt = kt + VOFF;
-                f32x16 s[KB];
-#pragma unroll
-                for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
-                constexpr int KS = DH / 16;
-                read_ahead<T, KB * KS>([&](int i) { return read_k<T, DH>(kt, i / KS, i % KS, fr, fh); },
-                                       [&](int i, V8 f) { s[i / KS] = mma<T>(f, qf[i % KS], s[i / KS]); });
                 const unsigned word[2] = {(unsigned)__builtin_amdgcn_readlane(tw.lo, li),
                                           (unsigned)__builtin_amdgcn_readlane(tw.hi, li)};
-                if ((KB == 2 ? word[0] & word[1] : word[0]) != 0xffffffffu) {  // keys 32 kb + 8 g + 4 fh + i of this lane
+                f32x16 s[KB];
+                auto scores = [&](auto fence) {
 #pragma unroll
-                    for (int kb = 0; kb < KB; kb++) {
-                        const int wd = (int)(word[kb] >> (4 * fh));
+                    for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            s[kb][e] = bit_select(__builtin_amdgcn_sbfe(wd, 8 * (e >> 2) + (e & 3), 1), s[kb][e], masked);
+                        for (int e = 0; e < 16; e++) s[kb][e] = 0.f;
+                    constexpr int KS = DH / 16;
+                    read_ahead<T, KB * KS, decltype(fence)::value>([&](int i) { return read_k<T, DH>(kt, i / KS, i % KS, fr, fh); },
+                                           [&](int i, V8 f) { s[i / KS] = mma<T>(f, qf[i % KS], s[i / KS]); });
+                    if ((KB == 2 ? word[0] & word[1] : word[0]) != 0xffffffffu) {  // keys 32 kb + 8 g + 4 fh + i of this lane
+#pragma unroll
+                        for (int kb = 0; kb < KB; kb++) {
+                            const int wd = (int)(word[kb] >> (4 * fh));
+#pragma unroll
+                            for (int e = 0; e < 16; e++) {
+                                s[kb][e] = bit_select(__builtin_amdgcn_sbfe(wd, 8 * (e >> 2) + (e & 3), 1), s[kb][e], masked);
+                            }
                         }
                     }
-                }
-                // Largest of f(score) of the row over the tile.
-                auto tile_max = [&](auto f) {
+                };
+                scores(std::integral_constant<bool, sizeof(T) == 2>{});
+                // Largest of the row's scores over the tile, in the softmax's units.
+                auto tile_max = [&]() {
                     float mx = -INFINITY;
 #pragma unroll
                     for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) mx = fmaxf(mx, f(s[kb][e]));
+                        for (int e = 0; e < 16; e++) mx = fmaxf(mx, rounded_product(s[kb][e], c));
                     return max_halves(mx);
                 };
                 if (first) {
                     // (A row whose scores are all -inf so far adds nothing at any m, and must not keep one.)
-                    const float t = tile_max([&](float x) { return x * c; });
+                    const float t = tile_max();
                     if (unset && t != -INFINITY) {
                         m = t;
                         unset = false;
                     }
                     first = __any(unset);
                 }
-                // The scores become their distances f(s) from the reference, which alone stay live.
+                // The scores become their distances from the reference, which alone stay live.
                 V8 pf[2 * KB];
-                auto exps = [&](auto f) {
+                auto exps = [&](auto distance) {
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            s[kb][e] = f(s[kb][e]);
-                            const float p = fast_exp2(s[kb][e]);
+                            const float p = fast_exp2(distance(s[kb][e]));
                             pf[2 * kb + (e >> 3)][e & 7] = static_cast<T>(p);
                             if (sizeof(T) == 4) sum[e & 3] += p;
                         }
@@ -457,13 +466,16 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
                 if (over) {
                     // Lanes l and l ^ 32 hold one row's two key halves: either one asks for both.
                     const bool need = ((over >> lane) | (over >> (lane ^ 32))) & 1ull;
-                    const float mx = tile_max([](float x) { return x; });
-                    const float shift = need ? mx : 0.f, corr = fast_exp2(-shift);
-                    m += shift;
+                    // The scores are formed again: a distance from a reference far below has lost them in its rounding.  And the new
+                    // distances are those of rounded products, as the reference is one: beside a product above 2^28 its
+                    // rounding alone could exceed the slack.
+                    scores(std::true_type{});
+                    const float mx = tile_max(), mn = need ? fmaxf(m, mx) : m, corr = fast_exp2(m - mn);
+                    m = mn;
 #pragma unroll
                     for (int db = 0; db < DB; db++) o[db] *= corr;
                     l_run *= corr;
-                    psum = exps([&](float x) { return x - shift; });
+                    psum = exps([&](float x) { return rounded_product(x, c) - m; });
                 }
                 l_run += psum;
                 read_ahead<T, 2 * KB * DB>([&](int i) { return read_v<T, DH>(vt, i / DB, i % DB, lane); },

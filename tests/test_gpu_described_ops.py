@@ -575,6 +575,20 @@ def test_cross_attention_keys_far_apart(dtype):
         check_cross(out, q, k, v, dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sq,skv,low", [(1, 9000, 6000), (40, 600, 200), (300, 600, 64), (3, 100, 99)])
+def test_cross_attention_first_scores_far_below_the_rest(dtype, sq, skv, low):
+    """Keys that a first component puts out of reach come first: the softmax of the others loses nothing by it."""
+    big = 60000.0 if dtype == "f16" else 1e15
+    q, k, v = (randn(i, 2, n, 2, 64, dtype=dtype) for i, n in ((1, sq), (2, skv), (3, skv)))
+    q[..., 0] = big
+    k[..., 0] = 0
+    k[:, :low, :, 0] = -big
+    out = torch.empty_like(q)
+    run_cross(q, k, v, out, dtype)
+    check_cross(out, q, k[:, low:], v[:, low:], dtype)
+
+
 # ---- the half block they make up ----------------------------------------------------------------
 class HalfBlock:
     """x + g * (cross(rope(norm(x) Wq + bq), states Wk, states Wv) Wo), each step one operator."""
