@@ -313,6 +313,22 @@ def test_linear_broadcast_rows_and_specials():
     close(y[rest], ref, tol)
 
 
+@pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("m", [16, 300])
+def test_linear_tanh_of_small_arguments(dtype, out, m):
+    """Relative to the result, however small: the argument is one exact product."""
+    n = 64
+    z = torch.logspace(-30, 1.2, m, dtype=torch.float64).to(TYPE[dtype]).cuda()
+    z[::2] *= -1
+    w = torch.ones(n, 1, dtype=TYPE[dtype], device="cuda")
+    y = torch.empty(m, n, dtype=TYPE[out], device="cuda")
+    run_linear(z[:, None].contiguous(), w, y, dtype, out, "tanh")
+    ref = torch.tanh(z.double())[:, None].expand(m, n)
+    # z + z^3 P(z^2) is off by 2 F (6 with one coefficient).  1 - t: t has an exponential of a rounded argument, a sum and a
+    # reciprocal, 6 F of it, and there is less of it than 1.2 of the result from 1/2 on (15 from 1/16 on); then a rounding.
+    close(y, ref, ((10 if out == "f32" else 90) * F + u(out)) * ref.abs() + tiny(out), "tanh")
+
+
 # ---- cross attention --------------------------------------------------------------------------
 def run_cross(q, k, v, out, dtype, mask=None, q_len=None, kv_len=None, scale=None):
     b, sq, h, d = q.shape
