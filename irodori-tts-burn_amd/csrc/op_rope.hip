@@ -163,16 +163,18 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 constexpr double kMaxTurns = 1048576.;
 bool make_turns(const irodori_rope_desc& d, double* turns) {
     const int n = d.rot_dim / 2;
-    double theta = d.theta;
-    if (d.scaling == IRODORI_ROPE_NTK) theta *= std::pow(d.factor, d.rot_dim / (d.rot_dim - 2.0));
-    const double ratio = std::pow(theta, -2.0 / d.rot_dim);
-    double f = 0.15915494309189535;  // 1 / 2 pi; the product's error stays below n 2^-53
+    // Powers by products in the host's 64-bit significands, which leave float64's own rounding; products in float64 lose up
+    // to 2 n 2^-53 (2.5e-6 radians at position 2^28 with 256 pairs and a theta of 1.5).
+    long double theta = d.theta;
+    if (d.scaling == IRODORI_ROPE_NTK) theta *= std::pow((long double)d.factor, d.rot_dim / (d.rot_dim - 2.0L));
+    const long double ratio = std::pow(theta, -2.0L / d.rot_dim);
+    long double f = 0.159154943091895335768884L;  // 1 / 2 pi
     for (int p = 0; p < n; p++, f *= ratio) {
-        double t = f;
+        double t = (double)f;
         if (d.scaling == IRODORI_ROPE_LINEAR) {
             t /= d.factor;
         } else if (d.scaling == IRODORI_ROPE_BY_PARTS) {
-            const double whole = d.trained_len * f;  // turns over the trained length
+            const double whole = d.trained_len * (double)f;  // turns over the trained length
             const double keep = std::min(1.0, std::max(0.0, (whole - d.beta_slow) / (d.beta_fast - d.beta_slow)));
             t *= keep + (1.0 - keep) / d.factor;
         }

@@ -182,6 +182,19 @@ def test_rope_lengths_below_zero():
     assert (flat[b * s * h * d:] == CANARY).all()
 
 
+@pytest.mark.parametrize("theta,kw", [(10000.0, dict()), (1.5, dict()), (1.5, dict(scaling="ntk", factor=2.0))])
+@pytest.mark.parametrize("layout", ["interleaved", "halves"])
+def test_rope_far_positions_of_many_pairs(theta, kw, layout):
+    # 2^28 times a frequency of half a radian: the frequencies of all 256 pairs have to hold float64 (2^28 2^-53 is F / 2).
+    pos = torch.tensor([[2 ** 28 - 1, 2 ** 27 + 1, 12345678, -(2 ** 28)]], dtype=torch.int32, device="cuda")
+    x = randn(4, 1, 4, 2, 512)
+    y = torch.empty_like(x)
+    ih.ops.rope(ih.RopeDesc(1, 4, 512, heads=2, dtype="f32", theta=theta, layout=layout, **kw), ptr(x), ptr(y), d_positions=ptr(pos),
+                stream=stream())
+    ref, mag = rope_ref(x, pos, rope_freq(512, theta, **kw), layout, 2)
+    close(y, ref, rope_tol(ref, mag, "f32"))
+
+
 # ---- linear layer -----------------------------------------------------------------------------
 ACTS = {
     "none": lambda z: z, "relu": torch.relu, "silu": torch.nn.functional.silu, "sigmoid": torch.sigmoid, "tanh": torch.tanh,
