@@ -270,9 +270,10 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
         hk = id % a.kv_heads;
         b = id / a.kv_heads;
     }
-    // c = 0 would turn a masked key's -inf into NaN; the smallest normal gives the same exp2(0).
+    // c = 0 would turn a masked key's -inf into NaN: the queries are multiplied by it instead.
     float c = a.scale * 1.4426950408889634f;
-    c = fabsf(c) < 1.1754944e-38f ? 1.1754944e-38f : c;
+    const bool zero = c == 0.f;
+    if (zero) c = 1.f;
     const float masked = c > 0.f ? -INFINITY : INFINITY;  // the score that vanishes
     // Load instruction ii of this wave in a stage: rows RPI (row0 + ii) .. of tile `tile` of the step's;
     // lane -> row lane / CH, physical chunk lane % CH.
@@ -326,6 +327,10 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
             const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + tok * a.qs[1] + head * a.qs[2] + 8 * fh;
 #pragma unroll
             for (int ks = 0; ks < DH / 16; ks++) qf[ks] = __builtin_bit_cast(V8, *reinterpret_cast<const Q8*>(qp + 16 * ks));
+            if (zero) {
+#pragma unroll
+                for (int ks = 0; ks < DH / 16; ks++) qf[ks] *= static_cast<T>(0.f);
+            }
         }
         f32x16 o[DB];
 #pragma unroll

@@ -618,6 +618,19 @@ def test_cross_attention_first_scores_far_below_the_rest(dtype, sq, skv, low):
     check_cross(out, q, k[:, low:], v[:, low:], dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.0, 1e-42])
+def test_cross_attention_scales_next_to_zero(dtype, scale):
+    # However large the products, 0 times them is 0, and so is the lowest scale times them nearly.
+    big = 60000.0 if dtype == "f16" else 2e18
+    q, k, v = (randn(i, 2, n, 2, 64, dtype=dtype) for i, n in ((1, 5), (2, 300), (3, 300)))
+    q, k = q.sign() * big, k.sign() * big
+    out = torch.empty_like(q)
+    mask = (torch.rand(2, 300, generator=torch.Generator().manual_seed(3)) < 0.6).to(torch.uint8).cuda()
+    run_cross(q, k, v, out, dtype, mask=mask, scale=scale)
+    check_cross(out, q, k, v, dtype, mask=mask, scale=scale)
+
+
 # ---- the half block they make up ----------------------------------------------------------------
 class HalfBlock:
     """x + g * (cross(rope(norm(x) Wq + bq), states Wk, states Wv) Wo), each step one operator."""
