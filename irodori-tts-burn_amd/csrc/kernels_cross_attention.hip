@@ -670,10 +670,21 @@ int launch_cross(const CrossArgs& a, hipStream_t st) {
     if constexpr (!F32 && DH == 128) {
         if (a.splits > 1) return launch_cfg<T, DH, 2, 1, 1, false>(a, st);
     }
-    // Where 64 rows a workgroup with two key groups take more than the one round that fits the chip, 128 rows
-    // with one: at 750 queries x 1381 keys x 16 heads (bf16, 64-dim) 21.4 against 27.1 us for 2 batch rows, 34.6 against
-    // 32.7 for 4, 59 against 47 for 8; 10 heads of 128 dimensions 26.9 / 39.4, 51.8 / 41.3 and 102 / 54.
     if (a.splits > 1 || row_groups(a.batch, a.kv_heads, a.rows) <= 256 * SMALL) return launch_cfg<T, DH, 2, 2, SMALL, false>(a, st);
+    // More workgroups than the one round that fits the chip.  Where a key head has 64 rows at most, wider ones would hold rows
+    // that do not exist.  16-bit: two wavefronts, one key group (32 batch rows x 20 heads, one row over 100 / 600 / 4100 keys,
+    // 64-dim 7.7 / 19.6 / 130 us, against 8.4 / 22.3 / 134 with 128 rows a workgroup and 10.1 / 23.3 / 156 with two key groups;
+    // 10 x 64 x 64 rows over 1000 keys 29, 38, 36 us, 128-dim 76, 82, 84).  f32, bound by the matrix cores: two key groups
+    // (128-dim, 32 x 20 x one row over 100 / 600 / 4100 keys 46 / 166 / 979 against 56 / 231 / 1510 us; 64-dim, 128 x 4 x 64 rows
+    // over 600 keys 52 against 84).
+    if (a.rows <= 64) {
+        if constexpr (F32) return launch_cfg<T, DH, 2, 2, SMALL, false>(a, st);
+        else return launch_cfg<T, DH, 2, 1, SMALL, false>(a, st);
+    }
+    // 128 rows a workgroup with one key group: at 750 queries x 1381 keys x 16 heads (bf16, 64-dim), against 64 rows with two,
+    // 21.4 / 27.1 us for 2 batch rows, 34 / 31 for 4, 46 / 55 for 8; 8 heads of 128 dimensions, 4 and 8 batch rows, 31 / 42 and
+    // 49 / 64; in f32 186 / 150 and 271 / 291, 128-dim 189 / 203 and 350 / 306; 32 x 20 x 130 rows over 1000 keys 56 / 57, f32
+    // 329 / 287.
     return launch_cfg<T, DH, 4, 1, DH == 64 && !F32 ? 3 : 2, false>(a, st);
 }
 

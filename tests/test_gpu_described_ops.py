@@ -631,6 +631,31 @@ def test_cross_attention_scales_next_to_zero(dtype, scale):
     check_cross(out, q, k, v, dtype, mask=mask, scale=scale)
 
 
+@pytest.mark.parametrize("d,sq", [(64, 40), (128, 1), (128, 40)])
+def test_cross_attention_few_rows_do_not_depend_on_the_batch(d, sq):
+    # However many batch rows: 64 rows a workgroup, in two key groups (and not 128, most of which would not exist).
+    b, skv, h, dtype = 40, 900, 20, "f32"
+    q, k, v = randn(1, b, sq, h, d, dtype=dtype), randn(2, b, skv, h, d, dtype=dtype), randn(3, b, skv, h, d, dtype=dtype)
+    out, few = torch.empty_like(q), torch.empty_like(q[:10])
+    for n, o in ((b, out), (10, few)):
+        assert ih.ops.cross_attention_workspace(ih.CrossAttentionDesc(n, sq, skv, h, h, d, dtype=dtype)) == 0
+        run_cross(q[:n], k[:n], v[:n], o, dtype)
+    assert torch.equal(out[:10], few)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq,h,hk", [(1, 20, 20), (9, 80, 20), (64, 20, 20), (65, 20, 20)])
+def test_cross_attention_many_batch_rows(dtype, d, sq, h, hk):
+    b, skv = 27, 133
+    q, k, v = randn(1, b, sq, h, d, dtype=dtype), randn(2, b, skv, hk, d, dtype=dtype), randn(3, b, skv, hk, d, dtype=dtype)
+    lens = torch.tensor([(skv - 17 * i) % (skv + 1) for i in range(b)], dtype=torch.int32, device="cuda")
+    mask = (torch.rand(b, skv, generator=torch.Generator().manual_seed(3)) < 0.6).to(torch.uint8).cuda()
+    out = torch.full((b, sq, h, d), CANARY, dtype=TYPE[dtype], device="cuda")
+    run_cross(q, k, v, out, dtype, mask=mask, kv_len=lens)
+    check_cross(out, q, k, v, dtype, mask=mask, kv_len=lens)
+
+
 # ---- the half block they make up ----------------------------------------------------------------
 class HalfBlock:
     """x + g * (cross(rope(norm(x) Wq + bq), states Wk, states Wv) Wo), each step one operator."""
