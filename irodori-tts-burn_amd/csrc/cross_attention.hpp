@@ -27,8 +27,8 @@ inline int64_t cross_partial_bytes(int splits, int batch, int kv_heads, int rows
     return splits > 1 ? ((int64_t)splits + batch) * kv_heads * rows * (head_dim + 2) * 4 : 0;
 }
 
-// 0, or -1 where the grid would not fit one launch (2^32 threads).
+// 0, or -1 where the grid would not fit one launch (2^32 threads).  go: false only answers.
 template <typename T, int DH>
-int launch_cross(const CrossArgs& a, hipStream_t st);
+int launch_cross(const CrossArgs& a, hipStream_t st, bool go);
 
 }  // namespace irodori

@@ -623,11 +623,12 @@ __global__ __launch_bounds__(64) void cross_join_kernel(CrossArgs a) {
 }
 
 template <typename T, int DH, int QW, int KW, int WPE, bool UNAL>
-int launch_cfg(const CrossArgs& a, hipStream_t st) {
+int launch_cfg(const CrossArgs& a, hipStream_t st, bool go) {
     const int rbs = (int)(((int64_t)a.rows + 32 * QW - 1) / (32 * QW));
     const int64_t wgs = (int64_t)rbs * a.kv_heads * (a.splits > 1 ? a.splits : a.batch);
     const int64_t joins = (int64_t)a.batch * a.kv_heads * a.rows;
     if (wgs > UINT32_MAX / (64 * QW * KW) || (a.splits > 1 && joins > UINT32_MAX / 64)) return -1;
+    if (!go) return 0;
     cross_kernel<T, DH, QW, KW, WPE, UNAL><<<(unsigned)wgs, 64 * QW * KW, 0, st>>>(a, rbs);
     if (a.splits > 1) cross_join_kernel<T, DH><<<(unsigned)joins, 64, 0, st>>>(a);
     return 0;
@@ -650,7 +651,7 @@ int cross_splits(bool f32, int batch, int kv_heads, int rows, int seq_kv, int he
 }
 
 template <typename T, int DH>
-int launch_cross(const CrossArgs& a, hipStream_t st) {
+int launch_cross(const CrossArgs& a, hipStream_t st, bool go) {
     constexpr int64_t es = sizeof(T);
     constexpr bool F32 = sizeof(T) == 4;
     // Windows of a tile's rows stay below 2^31 bytes, and the buffer-to-LDS loads take dword-aligned rows.  Values
@@ -659,18 +660,18 @@ int launch_cross(const CrossArgs& a, hipStream_t st) {
                       ((a.ks[0] | a.ks[1] | a.ks[2] | a.vs[0] | a.vs[1] | a.vs[2]) * es & 3) ||
                       a.ks[1] * es > (1 << 24) || a.vs[1] * es > (1 << 24) || a.vs[1] < DH;
     constexpr int SMALL = DH == 64 ? 2 : 1;  // wavefronts per SIMD, of two (one) workgroups a CU
-    if (unal) return launch_cfg<T, DH, 2, 2, SMALL, true>(a, st);
+    if (unal) return launch_cfg<T, DH, 2, 2, SMALL, true>(a, st, go);
     // f32 in one block of 32 rows is bound by the matrix cores, most of whose rows are padding: a group on every SIMD
     // (38 against 51 us at 8 x 4 key heads x 1 x 8200; at 128-dim the rings do not fit).
     if constexpr (F32 && DH == 64) {
-        if (a.rows <= 32) return launch_cfg<T, DH, 1, 4, 1, false>(a, st);
+        if (a.rows <= 32) return launch_cfg<T, DH, 1, 4, 1, false>(a, st, go);
     }
     // Runs of 128-dim heads in two workgroups a CU, which hide each other's ends, rather than one with two
     // key groups (27.2 against 30.0 us at 8 x 4 key heads x 1 x 8200; 64-dim heads fit two a CU either way).
     if constexpr (!F32 && DH == 128) {
-        if (a.splits > 1) return launch_cfg<T, DH, 2, 1, 1, false>(a, st);
+        if (a.splits > 1) return launch_cfg<T, DH, 2, 1, 1, false>(a, st, go);
     }
-    if (a.splits > 1 || row_groups(a.batch, a.kv_heads, a.rows) <= 256 * SMALL) return launch_cfg<T, DH, 2, 2, SMALL, false>(a, st);
+    if (a.splits > 1 || row_groups(a.batch, a.kv_heads, a.rows) <= 256 * SMALL) return launch_cfg<T, DH, 2, 2, SMALL, false>(a, st, go);
     // More workgroups than the one round that fits the chip.  Where a key head has 64 rows at most, wider ones would hold rows
     // that do not exist.  16-bit: two wavefronts, one key group (32 batch rows x 20 heads, one row over 100 / 600 / 4100 keys,
     // 64-dim 7.7 / 19.6 / 130 us, against 8.4 / 22.3 / 134 with 128 rows a workgroup and 10.1 / 23.3 / 156 with two key groups;
@@ -678,21 +679,21 @@ int launch_cross(const CrossArgs& a, hipStream_t st) {
     // (128-dim, 32 x 20 x one row over 100 / 600 / 4100 keys 46 / 166 / 979 against 56 / 231 / 1510 us; 64-dim, 128 x 4 x 64 rows
     // over 600 keys 52 against 84).
     if (a.rows <= 64) {
-        if constexpr (F32) return launch_cfg<T, DH, 2, 2, SMALL, false>(a, st);
-        else return launch_cfg<T, DH, 2, 1, SMALL, false>(a, st);
+        if constexpr (F32) return launch_cfg<T, DH, 2, 2, SMALL, false>(a, st, go);
+        else return launch_cfg<T, DH, 2, 1, SMALL, false>(a, st, go);
     }
     // 128 rows a workgroup with one key group: at 750 queries x 1381 keys x 16 heads (bf16, 64-dim), against 64 rows with two,
     // 21.4 / 27.1 us for 2 batch rows, 34 / 31 for 4, 46 / 55 for 8; 8 heads of 128 dimensions, 4 and 8 batch rows, 31 / 42 and
     // 49 / 64; in f32 186 / 150 and 271 / 291, 128-dim 189 / 203 and 350 / 306; 32 x 20 x 130 rows over 1000 keys 56 / 57, f32
     // 329 / 287.
-    return launch_cfg<T, DH, 4, 1, DH == 64 && !F32 ? 3 : 2, false>(a, st);
+    return launch_cfg<T, DH, 4, 1, DH == 64 && !F32 ? 3 : 2, false>(a, st, go);
 }
 
-template int launch_cross<bf16, 64>(const CrossArgs&, hipStream_t);
-template int launch_cross<bf16, 128>(const CrossArgs&, hipStream_t);
-template int launch_cross<f16, 64>(const CrossArgs&, hipStream_t);
-template int launch_cross<f16, 128>(const CrossArgs&, hipStream_t);
-template int launch_cross<float, 64>(const CrossArgs&, hipStream_t);
-template int launch_cross<float, 128>(const CrossArgs&, hipStream_t);
+template int launch_cross<bf16, 64>(const CrossArgs&, hipStream_t, bool);
+template int launch_cross<bf16, 128>(const CrossArgs&, hipStream_t, bool);
+template int launch_cross<f16, 64>(const CrossArgs&, hipStream_t, bool);
+template int launch_cross<f16, 128>(const CrossArgs&, hipStream_t, bool);
+template int launch_cross<float, 64>(const CrossArgs&, hipStream_t, bool);
+template int launch_cross<float, 128>(const CrossArgs&, hipStream_t, bool);
 
 }  // namespace irodori

@@ -663,20 +663,20 @@ __global__ __launch_bounds__(64 * NW) void linear_rows_kernel(LinearArgs a) {
 }
 
 template <typename T, typename TO, int MT, int NW>
-int launch_rows(const LinearArgs& a, hipStream_t st) {
+int launch_rows(const LinearArgs& a, hipStream_t st, bool go) {
     static_assert(MT <= NW, "a thread per four sums");
     const int64_t wgs = ((int64_t)a.N + 15) / 16;
     if (wgs * (64 * NW) > UINT32_MAX) return -1;
-    linear_rows_kernel<T, TO, MT, NW><<<(unsigned)wgs, 64 * NW, 0, st>>>(a);
+    if (go) linear_rows_kernel<T, TO, MT, NW><<<(unsigned)wgs, 64 * NW, 0, st>>>(a);
     return 0;
 }
 
 template <typename T, typename TO, int BM, int BN, int WM, int WN, int WK, int RB, int STAGES, bool ASYNC>
-int launch_tiles(const LinearArgs& a, hipStream_t st) {
+int launch_tiles(const LinearArgs& a, hipStream_t st, bool go) {
     constexpr int THREADS = 64 * WM * WN * WK;
     const int64_t wgs = (int64_t)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
     if (wgs * THREADS > UINT32_MAX) return -1;
-    linear_kernel<T, TO, BM, BN, WM, WN, WK, RB, STAGES, ASYNC><<<(unsigned)wgs, THREADS, 0, st>>>(a);
+    if (go) linear_kernel<T, TO, BM, BN, WM, WN, WK, RB, STAGES, ASYNC><<<(unsigned)wgs, THREADS, 0, st>>>(a);
     return 0;
 }
 
@@ -726,9 +726,9 @@ int best_tiles(const TileCost (&t)[N], const LinearArgs& a) {
 }  // namespace
 
 template <typename T, typename TO>
-int launch_linear(const LinearArgs& a, hipStream_t st) {
+int launch_linear(const LinearArgs& a, hipStream_t st, bool go) {
     // One new token or a few: 4.0 against 5.0 to 6.2 us with 32 x 32 tiles at 16 x 1024 x 1024 (bf16).
-    if (a.M <= 16) return launch_rows<T, TO, 1, 8>(a, st);
+    if (a.M <= 16) return launch_rows<T, TO, 1, 8>(a, st, go);
     // The buffer-to-LDS loads take dword-aligned rows, and windows of a tile's rows below 2^31 bytes.
     constexpr int64_t ES = sizeof(T), FAR = (int64_t)1 << 22;
     const bool async = !((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx * ES | a.ldw * ES) & 3) &&
@@ -737,30 +737,30 @@ int launch_linear(const LinearArgs& a, hipStream_t st) {
         // Through registers (16-bit rows an odd number of elements apart): 64 x 64 against 128 x 128 tiles 12.5 / 24.6 us at
         // 500 x 1024 x 1001 (32 tiles of 128), 24.4 / 33.9 at 1536 x 2048 (192), 36.9 / 26.3 at 2048 x 2048 (256), 786 / 552 at
         // 20000 x 5632.
-        if (((int64_t)a.M + 127) / 128 * ((a.N + 127) / 128) < 200) return launch_tiles<T, TO, 64, 64, 2, 2, 2, 128, 2, false>(a, st);
-        return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, false>(a, st);
+        if (((int64_t)a.M + 127) / 128 * ((a.N + 127) / 128) < 200) return launch_tiles<T, TO, 64, 64, 2, 2, 2, 128, 2, false>(a, st, go);
+        return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, false>(a, st, go);
     }
     if constexpr (sizeof(T) == 4) {
         switch (best_tiles(kTiles32, a)) {
-            case 0: return launch_tiles<T, TO, 32, 32, 1, 1, 4, 256, 2, true>(a, st);
-            case 1: return launch_tiles<T, TO, 64, 64, 2, 2, 2, 256, 2, true>(a, st);
-            default: return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, true>(a, st);
+            case 0: return launch_tiles<T, TO, 32, 32, 1, 1, 4, 256, 2, true>(a, st, go);
+            case 1: return launch_tiles<T, TO, 64, 64, 2, 2, 2, 256, 2, true>(a, st, go);
+            default: return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, true>(a, st, go);
         }
     } else {
         switch (best_tiles(kTiles16, a)) {
-            case 0: return launch_tiles<T, TO, 32, 32, 1, 1, 4, 256, 3, true>(a, st);
-            case 1: return launch_tiles<T, TO, 64, 64, 2, 2, 2, 256, 2, true>(a, st);
-            case 2: return launch_tiles<T, TO, 128, 64, 4, 2, 1, 128, 3, true>(a, st);
-            case 3: return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, true>(a, st);
-            default: return launch_tiles<T, TO, 256, 256, 2, 4, 1, 128, 2, true>(a, st);
+            case 0: return launch_tiles<T, TO, 32, 32, 1, 1, 4, 256, 3, true>(a, st, go);
+            case 1: return launch_tiles<T, TO, 64, 64, 2, 2, 2, 256, 2, true>(a, st, go);
+            case 2: return launch_tiles<T, TO, 128, 64, 4, 2, 1, 128, 3, true>(a, st, go);
+            case 3: return launch_tiles<T, TO, 128, 128, 4, 2, 1, 128, 2, true>(a, st, go);
+            default: return launch_tiles<T, TO, 256, 256, 2, 4, 1, 128, 2, true>(a, st, go);
         }
     }
 }
 
-template int launch_linear<bf16, bf16>(const LinearArgs&, hipStream_t);
-template int launch_linear<bf16, float>(const LinearArgs&, hipStream_t);
-template int launch_linear<f16, f16>(const LinearArgs&, hipStream_t);
-template int launch_linear<f16, float>(const LinearArgs&, hipStream_t);
-template int launch_linear<float, float>(const LinearArgs&, hipStream_t);
+template int launch_linear<bf16, bf16>(const LinearArgs&, hipStream_t, bool);
+template int launch_linear<bf16, float>(const LinearArgs&, hipStream_t, bool);
+template int launch_linear<f16, f16>(const LinearArgs&, hipStream_t, bool);
+template int launch_linear<f16, float>(const LinearArgs&, hipStream_t, bool);
+template int launch_linear<float, float>(const LinearArgs&, hipStream_t, bool);
 
 }  // namespace irodori

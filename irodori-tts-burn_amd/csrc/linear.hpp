@@ -17,8 +17,8 @@ struct LinearArgs {
     int M, N, K, act, gate_rows;
 };
 
-// 0, or -1 where the grid would not fit one launch (2^32 threads).
+// 0, or -1 where the grid would not fit one launch (2^32 threads).  go: false only answers.
 template <typename T, typename TO>
-int launch_linear(const LinearArgs& a, hipStream_t st);
+int launch_linear(const LinearArgs& a, hipStream_t st, bool go);
 
 }  // namespace irodori

@@ -38,8 +38,22 @@ int64_t bytes_of(const irodori_cross_attention_desc& d, int splits) {
 }
 
 template <typename T>
-int run(const CrossArgs& a, int head_dim, hipStream_t st) {
-    return head_dim == 64 ? launch_cross<T, 64>(a, st) : launch_cross<T, 128>(a, st);
+int run(const CrossArgs& a, int head_dim, hipStream_t st, bool go) {
+    return head_dim == 64 ? launch_cross<T, 64>(a, st, go) : launch_cross<T, 128>(a, st, go);
+}
+
+// out or the workspace over something that is read, or over one another.
+bool outputs_overlap(const irodori_cross_attention_desc& d, const CrossArgs& a, int64_t workspace) {
+    const size_t es = dtype_bytes(d.dtype);
+    const int64_t nq[3] = {d.batch, d.seq_q, d.heads}, nk[3] = {d.batch, d.seq_kv, d.kv_heads}, nm[3] = {d.batch, 1, 1},
+                  sm[3] = {d.mask_stride};
+    const Box out(a.out, es, nq, d.out_strides, d.head_dim), ws(workspace ? a.partial : nullptr, workspace);
+    const Box in[] = {Box(a.q, es, nq, d.q_strides, d.head_dim), Box(a.k, es, nk, d.k_strides, d.head_dim),
+                      Box(a.v, es, nk, d.v_strides, d.head_dim), Box(a.mask, 1, nm, sm, d.seq_kv),
+                      Box(a.q_len, (int64_t)4 * d.batch), Box(a.kv_len, (int64_t)4 * d.batch)};
+    for (const Box& x : in)
+        if (overlap(out, x) || overlap(ws, x)) return true;
+    return overlap(out, ws);
 }
 
 }  // namespace
@@ -90,11 +104,13 @@ int irodori_op_cross_attention(const irodori_cross_attention_desc* desc, const v
     a.seq_q = d.seq_q; a.seq_kv = d.seq_kv; a.splits = splits;
     a.rows = d.seq_q * a.group;
     a.scale = d.scale;
+    const bool apart = !outputs_overlap(d, a, need);
     int rc;
-    if (d.dtype == IRODORI_DTYPE_BF16) rc = run<bf16>(a, d.head_dim, st);
-    else if (d.dtype == IRODORI_DTYPE_F16) rc = run<f16>(a, d.head_dim, st);
-    else rc = run<float>(a, d.head_dim, st);
+    if (d.dtype == IRODORI_DTYPE_BF16) rc = run<bf16>(a, d.head_dim, st, apart);
+    else if (d.dtype == IRODORI_DTYPE_F16) rc = run<f16>(a, d.head_dim, st, apart);
+    else rc = run<float>(a, d.head_dim, st, apart);
     IRO_REQUIRE(rc == 0, IRODORI_ERR_SHAPE, "irodori_op_cross_attention: too many rows for one launch");
+    IRO_REQUIRE(apart, IRODORI_ERR_INVALID_ARG, "irodori_op_cross_attention: out or the workspace overlaps another argument");
     return check_launch("cross attention");
     IRO_GUARD_END
 }

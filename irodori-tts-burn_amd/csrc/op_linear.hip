@@ -27,6 +27,15 @@ int check_linear(const irodori_linear_desc* dp) {
     return IRODORI_OK;
 }
 
+// y over something that is read (it may be the residual itself).
+bool y_overlaps(const irodori_linear_desc& d, const LinearArgs& a) {
+    const size_t es = dtype_bytes(d.dtype), eo = dtype_bytes(d.out_dtype);
+    const int64_t nm[3] = {d.m, 1, 1}, nn[3] = {d.n, 1, 1}, sx[3] = {d.ldx}, sw[3] = {d.ldw}, sy[3] = {d.ldy}, sr[3] = {d.ldr};
+    const Box y(a.y, eo, nm, sy, d.n), x(a.x, es, nm, sx, d.k), w(a.w, es, nn, sw, d.k), r(a.residual, eo, nm, sr, d.n);
+    const Box bias(a.bias, (int64_t)4 * d.n), gate(a.gate, a.gate ? ((int64_t)d.m + d.gate_rows - 1) / d.gate_rows * d.n * 4 : 0);
+    return overlap(y, x) || overlap(y, w) || (a.residual != a.y && overlap(y, r)) || overlap(y, bias) || overlap(y, gate);
+}
+
 }  // namespace
 
 extern "C" {
@@ -58,12 +67,15 @@ int irodori_op_linear(const irodori_linear_desc* desc, const void* x, const void
     hipStream_t st = static_cast<hipStream_t>(stream);
     IRO_TRY(check_op_stream(st, "irodori_op_linear"));
     const LinearArgs a{x, w, residual, y, bias, gate, d.ldx, d.ldw, d.ldy, d.ldr, d.m, d.n, d.k, d.activation, d.gate_rows};
-    int rc;
-    if (d.dtype == IRODORI_DTYPE_F32) rc = launch_linear<float, float>(a, st);
-    else if (d.dtype == IRODORI_DTYPE_BF16)
-        rc = d.out_dtype == IRODORI_DTYPE_F32 ? launch_linear<bf16, float>(a, st) : launch_linear<bf16, bf16>(a, st);
-    else rc = d.out_dtype == IRODORI_DTYPE_F32 ? launch_linear<f16, float>(a, st) : launch_linear<f16, f16>(a, st);
-    IRO_REQUIRE(rc == 0, IRODORI_ERR_SHAPE, "irodori_op_linear: too many tiles for one launch");
+    auto launch = [&](bool go) {
+        if (d.dtype == IRODORI_DTYPE_F32) return launch_linear<float, float>(a, st, go);
+        if (d.dtype == IRODORI_DTYPE_BF16)
+            return d.out_dtype == IRODORI_DTYPE_F32 ? launch_linear<bf16, float>(a, st, go) : launch_linear<bf16, bf16>(a, st, go);
+        return d.out_dtype == IRODORI_DTYPE_F32 ? launch_linear<f16, float>(a, st, go) : launch_linear<f16, f16>(a, st, go);
+    };
+    const bool apart = !y_overlaps(d, a);
+    IRO_REQUIRE(launch(apart) == 0, IRODORI_ERR_SHAPE, "irodori_op_linear: too many tiles for one launch");
+    IRO_REQUIRE(apart, IRODORI_ERR_INVALID_ARG, "irodori_op_linear: y overlaps an input");
     return check_launch("linear");
     IRO_GUARD_END
 }

@@ -236,6 +236,17 @@ int check_rope(const irodori_rope_desc* dp) {
 
 unsigned ceil_inv(int d) { return (unsigned)(((1ull << 32) + d - 1) / d); }
 
+// An output over something that is read or over the other one (q_out may be q, and k_out k).
+bool outputs_overlap(const irodori_rope_desc& d, const RopeArgs& a) {
+    const size_t es = dtype_bytes(d.dtype);
+    const int64_t nq[3] = {d.batch, d.seq, d.q_heads}, nk[3] = {d.batch, d.seq, d.k_heads};
+    auto box = [&](const void* p, const int64_t (&n)[3], const int64_t* s) { return Box(n[2] ? p : nullptr, es, n, s, d.head_dim); };
+    const Box q = box(a.q.x, nq, a.q.xs), k = box(a.k.x, nk, a.k.xs), qo = box(a.q.y, nq, a.q.ys), ko = box(a.k.y, nk, a.k.ys);
+    const Box pos(a.positions, (int64_t)4 * d.batch * d.seq), len(a.lengths, (int64_t)4 * d.batch);
+    return (a.q.x != a.q.y && overlap(qo, q)) || (a.k.x != a.k.y && overlap(ko, k)) || overlap(qo, k) || overlap(ko, q) ||
+           overlap(qo, ko) || overlap(qo, pos) || overlap(qo, len) || overlap(ko, pos) || overlap(ko, len);
+}
+
 template <typename T, int V, bool HALVES>
 int launch(const irodori_rope_desc& d, RopeArgs& a, hipStream_t st) {
     const int total = a.q.heads + a.k.heads, most = 256 * kItems;
@@ -253,6 +264,7 @@ int launch(const irodori_rope_desc& d, RopeArgs& a, hipStream_t st) {
     a.div_heads = ceil_inv(a.heads);
     const int64_t wgs = (int64_t)d.batch * a.tok_blocks * a.head_blocks;
     IRO_REQUIRE(wgs <= UINT32_MAX / 256, IRODORI_ERR_SHAPE, "irodori_op_rope: too many tokens for one launch");
+    IRO_REQUIRE(!outputs_overlap(d, a), IRODORI_ERR_INVALID_ARG, "irodori_op_rope: an output overlaps another argument");
     rope_kernel<T, V, HALVES><<<(unsigned)wgs, 256, 0, st>>>(a);
     return check_launch("rope");
 }

@@ -2,6 +2,7 @@
 refuse, through the C ABI without a device: every call here fails, or answers, before its first
 device call."""
 import ctypes as C
+import itertools
 
 import pytest
 
@@ -162,3 +163,49 @@ def test_outputs_that_are_inputs_are_refused():
         refused("InvalidArg", "y is an input", lambda: ih.ops.linear(linear_desc(), P, 2 * P, at))
     for args in ((P, 2 * P, 3 * P, 2 * P), (P, 3 * P, 3 * P, 4 * P), (P, P, 3 * P, P)):
         refused("InvalidArg", "other side's", lambda: ih.ops.rope(rope_desc(), *args))
+
+
+def rows(at, dims, strides, inner):
+    """The elements of a tensor, as numbers."""
+    return {at + sum(i * s for i, s in zip(index, strides)) + e for index in itertools.product(*map(range, dims)) for e in range(inner)}
+
+
+@pytest.mark.parametrize("heads,between", [(2, 0), (2, 1), (3, 2)])
+def test_rope_refuses_outputs_inside_inputs(heads, between):
+    # q of one head and the next head's place: every offset inside a buffer of heads that shares an element is refused.
+    d, seq, rowlen = 4, 3, (heads + between) * 4
+    strides = (seq * rowlen, rowlen, d)
+    desc = rope_desc(batch=2, seq=seq, head_dim=d, heads=heads, kv_heads=0, dtype="f32", q_strides=strides, q_out_strides=strides)
+    q = rows(0, (2, seq, heads), strides, d)
+    seen = 0
+    for at in range(-2 * seq * rowlen, 2 * seq * rowlen):
+        if at and q & rows(at, (2, seq, heads), strides, d):
+            refused("InvalidArg", "overlaps", lambda: ih.ops.rope(desc, 1 << 20, (1 << 20) + 4 * at))
+            seen += 1
+    assert seen > 2 * seq * heads
+
+
+def test_outputs_that_overlap_other_arguments_are_refused():
+    M = 1 << 20
+    # y: a part of x, of w, of a residual at another place, of the bias and of the gate
+    d = linear_desc(m=64, n=8, k=16, dtype="f32", gate_rows=2)
+    for x, w, kw in ((M - 4 * 63 * 16, 2 * M, {}), (2 * M, M + 64 * 8 * 4 - 4, {}), (2 * M, 3 * M, dict(d_residual=M + 32)),
+                     (2 * M, 3 * M, dict(d_bias=M + 4 * 40)), (2 * M, 3 * M, dict(d_gate=M - 4 * 31 * 8))):
+        gate = kw.get("d_gate", 5 * M)
+        refused("InvalidArg", "y overlaps", lambda: ih.ops.linear(d, x, w, M, **dict(kw, d_gate=gate)))
+    # columns of one buffer, one too far
+    d = linear_desc(m=9, n=8, k=16, ldx=24, ldy=24)
+    refused("InvalidArg", "y overlaps", lambda: ih.ops.linear(d, M, 2 * M, M + 2 * 15))
+    refused("InvalidArg", "y overlaps", lambda: ih.ops.linear(d, M, 2 * M, M - 2 * 7))
+    # out over each input, and the workspace over each and over out
+    d = cross_desc(batch=2, seq_q=1, seq_kv=100000, dtype="f32")
+    need = ih.ops.cross_attention_workspace(d)
+    place = dict(d_q=1 * M, d_k=1024 * M, d_v=2048 * M, d_out=3 * M, d_mask=4 * M, d_q_len=5 * M, d_kv_len=6 * M, d_workspace=7 * M)
+    for name in ("d_q", "d_k", "d_v", "d_mask", "d_q_len", "d_kv_len", "d_workspace"):
+        refused("InvalidArg", "overlaps", lambda: ih.ops.cross_attention(d, **dict(place, d_out=place[name] + 4), workspace_bytes=need))
+    for name in ("d_q", "d_k", "d_v", "d_mask", "d_q_len", "d_kv_len", "d_out"):
+        refused("InvalidArg", "overlaps", lambda: ih.ops.cross_attention(d, **dict(place, d_workspace=place[name] - 16), workspace_bytes=need))
+    d = rope_desc()
+    refused("InvalidArg", "overlaps", lambda: ih.ops.rope(d, M, 2 * M, 3 * M, 4 * M, d_positions=2 * M + 64))
+    refused("InvalidArg", "overlaps", lambda: ih.ops.rope(d, M, 2 * M, 3 * M, 4 * M, d_lengths=4 * M + 64))
+    refused("InvalidArg", "overlaps", lambda: ih.ops.rope(d, M, 2 * M, 3 * M, 2 * M + 64))

@@ -195,6 +195,21 @@ def test_rope_far_positions_of_many_pairs(theta, kw, layout):
     close(y, ref, rope_tol(ref, mag, "f32"))
 
 
+def test_rope_between_heads_of_one_buffer():
+    # From some heads of a buffer into others, and in place beside them: no element is shared.
+    b, s, h, d = 2, 5, 2, 64
+    for at in (0, 2, 4):
+        buf = randn(1, b, s, 6, d)
+        before = buf.clone()
+        q, out = buf[:, :, 2:4], buf[:, :, at:at + h]
+        desc = ih.RopeDesc(b, s, d, heads=h, dtype="f32", q_strides=q.stride()[:3], q_out_strides=out.stride()[:3])
+        ih.ops.rope(desc, ptr(q), ptr(out), stream=stream())
+        ref, mag = rope_ref(before[:, :, 2:4], torch.arange(s, device="cuda").expand(b, s), rope_freq(d), "interleaved", h)
+        close(out, ref, rope_tol(ref, mag, "f32"))
+        rest = [i for i in range(6) if not at <= i < at + h]
+        assert torch.equal(buf[:, :, rest], before[:, :, rest])
+
+
 # ---- linear layer -----------------------------------------------------------------------------
 ACTS = {
     "none": lambda z: z, "relu": torch.relu, "silu": torch.nn.functional.silu, "sigmoid": torch.sigmoid, "tanh": torch.tanh,
@@ -340,6 +355,19 @@ def test_linear_tanh_of_small_arguments(dtype, out, m):
     # z + z^3 P(z^2) is off by 2 F (6 with one coefficient).  1 - t: t has an exponential of a rounded argument, a sum and a
     # reciprocal, 6 F of it, and there is less of it than 1.2 of the result from 1/2 on (15 from 1/16 on); then a rounding.
     close(y, ref, ((10 if out == "f32" else 90) * F + u(out)) * ref.abs() + tiny(out), "tanh")
+
+
+@pytest.mark.parametrize("m", [9, 200])
+def test_linear_between_columns_of_one_buffer(m):
+    # x, y and the residual are columns of one buffer; w stands before it.
+    k, n = 64, 48
+    buf = randn(1, m, k + 2 * n)
+    before, w = buf.clone(), randn(2, n, k, std=k ** -0.5)
+    x, res, y = buf[:, n:n + k], buf[:, n + k:], buf[:, :n]
+    ref = linear_ref(x, w, "f32", "none", None, None, 0, res.clone())
+    run_linear(x, w, y, "f32", "f32", residual=res)
+    close(y, *ref, "columns")
+    assert torch.equal(buf[:, n:], before[:, n:])
 
 
 # ---- cross attention --------------------------------------------------------------------------
@@ -654,6 +682,15 @@ def test_cross_attention_many_batch_rows(dtype, d, sq, h, hk):
     out = torch.full((b, sq, h, d), CANARY, dtype=TYPE[dtype], device="cuda")
     run_cross(q, k, v, out, dtype, mask=mask, kv_len=lens)
     check_cross(out, q, k, v, dtype, mask=mask, kv_len=lens)
+
+
+def test_cross_attention_into_a_part_of_the_queries_buffer():
+    b, sq, skv, h, d = 2, 9, 70, 2, 64
+    buf = randn(1, b, sq, 3 * h, d)
+    before, k, v = buf.clone(), randn(2, b, skv, h, d), randn(3, b, skv, h, d)
+    run_cross(buf[:, :, h:2 * h], k, v, buf[:, :, :h], "f32")
+    check_cross(buf[:, :, :h], before[:, :, h:2 * h], k, v, "f32")
+    assert torch.equal(buf[:, :, h:], before[:, :, h:])
 
 
 # ---- the half block they make up ----------------------------------------------------------------
