@@ -165,9 +165,10 @@ bool make_turns(const irodori_rope_desc& d, double* turns) {
     const int n = d.rot_dim / 2;
     // Powers by products in the host's 64-bit significands, which leave float64's own rounding; products in float64 lose up
     // to 2 n 2^-53 (2.5e-6 radians at position 2^28 with 256 pairs and a theta of 1.5).
-    long double theta = d.theta;
-    if (d.scaling == IRODORI_ROPE_NTK) theta *= std::pow((long double)d.factor, d.rot_dim / (d.rot_dim - 2.0L));
-    const long double ratio = std::pow(theta, -2.0L / d.rot_dim);
+    // (Through logarithms: pow in these numbers takes 0.5 us.)
+    long double log_theta = std::log2((long double)d.theta);
+    if (d.scaling == IRODORI_ROPE_NTK) log_theta += d.rot_dim / (d.rot_dim - 2.0L) * std::log2((long double)d.factor);
+    const long double ratio = std::exp2(-2.0L / d.rot_dim * log_theta);
     long double f = 0.159154943091895335768884L;  // 1 / 2 pi
     for (int p = 0; p < n; p++, f *= ratio) {
         double t = (double)f;
