@@ -12,6 +12,7 @@ Errors map the C status codes onto IrodoriError variants (src/error.rs:4-60).
 from __future__ import annotations
 
 import ctypes as C
+import operator
 
 import numpy as np
 
@@ -540,13 +541,36 @@ def _choice(table, value, what: str) -> int:
     return table[value]
 
 
+def _held(value, bits: int, what: str) -> int:
+    """A number as a signed field of so many bits holds it; ctypes would keep its low bits alone."""
+    value = operator.index(value)
+    if not -(1 << bits - 1) <= value < 1 << bits - 1:
+        raise IrodoriError("Shape", "%s of %d does not fit %d bits" % (what, value, bits))
+    return value
+
+
 def _strides(given, seq: int, heads: int, dim: int):
     """(batch, token, head) strides in elements; None: a contiguous [batch, seq, heads, dim]."""
     if given is None:
         given = (seq * heads * dim, heads * dim, dim)
     if len(given) != 3:
         raise IrodoriError("Shape", "strides are (batch, token, head), got %r" % (given,))
-    return (C.c_int64 * 3)(*given)
+    return (C.c_int64 * 3)(*(_held(x, 64, "a stride") for x in given))
+
+
+_BITS = {C.c_int32: 32, C.c_int64: 64}
+
+
+def _fill(desc, *values) -> None:
+    """The fields of a description, in their order."""
+    for (name, kind), value in zip(desc._fields_, values, strict=True):
+        setattr(desc, name, _held(value, _BITS[kind], name) if kind in _BITS else value)
+
+
+def _workspace_bytes(n) -> int:
+    if n < 0:
+        raise IrodoriError("InvalidArg", "workspace_bytes must not be negative, got %d" % n)
+    return n
 
 
 class RopeDesc(L.RopeDescC):
@@ -559,13 +583,13 @@ class RopeDesc(L.RopeDescC):
                  trained_len: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0, amplitude: float = 1.0,
                  inverse: bool = False, first_pos: int = 0, q_strides=None, q_out_strides=None, k_strides=None,
                  k_out_strides=None):
-        super().__init__(_choice(_OP_DTYPES, dtype, "dtype"), batch, seq, head_dim,
-                         head_dim if rot_dim is None else rot_dim, heads, kv_heads,
-                         heads if rot_heads is None else rot_heads, kv_heads if rot_kv_heads is None else rot_kv_heads,
-                         _choice(L.ROPE_LAYOUTS, layout, "layout"), _choice(L.ROPE_SCALINGS, scaling, "scaling"),
-                         int(inverse), first_pos, 0, theta, factor, trained_len, beta_fast, beta_slow, amplitude,
-                         _strides(q_strides, seq, heads, head_dim), _strides(q_out_strides, seq, heads, head_dim),
-                         _strides(k_strides, seq, kv_heads, head_dim), _strides(k_out_strides, seq, kv_heads, head_dim))
+        _fill(self, _choice(_OP_DTYPES, dtype, "dtype"), batch, seq, head_dim,
+              head_dim if rot_dim is None else rot_dim, heads, kv_heads,
+              heads if rot_heads is None else rot_heads, kv_heads if rot_kv_heads is None else rot_kv_heads,
+              _choice(L.ROPE_LAYOUTS, layout, "layout"), _choice(L.ROPE_SCALINGS, scaling, "scaling"),
+              int(inverse), first_pos, 0, theta, factor, trained_len, beta_fast, beta_slow, amplitude,
+              _strides(q_strides, seq, heads, head_dim), _strides(q_out_strides, seq, heads, head_dim),
+              _strides(k_strides, seq, kv_heads, head_dim), _strides(k_out_strides, seq, kv_heads, head_dim))
 
 
 class LinearDesc(L.LinearDescC):
@@ -574,9 +598,9 @@ class LinearDesc(L.LinearDescC):
     def __init__(self, m: int, n: int, k: int, *, dtype: str = "bf16", out_dtype: str | None = None,
                  activation: str = "none", gate_rows: int = 0, ldx: int | None = None, ldw: int | None = None,
                  ldy: int | None = None, ldr: int | None = None):
-        super().__init__(_choice(_OP_DTYPES, dtype, "dtype"), _choice(_OP_DTYPES, out_dtype or dtype, "out_dtype"), m, n, k,
-                         _choice(L.ACTIVATIONS, activation, "activation"), gate_rows, 0, k if ldx is None else ldx,
-                         k if ldw is None else ldw, n if ldy is None else ldy, n if ldr is None else ldr)
+        _fill(self, _choice(_OP_DTYPES, dtype, "dtype"), _choice(_OP_DTYPES, out_dtype or dtype, "out_dtype"), m, n, k,
+              _choice(L.ACTIVATIONS, activation, "activation"), gate_rows, 0, k if ldx is None else ldx,
+              k if ldw is None else ldw, n if ldy is None else ldy, n if ldr is None else ldr)
 
 
 class CrossAttentionDesc(L.CrossAttentionDescC):
@@ -587,11 +611,11 @@ class CrossAttentionDesc(L.CrossAttentionDescC):
     def __init__(self, batch: int, seq_q: int, seq_kv: int, heads: int, kv_heads: int, head_dim: int, *,
                  dtype: str = "bf16", scale: float | None = None, q_strides=None, k_strides=None, v_strides=None,
                  out_strides=None, mask_stride: int | None = None):
-        super().__init__(_choice(_OP_DTYPES, dtype, "dtype"), batch, seq_q, seq_kv, heads, kv_heads, head_dim,
-                         (head_dim ** -0.5 if head_dim > 0 else 0.0) if scale is None else scale,
-                         _strides(q_strides, seq_q, heads, head_dim), _strides(k_strides, seq_kv, kv_heads, head_dim),
-                         _strides(v_strides, seq_kv, kv_heads, head_dim), _strides(out_strides, seq_q, heads, head_dim),
-                         seq_kv if mask_stride is None else mask_stride)
+        _fill(self, _choice(_OP_DTYPES, dtype, "dtype"), batch, seq_q, seq_kv, heads, kv_heads, head_dim,
+              (head_dim ** -0.5 if head_dim > 0 else 0.0) if scale is None else scale,
+              _strides(q_strides, seq_q, heads, head_dim), _strides(k_strides, seq_kv, kv_heads, head_dim),
+              _strides(v_strides, seq_kv, kv_heads, head_dim), _strides(out_strides, seq_q, heads, head_dim),
+              seq_kv if mask_stride is None else mask_stride)
 
 
 class ops:
@@ -646,7 +670,7 @@ class ops:
                stream: int = 0) -> None:
         """y = residual + gate * act(x w^T + bias); bias and gate f32, each optional one 0."""
         _check(L.load().irodori_op_linear(desc, d_x, d_w, d_bias or None, d_gate or None, d_residual or None, d_y,
-                                          d_workspace or None, workspace_bytes, stream or None))
+                                          d_workspace or None, _workspace_bytes(workspace_bytes), stream or None))
 
     @staticmethod
     def cross_attention_workspace(desc: CrossAttentionDesc) -> int:
@@ -659,4 +683,4 @@ class ops:
                         workspace_bytes: int = 0, stream: int = 0) -> None:
         """Attention of each query to its row's keys (mask uint8, lengths int32, each 0 for all)."""
         _check(L.load().irodori_op_cross_attention(desc, d_q, d_k, d_v, d_mask or None, d_q_len or None, d_kv_len or None,
-                                                   d_out, d_workspace or None, workspace_bytes, stream or None))
+                                                   d_out, d_workspace or None, _workspace_bytes(workspace_bytes), stream or None))

@@ -209,3 +209,19 @@ def test_outputs_that_overlap_other_arguments_are_refused():
     refused("InvalidArg", "overlaps", lambda: ih.ops.rope(d, M, 2 * M, 3 * M, 4 * M, d_positions=2 * M + 64))
     refused("InvalidArg", "overlaps", lambda: ih.ops.rope(d, M, 2 * M, 3 * M, 4 * M, d_lengths=4 * M + 64))
     refused("InvalidArg", "overlaps", lambda: ih.ops.rope(d, M, 2 * M, 3 * M, 2 * M + 64))
+
+
+def test_numbers_that_the_fields_cannot_hold_are_refused():
+    # Their low bits alone would be another, valid call.
+    for text, make in (("m of", lambda: linear_desc(m=2 ** 32 + 4)), ("k of", lambda: linear_desc(k=-2 ** 32 + 16)),
+                       ("gate_rows of", lambda: linear_desc(gate_rows=2 ** 32)), ("ldx of", lambda: linear_desc(ldx=2 ** 64 + 16)),
+                       ("seq_kv of", lambda: cross_desc(seq_kv=2 ** 32 + 7)), ("heads of", lambda: cross_desc(heads=2 ** 33 + 4)),
+                       ("mask_stride of", lambda: cross_desc(mask_stride=2 ** 63)), ("stride of", lambda: cross_desc(k_strides=(2 ** 64, 128, 64))),
+                       ("first_pos of", lambda: rope_desc(first_pos=2 ** 31)), ("seq of", lambda: rope_desc(seq=2 ** 32 + 5)),
+                       ("stride of", lambda: rope_desc(q_strides=(640, 2 ** 63, 64)))):
+        refused("Shape", text, make)
+    assert rope_desc(first_pos=-2 ** 31).first_pos == -2 ** 31
+    for call in (lambda n: ih.ops.linear(linear_desc(), P, 2 * P, 3 * P, d_workspace=4 * P, workspace_bytes=n),
+                 lambda n: ih.ops.cross_attention(cross_desc(batch=1, seq_q=1, seq_kv=100000), P, 2 * P, 3 * P, 4 * P, d_workspace=5 * P,
+                                                  workspace_bytes=n)):
+        refused("InvalidArg", "negative", lambda: call(-1))
