@@ -568,7 +568,7 @@ void linear_kernel(LinearArgs a) {
 }
 
 // ---- few rows ---------------------------------------------------------------------------------
-// M <= 16 MT rows: a workgroup takes 16 columns of Y, its wavefronts share K and are summed through LDS.
+// M <= 16 rows: a workgroup takes 16 columns of Y, its wavefronts share K and are summed through LDS.
 // W moves HBM -> registers in the operand layout of the 16x16 matrix-core step (lane l: W row l % 16, 16
 // bytes at piece l / 16), each byte once; X, the B operand, comes from L2.  Bound by reading W.
 template <typename T>
@@ -604,39 +604,30 @@ __device__ __forceinline__ typename Piece<T>::type load_piece(const T* p, int k,
     return v;
 }
 
-template <typename T, typename TO, int MT, int NW>
-__global__ __launch_bounds__(64 * NW) void linear_rows_kernel(LinearArgs a) {
+constexpr int kRowWaves = 8;
+template <typename T, typename TO>
+__global__ __launch_bounds__(64 * kRowWaves) void linear_rows_kernel(LinearArgs a) {
     typedef typename Piece<T>::type V;
-    constexpr int E = 16 / sizeof(T), STEP = 4 * E, U = MT == 1 ? 8 : 4;  // elements of K a step takes, steps in flight
-    __shared__ float sums[NW][16 * MT][20];
+    constexpr int NW = kRowWaves, E = 16 / sizeof(T), STEP = 4 * E, U = 8;  // elements of K a step takes, steps in flight
+    __shared__ float sums[NW][16][20];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n0 = blockIdx.x * 16, r = lane & 15, piece = lane >> 4;
     const int n = n0 + r < a.N ? n0 + r : a.N - 1;
     const T* w = static_cast<const T*>(a.w) + (int64_t)n * a.ldw;
-    const T* x[MT];
-#pragma unroll
-    for (int j = 0; j < MT; j++) {
-        const int m = 16 * j + r < a.M ? 16 * j + r : a.M - 1;  // (a column of its own: never stored)
-        x[j] = static_cast<const T*>(a.x) + (int64_t)m * a.ldx;
-    }
+    const T* x = static_cast<const T*>(a.x) + (int64_t)(r < a.M ? r : a.M - 1) * a.ldx;  // (past M a column that is never stored)
     const int steps = (a.K + STEP - 1) / STEP, s0 = steps * wave / NW, s1 = steps * (wave + 1) / NW;
-    f32x4 acc[MT];
-#pragma unroll
-    for (int j = 0; j < MT; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     auto run = [&](int s, auto whole, auto count) {
         constexpr int C = decltype(count)::value;
-        V vw[C], vx[MT][C];
+        V vw[C], vx[C];
 #pragma unroll
         for (int i = 0; i < C; i++) {
             const int k = (s + i) * STEP + E * piece;
             vw[i] = load_piece<T, decltype(whole)::value>(w, k, a.K);
-#pragma unroll
-            for (int j = 0; j < MT; j++) vx[j][i] = load_piece<T, decltype(whole)::value>(x[j], k, a.K);
+            vx[i] = load_piece<T, decltype(whole)::value>(x, k, a.K);
         }
 #pragma unroll
-        for (int i = 0; i < C; i++)
-#pragma unroll
-            for (int j = 0; j < MT; j++) acc[j] = mma16(vw[i], vx[j][i], acc[j]);
+        for (int i = 0; i < C; i++) acc = mma16(vw[i], vx[i], acc);
     };
     const int whole = a.K / STEP < s1 ? a.K / STEP : s1;  // steps with all of their elements
     int s = s0;
@@ -644,12 +635,11 @@ __global__ __launch_bounds__(64 * NW) void linear_rows_kernel(LinearArgs a) {
     for (; s + 2 <= whole; s += 2) run(s, std::true_type{}, std::integral_constant<int, 2>{});
     for (; s < s1; s++) run(s, std::false_type{}, std::integral_constant<int, 1>{});
 
-    // acc[j][e]: row m = 16 j + r, column 4 piece + e.
-#pragma unroll
-    for (int j = 0; j < MT; j++) *reinterpret_cast<float4*>(&sums[wave][16 * j + r][4 * piece]) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+    // acc[e]: row m = r, column 4 piece + e.
+    *reinterpret_cast<float4*>(&sums[wave][r][4 * piece]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     __syncthreads();
     const int m = threadIdx.x >> 2, c = 4 * (threadIdx.x & 3);
-    if (threadIdx.x >= 64 * MT || m >= a.M || n0 + c >= a.N) return;
+    if (threadIdx.x >= 64 || m >= a.M || n0 + c >= a.N) return;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int q = 0; q < NW; q++) {
@@ -662,12 +652,11 @@ __global__ __launch_bounds__(64 * NW) void linear_rows_kernel(LinearArgs a) {
     finish<TO>(a, m, n0 + c, v);
 }
 
-template <typename T, typename TO, int MT, int NW>
+template <typename T, typename TO>
 int launch_rows(const LinearArgs& a, hipStream_t st, bool go) {
-    static_assert(MT <= NW, "a thread per four sums");
     const int64_t wgs = ((int64_t)a.N + 15) / 16;
-    if (wgs * (64 * NW) > UINT32_MAX) return -1;
-    if (go) linear_rows_kernel<T, TO, MT, NW><<<(unsigned)wgs, 64 * NW, 0, st>>>(a);
+    if (wgs * (64 * kRowWaves) > UINT32_MAX) return -1;
+    if (go) linear_rows_kernel<T, TO><<<(unsigned)wgs, 64 * kRowWaves, 0, st>>>(a);
     return 0;
 }
 
@@ -728,7 +717,7 @@ int best_tiles(const TileCost (&t)[N], const LinearArgs& a) {
 template <typename T, typename TO>
 int launch_linear(const LinearArgs& a, hipStream_t st, bool go) {
     // One new token or a few: 4.0 against 5.0 to 6.2 us with 32 x 32 tiles at 16 x 1024 x 1024 (bf16).
-    if (a.M <= 16) return launch_rows<T, TO, 1, 8>(a, st, go);
+    if (a.M <= 16) return launch_rows<T, TO>(a, st, go);
     // The buffer-to-LDS loads take dword-aligned rows, and windows of a tile's rows below 2^31 bytes.
     constexpr int64_t ES = sizeof(T), FAR = (int64_t)1 << 22;
     const bool async = !((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx * ES | a.ldw * ES) & 3) &&
