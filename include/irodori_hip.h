@@ -488,7 +488,8 @@ int irodori_op_gemm_fp8(const uint8_t* a, const uint8_t* a_scale, const uint8_t*
  * must belong to the current device (else IRODORI_ERR_INVALID_ARG), without waiting, allocates
  * nothing, keeps nothing between calls and may be captured from the first call on.  Tensors are in the
  * description's dtype (IRODORI_DTYPE_F32, _BF16 or _F16) and need the alignment of an element;
- * strides count elements.  An output may not overlap an input except where said. */
+ * strides count elements.  An output (or a workspace) may not overlap another argument except where said: refused
+ * where the extents show it, as they do for tensors without gaps and for parts of one buffer. */
 
 /* Rotary positions: the pairs of a head turned by position * frequency.
  *   (a, b) -> amplitude * (a cos - b sin, a sin + b cos)
@@ -523,7 +524,7 @@ typedef struct irodori_rope_desc {
     int64_t k_strides[3], k_out_strides[3];
 } irodori_rope_desc;
 /* positions [batch, seq] or NULL; lengths [batch] or NULL (tokens at or past a row's length are left
- * as they were in the outputs).  q_out may be q, and k_out k, with equal strides. */
+ * as they were in the outputs; below 0 a length is 0).  q_out may be q, and k_out k, with equal strides. */
 int irodori_op_rope(const irodori_rope_desc* desc, const void* q, void* q_out, const void* k, void* k_out,
                     const int32_t* positions, const int32_t* lengths, void* stream);
 
@@ -547,8 +548,8 @@ typedef struct irodori_linear_desc {
     int32_t reserved;
     int64_t ldx, ldw, ldy, ldr;  /* between rows */
 } irodori_linear_desc;
-/* Bytes of device workspace that a call of this description takes (often 0).  Its contents need not be
- * kept between calls; calls that may run at the same time need one each. */
+/* Bytes of device workspace that a call of this description takes: 0 for every one, and irodori_op_linear reads
+ * neither `workspace` nor its size.  (Part of the interface beside irodori_op_cross_attention's.) */
 int irodori_op_linear_workspace(const irodori_linear_desc* desc, uint64_t* bytes);
 int irodori_op_linear(const irodori_linear_desc* desc, const void* x, const void* w, const float* bias,
                       const float* gate, const void* residual, void* y, void* workspace,
@@ -572,7 +573,8 @@ typedef struct irodori_cross_attention_desc {
     int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
     int64_t mask_stride;         /* between rows of the mask */
 } irodori_cross_attention_desc;
-/* As irodori_op_linear_workspace. */
+/* Bytes of device workspace that a call of this description takes (0 where the keys are not split).  Its contents need
+ * not be kept between calls; calls that may run at the same time need one each. */
 int irodori_op_cross_attention_workspace(const irodori_cross_attention_desc* desc, uint64_t* bytes);
 int irodori_op_cross_attention(const irodori_cross_attention_desc* desc, const void* q, const void* k,
                                const void* v, const uint8_t* mask, const int32_t* q_len,

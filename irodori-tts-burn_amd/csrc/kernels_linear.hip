@@ -675,7 +675,8 @@ namespace {
 
 // The tiles a launch takes: of these, the one whose busiest CU is done first, by the microseconds of a tile
 // (f + a K) fitted to all tiles' times at 288 sizes (16-bit) and 202 (f32): M from 20 to 69 694, N from 333 to 5632, K from 32 to
-// 3680.  The choice loses 1.3 % on the best of them on average, 23 % at most (0.1 % and 11 % in f32).  Tiles that share a CU
+// 3680.  On 150 (120) other sizes, M from 17 to 70 000, N from 64 to 6000, K from 32 to 4000, the choice loses 1.45 % on the best
+// of them on average (0.18 % in f32), 27 % at most (9 %) and over 10 % at six: short reductions in a few 128-row tiles.  Tiles that share a CU
 // overlap where they wait (rounds count in parts); one a CU may take longer than one of many.  E.g. in bf16 with
 // 32 x 32 / 64 x 64 / 128 x 64 / 128 x 128 / 256 x 256 tiles: 256 x 1024 x 1024 5.5 / 6.0 / 8.9 / 10.4 / 27 us, 1500 x 1024 x 1024
 // 14.1 / 9.1 / 9.9 / 11.1 / 27, 12000 x 5632 x 1024 - / 244 / 195 / 150 / 162, 24000 x 5632 x 1024 the last two 295 / 281 (with silu

@@ -370,6 +370,29 @@ def test_linear_between_columns_of_one_buffer(m):
     assert torch.equal(buf[:, n:], before[:, n:])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m", [5, 40, 700])
+def test_linear_rows_far_apart(dtype, m):
+    # Rows 2^22 bytes and more apart, past the windows of the asynchronous loads; 700 of x past 2^32 bytes.
+    n, k = 40, 70
+    step = (1 << 23) // TYPE[dtype].itemsize
+    x = torch.empty((m - 1) * step + k, dtype=TYPE[dtype], device="cuda").as_strided((m, k), (step, 1))
+    w = torch.empty((n - 1) * step + k, dtype=TYPE[dtype], device="cuda").as_strided((n, k), (step, 1))
+    x.copy_(randn(1, m, k, dtype=dtype)), w.copy_(randn(2, n, k, dtype=dtype, std=k ** -0.5))
+    y = torch.empty(m, n, dtype=TYPE[dtype], device="cuda")
+    run_linear(x, w, y, dtype, dtype)
+    close(y, *linear_ref(x, w, dtype), "far apart")
+
+
+@pytest.mark.parametrize("dtype,k", [("bf16", (1 << 21) + 3), ("f32", (1 << 20) + 3)])
+@pytest.mark.parametrize("m", [3, 18])
+def test_linear_long_reduction(dtype, k, m):
+    x, w = randn(1, m, k, dtype=dtype), randn(2, 33, k, dtype=dtype, std=k ** -0.5)
+    y = torch.empty(m, 33, device="cuda")
+    run_linear(x, w, y, dtype, "f32")
+    close(y, *linear_ref(x, w, "f32"), "long")
+
+
 # ---- cross attention --------------------------------------------------------------------------
 def run_cross(q, k, v, out, dtype, mask=None, q_len=None, kv_len=None, scale=None):
     b, sq, h, d = q.shape
