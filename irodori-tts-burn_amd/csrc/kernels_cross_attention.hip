@@ -6,21 +6,24 @@
 // heads share every tile that is loaded), on the 32x32 matrix-core shapes:
 //   S^T = K Q^T      lane l holds row l % 32 and keys 8a + 4 (l / 32) + c of every 32.
 //   softmax          p = exp2(s c - m) in f32, c = scale log2(e).  The reference m is lazy: a row's
-//                    first score above -inf sets it, and it moves when a lane's sum of p over a tile
-//                    shows a p beyond the slack.
+//                    first score above -inf sets it, and it moves, with the tile's scores formed again, when a
+//                    lane's sum of p over a tile shows a p beyond the slack.
 //   O^T += V^T P^T   P^T is the S^T accumulator, rounded to the operand type in the 16-bit forms (the
-//                    matrix core's operand; its rounding averages out over the keys as V's own does);
+//                    matrix core's operand; its rounding averages out over the keys as V's own does), and summed as
+//                    rounded: 2.3e-3 relative L2 from float64 in bf16 and 2.9e-4 in f16, where the output's rounding
+//                    alone is 1.7e-3 and 2.1e-4.  (Two operands to a probability would take half as many products again.)
 //                    V^T comes from the row-major tile, 16-bit by the transposing LDS read.
-// A tile that the mask empties is never loaded; in a tile that it thins, the masked scores are -inf and
-// the masked values, which are not loaded, zero.
+// A tile that the mask empties is not loaded, but for the first step's K where there are two key groups or more, which
+// is loaded under the mask's latency on the guess that it counts; in a tile that the mask thins, the masked scores are
+// -inf and the masked values, which are not loaded, zero.
 //
 // Measured a call, host side included (the operator's floor in brackets):
-//   8 x 1 token over 8200 ragged keys, 16 heads on 4 of 128 (bf16)   26.4 us [19.5]  memory: the runs stream at 4.5 TB/s for
+//   8 x 1 token over 8200 ragged keys, 16 heads on 4 of 128 (bf16)   26.1 us [19.5]  memory: the runs stream at 4.5 TB/s for
 //                                        21 us, the joining launch takes 5
-//   2 x 101 over 37 keys, 16 heads of 64 (f32)    8.2 [0.4]   one chain: mask, tile, 4096 cycles of f32 matrix core, join
-//   2 x 750 over 631 masked keys, 16 heads of 64 (bf16)   14.8 [1.7]  384 workgroups, a chain of five steps of about 1.2 us
+//   2 x 101 over 37 keys, 16 heads of 64 (f32)    8.1 [0.4]   one chain: mask, tile, 4096 cycles of f32 matrix core, join
+//   2 x 750 over 631 masked keys, 16 heads of 64 (bf16)   14.3 [1.7]  384 workgroups, a chain of five steps of about 1.2 us
 //                                        (softmax on the VALU, then the products) between 4 us of loads and 2 of joining
-//   32 x 750 over 4100 ragged keys, 20 heads of 64 (f16)  455 [219]   VALU 64 % and matrix cores 43 % of the cycles, at the
+//   32 x 750 over 4100 ragged keys, 20 heads of 64 (f16)  460 [219]   VALU 65 % and matrix cores 44 % of the cycles, at the
 //                                        1.7 GHz that the card's power leaves; 128-dim heads 855 TFLOP/s (bf16)
 #include <type_traits>
 

@@ -10,8 +10,8 @@
 // HBM-bound: every element is read and written once.  A workgroup takes some tokens and some of
 // their heads; it issues all of its loads, then makes the tokens' cosines and sines (one per pair,
 // shared by all heads) in LDS under their latency, then rotates and stores.  Measured a call, host side
-// included (floor at a large copy's 4.9 TB/s in brackets): 8 tokens of 20 128-dim heads 7.6 us (the launch;
-// 4.3 of kernel), 2 x 750 x 32 heads in f32 7.5 [5.0], 8 x 4001 ragged tokens x 40 heads in bf16 59 [48], 43 us of
+// included (floor at a large copy's 4.9 TB/s in brackets): 8 tokens of 20 128-dim heads 7.8 us (the launch;
+// 4.4 of kernel), 2 x 750 x 32 heads in f32 7.6 [5.0], 8 x 4001 ragged tokens x 40 heads in bf16 59 [48], 44 us of
 // kernel where the inputs are in the last-level cache.  Stores past the caches lost (60.6 against 58.9).
 #include "common.hpp"
 #include "op_util.hpp"
