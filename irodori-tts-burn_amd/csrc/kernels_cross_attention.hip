@@ -41,6 +41,9 @@ constexpr int kTile = sizeof(T) == 2 ? 64 : 32;  // keys
 template <typename T>
 constexpr float kSumMax = std::is_same<T, f16>::value ? 32768.f : 65536.f;
 
+// Beside a larger reference, the rounding that a distance's product is spared could be more than the distance.
+constexpr float kVast = 16777216.f;
+
 // 16-byte chunk c of tile row r (ROWB bytes): K is read 32 rows at one chunk, 16-bit V 8 rows at two
 // neighbouring chunks, f32 V one row at a time.
 template <int ROWB>
@@ -343,6 +346,7 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
         float m = 0.f, l_run = 0.f;
         bool unset = true;  // m is no reference yet: no tile so far, or only scores of -inf
         bool first = true;  // any lane's unset
+        bool vast = false;  // any lane's |m| above kVast
 
         for (int t0 = t_begin; t0 < t_end; t0 += 64) {
             wait_lds();
@@ -447,6 +451,7 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
                         unset = false;
                     }
                     first = __any(unset);
+                    vast = __any(fabsf(m) > kVast);
                 }
                 // The scores become their distances from the reference, which alone stay live.
                 V8 pf[2 * KB];
@@ -471,15 +476,15 @@ __global__ __launch_bounds__(64 * QW * KW) __attribute__((amdgpu_waves_per_eu(WP
                 };
                 float psum = exps([&](float x) { return fmaf(x, c, -m); });
                 const unsigned long long over = __ballot(!(psum <= kSumMax<T>));
-                if (over) {
+                if (over || vast) {
                     // Lanes l and l ^ 32 hold one row's two key halves: either one asks for both.
-                    const bool need = ((over >> lane) | (over >> (lane ^ 32))) & 1ull;
-                    // The scores are formed again: a distance from a reference far below has lost them in its rounding.  And the new
-                    // distances are those of rounded products, as the reference is one: beside a product above 2^28 its
-                    // rounding alone could exceed the slack.
+                    const bool need = (((over >> lane) | (over >> (lane ^ 32))) & 1ull) || fabsf(m) > kVast;
+                    // The scores are formed again: a distance from a reference far below has lost them in its rounding.  The new
+                    // distances are those of rounded products, as the reference is one, so the largest is 0.
                     scores(std::true_type{});
                     const float mx = tile_max(), mn = need ? fmaxf(m, mx) : m, corr = fast_exp2(m - mn);
                     m = mn;
+                    vast = __any(fabsf(m) > kVast);
 #pragma unroll
                     for (int db = 0; db < DB; db++) o[db] *= corr;
                     l_run *= corr;

@@ -716,6 +716,29 @@ def test_cross_attention_into_a_part_of_the_queries_buffer():
     assert torch.equal(buf[:, :, h:], before[:, :, h:])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq,skv", [(1, 1), (1, 9000), (40, 300), (300, 70)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_cross_attention_equal_scores_of_any_size(dtype, d, sq, skv, sign):
+    """Every key at one score, up to the type's lowest and largest value: the plain mean of the values."""
+    q, k, v = (torch.zeros(1, n, 2, d, dtype=TYPE[dtype], device="cuda") for n in (sq, skv, skv))
+    v.copy_(randn(3, 1, skv, 2, d, dtype=dtype))
+    want, mag = v.double().mean(1, keepdim=True).expand(1, sq, 2, d), v.double().abs().mean(1, keepdim=True).expand(1, sq, 2, d)
+    for big in (1e3, 6e4) + ((1e9, 1.7e15, 3e30, torch.finfo(TYPE[dtype]).max) if dtype != "f16" else (65504.0,)):
+        k[..., 0] = sign * big
+        q[..., 0] = (1 + torch.rand(sq, 2, generator=torch.Generator().manual_seed(5))).to(TYPE[dtype]).cuda()
+        q[..., 1], k[..., 1] = 60000 if dtype == "f16" else 0, sign * big if dtype == "f16" else 0
+        out = torch.full_like(q, CANARY)
+        run_cross(q, k, v, out, dtype)
+        # A product above f32's largest value is an infinite score: NaN, or below all others, with no other there 0.
+        inf = (q[..., 0].double() * big > torch.finfo(torch.float32).max * (1 + F / 2))[..., None].expand_as(out)
+        assert (out[inf].isnan() if sign > 0 else out[inf] == 0).all()
+        # Weights of exactly 1: the sums' roundings, the reciprocal's, the output's.
+        tol = (skv + 4) * F * mag + u(dtype) * want.abs() * (1 + 2.0 ** -6) + tiny(dtype)
+        close(out[~inf], want[~inf], tol[~inf], "%g" % big)
+
+
 # ---- the half block they make up ----------------------------------------------------------------
 class HalfBlock:
     """x + g * (cross(rope(norm(x) Wq + bq), states Wk, states Wv) Wo), each step one operator."""
