@@ -582,6 +582,75 @@ int irodori_op_cross_attention(const irodori_cross_attention_desc* desc, const v
                                const int32_t* kv_len, void* out, void* workspace,
                                uint64_t workspace_bytes, void* stream);
 
+/* ---- described operators of an fp8 half block ---------------------------------------------------
+ * No counterparts in the reference either; the conventions of the described operators above hold.  FP8 operands
+ * are e4m3 codes with one f32 scale s for each block of 128 along a row (the last one may be shorter): a code's value
+ * times s.  Blocks are quantized as s = max(amax / 448, 2^-126), codes = round-to-nearest-even e4m3(v / s), amax
+ * the largest finite magnitude of the block; an infinity or a NaN becomes e4m3's NaN. */
+
+/* Norms around a block: the block's output (the branch) normed, gated and added to the residual stream, and
+ * the next block's normed and modulated input, in one pass over a row:
+ *   r     = stream_scale x + branch_scale gate[row / mod_rows] (N_b(branch) branch_weight + branch_bias)
+ *   x_out = r
+ *   h     = (N(r) weight + bias) (1 + scale[row / mod_rows]) + shift[row / mod_rows]
+ * with N (norm) and N_b (branch_norm) none, RMS: v / sqrt(mean(v^2) + eps), or LAYER: (v - mean(v)) /
+ * sqrt(var(v) + eps).  Everything is f32 between the loads and one rounding at the stores, and h is of the unrounded r.
+ * Every argument but x may be NULL and then stands for its neutral value (without a branch r = stream_scale x), h and
+ * x_out for an output that is not wanted; one of them is.  Weights and biases are f32 [dim], gate, scale and shift
+ * f32 rows of dim with ldm between them; one of these three and a positive mod_rows go together. */
+#define IRODORI_NORM_NONE 0
+#define IRODORI_NORM_RMS 1
+#define IRODORI_NORM_LAYER 2
+typedef struct irodori_block_norm_desc {
+    int32_t dtype;        /* of the branch, and of h unless that is FP8 */
+    int32_t stream_dtype; /* of x and x_out: dtype or F32 */
+    int32_t h_dtype;      /* dtype or FP8: codes in h, their scales in h_scales */
+    int32_t rows, dim;    /* dim <= 16384 */
+    int32_t branch_norm, norm;
+    int32_t mod_rows;     /* rows that share a row of gate, scale and shift; 0 without them */
+    float branch_eps, eps; /* 1e-30 .. 1e30 */
+    float stream_scale, branch_scale;
+    int64_t ldx, ldb, ldxo, ldh; /* between rows of x, branch, x_out and h */
+    int64_t ldhs;         /* between rows of h_scales [rows, ceil(dim / 128)] */
+    int64_t ldm;
+} irodori_block_norm_desc;
+/* x_out may be x, with ldxo == ldx. */
+int irodori_op_block_norm(const irodori_block_norm_desc* desc, const void* x, const void* branch,
+                          const float* branch_weight, const float* branch_bias, const float* gate, void* x_out,
+                          const float* weight, const float* bias, const float* scale, const float* shift, void* h,
+                          float* h_scales, void* stream);
+
+/* Quantization of v [rows, dim] to q with scales [ceil(rows / block_rows), ceil(dim / 128)]: block_rows 1, a row's blocks
+ * of 128 (irodori_op_linear_fp8's x), or 128, blocks of 128 x 128 (its w).  v = act(x), or with `gated`
+ * act(x[:, :dim]) * x[:, dim:] of x [rows, 2 dim], a feed-forward's two halves; blocks of 128 rows take x as it is. */
+typedef struct irodori_block_quantize_desc {
+    int32_t dtype;      /* of x */
+    int32_t rows, dim;  /* at most 2^28 */
+    int32_t block_rows; /* 1 or 128 */
+    int32_t gated;
+    int32_t activation; /* IRODORI_ACT_* */
+    int64_t ldx, ldq, lds; /* between rows */
+} irodori_block_quantize_desc;
+int irodori_op_block_quantize(const irodori_block_quantize_desc* desc, const void* x, uint8_t* q, float* scales,
+                              void* stream);
+
+/* Linear layer on FP8 operands: y[m, n] = residual[m, n] + gate[m / gate_rows, n] * act(bias[n] +
+ *   sum_b x_scales[m, b] w_scales[n / 128, b] sum_{k in block b} x[m, k] w[n, k])
+ * with x [m, k] and w [n, k] e4m3 codes, b the blocks of 128 along k, x_scales [m, blocks] and w_scales [ceil(n / 128),
+ * blocks]; the blocks' sums, the scales and everything after them in f32, rounded once to out_dtype (F32, BF16 or F16).
+ * bias, gate and residual as irodori_op_linear's.  y may be the residual, with ldy == ldr. */
+typedef struct irodori_linear_fp8_desc {
+    int32_t out_dtype;
+    int32_t m, n, k;             /* at most 2^28 */
+    int32_t activation;
+    int32_t gate_rows;           /* rows that share a row of the gate; 0 without one */
+    int64_t ldx, ldw, ldy, ldr;  /* between rows */
+    int64_t ldxs, ldws;          /* between rows of the scales */
+} irodori_linear_fp8_desc;
+int irodori_op_linear_fp8(const irodori_linear_fp8_desc* desc, const uint8_t* x, const float* x_scales,
+                          const uint8_t* w, const float* w_scales, const float* bias, const float* gate,
+                          const void* residual, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

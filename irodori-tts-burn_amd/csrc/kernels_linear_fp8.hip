@@ -1,0 +1,465 @@
+// The fp8 linear operator's kernels (irodori_op_linear_fp8): Y = R + G * act(sum_b sx[m, b] sw[n / 128, b] (X W^T)_b + b),
+// (X W^T)_b the product over the b-th 128 of K of the e4m3 codes X [M, K] and W [N, K], on the matrix cores with f32 sums.
+//
+// A block's product starts from zero in registers of its own and joins the tile's sums by one multiply-add an element
+// with sx sw in f32: the product is formed transposed (W's rows are the A operand), so a lane has one row of Y and one factor a
+// block.  The 16 multiply-adds of a 32 x 32 block take half of the cycles of its two matrix instructions, and run beside
+// others'.  The epilogue is the linear operator's.
+//
+// The fp8 matrix instructions align each 8 products of neighbouring codes to the largest and keep 13 bits below its exponent
+// (measured; beyond the 8 their sums are f32): 1.5e-5 relative L2 for normal operands, far below the rounding of a 16-bit Y (1.7e-3
+// bf16, 2.1e-4 f16).  An f32 Y takes the codes as bf16, which holds them and their products exactly, at half of the rate (1e-7);
+// so do few rows, which wait for W.
+#include <type_traits>
+
+#include "attn_util.hpp"
+#include "fp8_block.hpp"
+#include "kernels.hpp"
+#include "linear_fp8.hpp"
+#include "linear_tile.hpp"
+
+namespace irodori {
+
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+// A uniform value, by the scalar cache.
+typedef const __attribute__((address_space(4))) float* uniform_ptr;
+__device__ __forceinline__ uniform_ptr uniform(const float* p) { return (uniform_ptr)(uintptr_t)p; }
+
+// The 32 codes a lane supplies to a 64-deep step: K bytes 64 ks + 16 h .. + 15 and 32 more on, h = lane / 32.
+__device__ __forceinline__ f32x16 mma8(const i32x8& a, const i32x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);  // (the form without block scales)
+}
+// Codes 8 q .. 8 q + 7 of a lane's 32 as bf16, exactly.
+__device__ __forceinline__ bf16x8 widen(const i32x8& v, int q) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * q + i], 1.f, false);
+        const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * q + i], 1.f, true);
+        r[4 * i] = lo[0];
+        r[4 * i + 1] = lo[1];
+        r[4 * i + 2] = hi[0];
+        r[4 * i + 3] = hi[1];
+    }
+    return r;
+}
+template <int RB>
+__device__ __forceinline__ i32x8 read_codes(const unsigned char* row, int r, int ks, int h) {
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(row + (lswz<RB>(r, 4 * ks + h) << 4));
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(row + (lswz<RB>(r, 4 * ks + 2 + h) << 4));
+    i32x8 f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        f[e] = lo[e];
+        f[4 + e] = hi[e];
+    }
+    return f;
+}
+// The dword of codes that begins at k without those past K.
+__device__ __forceinline__ int cut_dword(int v, int k, int K) {
+    const int left = K - k;
+    return left >= 4 ? v : left <= 0 ? 0 : v & ((1 << 8 * left) - 1);
+}
+
+// A tile of BM rows and BN columns of Y per workgroup of WM x WN x WK wavefronts.  K advances in slices of WK blocks of 128
+// codes, one for each of the WK, which are summed through LDS at the end.  ASYNC: slices move HBM -> LDS by
+// buffer_load_dwordx4 ... lds, which take dword-aligned rows, up to STAGES ahead; a piece that straddles K's end is cut in the
+// last slice's fragments.  Otherwise through registers.  The scales of X come along every fourth block.
+template <typename TO, int BM, int BN, int WM, int WN, int WK, int STAGES, bool ASYNC>
+__global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_eu(WM * WN * WK <= 4 ? 1 : 2)))
+void linear_fp8_kernel(LinearFp8Args args) {
+    const LinearArgs& a = args.l;
+    constexpr int NW = WM * WN * WK, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+    constexpr int RB = 128 * WK, ROWS = BM + BN, STAGE = ROWS * RB, RC = RB / 16;
+    constexpr int RPI = 64 / RC, LPW = ROWS / RPI / NW;  // rows a load instruction fills, instructions per wave per slice
+    constexpr int PER = 4 / WK, SLOTS = WK == 4 ? STAGES : 2;  // slices that share a load of scales, loads held
+    constexpr int SROWS = BM < 64 ? 64 : BM;
+    constexpr bool PAIR = FN % 2 == 0 && sizeof(TO) == 2;
+    constexpr int C = PAIR ? 32 : 16;  // neighbouring columns of Y a lane ends with
+    static_assert(LPW * RPI * NW == ROWS && BN % RPI == 0 && NW * 64 >= SROWS && 128 % TN == 0, "slices split over the waves");
+    static_assert(WK == 1 || (WK - 1) * BM * BN * 4 <= STAGES * STAGE, "the k groups' sums fit the ring");
+    static_assert(STAGES <= 3, "a load of scales is replaced when the slices of the one before it are all being read");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * STAGE];
+    __shared__ __attribute__((aligned(1024))) float xscale[SLOTS][SROWS][4];
+
+    const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wk = wave / (WM * WN), wmn = wave % (WM * WN), wm = wmn / WN, wn = wmn % WN;
+    // Groups of 8 row tiles sweep the column tiles, an XCD's workgroups consecutive.
+    const int pid = xcd_remap(blockIdx.x, gridDim.x);
+    const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN;
+    const int group = pid / (8 * tiles_n), first = group * 8;
+    const int gm = tiles_m - first < 8 ? tiles_m - first : 8, local = pid - group * 8 * tiles_n;
+    const int m0 = (first + local % gm) * BM, n0 = (local / gm) * BN;
+    const int rows_m = a.M - m0 < BM ? a.M - m0 : BM, rows_n = a.N - n0 < BN ? a.N - n0 : BN;
+    const unsigned char* X = static_cast<const unsigned char*>(a.x) + (int64_t)m0 * a.ldx;
+    const unsigned char* W = static_cast<const unsigned char*>(a.w) + (int64_t)n0 * a.ldw;
+    const float* XS = args.xs + (int64_t)m0 * args.ldxs;
+    // The wave's columns share their scales (columns past N, which are not stored, take the last ones').
+    const int wblock = n0 + wn * TN < a.N ? (n0 + wn * TN) / kBlock : (a.N - 1) / kBlock;
+    const uniform_ptr ws = uniform(args.ws + (int64_t)wblock * args.ldws);
+    const int nk = (args.blocks + WK - 1) / WK;
+
+    // Load instruction i of this wave fills stage rows RPI (wave LPW + i) .. (W rows, then X rows):
+    // lane -> row lane / RC, physical chunk lane % RC, which holds the row's chunk `chunk`.
+    auto chunk = [&](int i) {
+        const int r = (wave * LPW + i) * RPI + lane / RC;
+        return lswz<RB>(r < BN ? operand_row<PAIR>(r) : r, lane % RC);
+    };
+    [[maybe_unused]] __amdgpu_buffer_rsrc_t rX, rW, rS;
+    [[maybe_unused]] unsigned voff[LPW], soff = 0;
+    if constexpr (ASYNC) {
+        // Windows end with the last row's last whole dword (its other bytes are in the same memory word).
+        rX = make_rsrc(X, ((unsigned)((int64_t)(rows_m - 1) * a.ldx + a.K) + 3) & ~3u);
+        rW = make_rsrc(W, ((unsigned)((int64_t)(rows_n - 1) * a.ldw + a.K) + 3) & ~3u);
+        rS = make_rsrc(XS, (unsigned)((int64_t)(rows_m - 1) * args.ldxs + args.blocks) * 4u);
+#pragma unroll
+        for (int i = 0; i < LPW; i++) {
+            const int r = (wave * LPW + i) * RPI + lane / RC;
+            // Rows past the last (which short strides would leave inside the window) lie behind it and read as zero.
+            const bool there = r < BN ? r < rows_n : r - BN < rows_m;
+            voff[i] = there ? (unsigned)(r < BN ? r * a.ldw : (r - BN) * a.ldx) + chunk(i) * 16u : 0x80000000u;
+        }
+        soff = 64 * wave + lane < rows_m ? (unsigned)((64 * wave + lane) * args.ldxs) * 4u : 0x80000000u;
+    }
+    // Slice kt into its ring slot; without ASYNC the slice that `stash` holds, and the next into it.
+    [[maybe_unused]] u32x4 stash[LPW];
+    [[maybe_unused]] f32x4 sstash;
+    [[maybe_unused]] auto load_stash = [&](int kt) {
+        typedef unsigned U4 __attribute__((ext_vector_type(4), aligned(1)));
+#pragma unroll
+        for (int i = 0; i < LPW; i++) {
+            const int r = (wave * LPW + i) * RPI + lane / RC, k = kt * RB + chunk(i) * 16, rr = r < BN ? r : r - BN;
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (rr < (r < BN ? rows_n : rows_m) && k < a.K) {
+                const unsigned char* src = (r < BN ? W + (int64_t)rr * a.ldw : X + (int64_t)rr * a.ldx) + k;
+                if (k + 16 <= a.K) {
+                    v = *reinterpret_cast<const U4*>(src);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 15; e++)
+                        if (k + e < a.K) v[e / 4] |= (unsigned)src[e] << (8 * (e & 3));
+                }
+            }
+            stash[i] = v;
+        }
+        if (kt % PER == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                sstash[e] = (int)threadIdx.x < rows_m && kt * WK + e < args.blocks ? XS[threadIdx.x * args.ldxs + kt * WK + e] : 0.f;
+        }
+    };
+    auto issue = [&](int kt) {
+        if (kt % PER == 0 && wave < SROWS / 64) {
+            float* dst = &xscale[kt / PER % SLOTS][64 * wave][0];
+            if constexpr (ASYNC) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rS, (__attribute__((address_space(3))) void*)dst, 16, soff + kt * WK * 4u, 0, 0, 0);
+            } else {
+                *reinterpret_cast<f32x4*>(dst + 4 * lane) = sstash;
+            }
+        }
+        unsigned char* dst = smem + kt % STAGES * STAGE + wave * LPW * 1024;
+#pragma unroll
+        for (int i = 0; i < LPW; i++) {
+            if constexpr (ASYNC) {
+                // Pieces past K read as zero (windows are below 2^31 bytes, the offsets whole in the checked part).
+                const unsigned vo = kt * RB + chunk(i) * 16 < a.K ? voff[i] + (unsigned)kt * RB : 0x80000000u;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds((wave * LPW + i) * RPI < BN ? rW : rX,
+                                                         (__attribute__((address_space(3))) void*)(dst + i * 1024), 16,
+                                                         vo, 0, 0, 0);
+            } else {
+                *reinterpret_cast<u32x4*>(dst + i * 1024 + 16 * lane) = stash[i];
+            }
+        }
+        if constexpr (!ASYNC) {
+            if (kt + 1 < nk) load_stash(kt + 1);
+        }
+    };
+
+    constexpr bool EXACT = sizeof(TO) == 4;
+    auto zeros = [] {
+        f32x16 z;
+#pragma unroll
+        for (int e = 0; e < 16; e++) z[e] = 0.f;
+        return z;
+    };
+    f32x16 acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int j = 0; j < FM; j++) acc[i][j] = zeros();
+
+    // One block a wavefront: its residual comes under the products.
+    constexpr bool EARLY = FM * FN == 1;
+    [[maybe_unused]] u32x4 early[kLanes<TO, C>];
+    if constexpr (EARLY) {
+        constexpr int Q = kLanes<TO, C>;
+        const int t = lane & (Q - 1);
+        if (a.residual && wk == 0) load_pieces<TO, false>(a, m0 + wm * TM + fr - t, n0 + wn * TN + 16 * fh + t * kPiece<TO>, early);
+    }
+
+    // Two sets of fragments: a slice's are read while the one before multiplies.  The slot that every wave has read by then is
+    // filled again.
+    i32x8 fw[2][FN][2], fx[2][FM][2];
+    float sx[2][FM], sw[2];
+    auto read_slice = [&](int kt, auto set) {
+        const unsigned char* st = smem + kt % STAGES * STAGE;
+        const int b = kt * WK + wk;
+        sw[set] = ws[b < args.blocks ? b : 0];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+#pragma unroll
+            for (int i = 0; i < FN; i++) fw[set][i][s] = read_codes<RB>(st + (wn * TN + w_row<PAIR>(i, fr)) * RB, fr, 2 * wk + s, fh);
+#pragma unroll
+            for (int j = 0; j < FM; j++) fx[set][j][s] = read_codes<RB>(st + (BN + wm * TM + 32 * j + fr) * RB, fr, 2 * wk + s, fh);
+        }
+#pragma unroll
+        for (int j = 0; j < FM; j++) {
+            const float s = xscale[kt / PER % SLOTS][wm * TM + 32 * j + fr][b % 4];
+            sx[set][j] = b < args.blocks ? s : 0.f;
+        }
+    };
+    auto cut = [&](i32x8& f, int k) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = cut_dword(f[e], k + 4 * (e & 3) + 32 * (e >> 2), a.K);
+    };
+    auto slice = [&](int kt, auto cur, auto last) {
+        constexpr std::integral_constant<int, 1 - decltype(cur)::value> next;
+        if constexpr (!decltype(last)::value) {
+            const int left = nk - 2 - kt;
+            if constexpr (ASYNC) wait_slices<STAGES - 2, LPW>(left < STAGES - 2 ? left : STAGES - 2);
+            wait_lds();
+            raw_barrier();
+            read_slice(kt + 1, next);
+            if (kt + STAGES < nk) issue(kt + STAGES);
+        } else if constexpr (ASYNC) {
+            if (a.K % 16) {
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    const int k = kt * RB + 128 * wk + 64 * s + 16 * fh;
+#pragma unroll
+                    for (int i = 0; i < FN; i++) cut(fw[cur][i][s], k);
+#pragma unroll
+                    for (int j = 0; j < FM; j++) cut(fx[cur][j][s], k);
+                }
+            }
+        }
+        float f[FM];
+#pragma unroll
+        for (int j = 0; j < FM; j++) f[j] = sx[cur][j] * sw[cur];
+        auto join = [&](const f32x16& p, int i, int j) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = fmaf(p[e], f[j], acc[i][j][e]);
+        };
+        if constexpr (EXACT) {
+            f32x16 p[FN][FM];
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                bf16x8 bw[FN], bx[FM];
+#pragma unroll
+                for (int i = 0; i < FN; i++) bw[i] = widen(fw[cur][i][s / 4], s % 4);
+#pragma unroll
+                for (int j = 0; j < FM; j++) bx[j] = widen(fx[cur][j][s / 4], s % 4);
+#pragma unroll
+                for (int i = 0; i < FN; i++)
+#pragma unroll
+                    for (int j = 0; j < FM; j++) p[i][j] = mma32x16(bw[i], bx[j], s == 0 ? zeros() : p[i][j]);
+            }
+#pragma unroll
+            for (int i = 0; i < FN; i++)
+#pragma unroll
+                for (int j = 0; j < FM; j++) join(p[i][j], i, j);
+        } else {
+#pragma unroll
+            for (int i = 0; i < FN; i++)
+#pragma unroll
+                for (int j = 0; j < FM; j++)
+                    join(mma8(fw[cur][i][1], fx[cur][j][1], mma8(fw[cur][i][0], fx[cur][j][0], zeros())), i, j);
+        }
+    };
+    if constexpr (!ASYNC) load_stash(0);
+#pragma unroll
+    for (int s = 0; s < STAGES; s++)
+        if (s < nk) issue(s);
+    if constexpr (ASYNC) wait_slices<STAGES - 1, LPW>(nk - 1 < STAGES - 1 ? nk - 1 : STAGES - 1);
+    wait_lds();
+    raw_barrier();
+    constexpr std::integral_constant<int, 0> zero;
+    constexpr std::integral_constant<int, 1> one;
+    read_slice(0, zero);
+    int kt = 0;
+    for (; kt + 2 < nk; kt += 2) {
+        slice(kt, zero, std::false_type{});
+        slice(kt + 1, one, std::false_type{});
+    }
+    if (kt + 1 < nk) {
+        slice(kt, zero, std::false_type{});
+        slice(kt + 1, one, std::true_type{});
+    } else {
+        slice(kt, zero, std::true_type{});
+    }
+
+    // The k groups' sums, added in their order.
+    if constexpr (WK > 1) {
+        __syncthreads();
+        float* part = reinterpret_cast<float*>(smem) + lane;
+        constexpr int SUMS = FN * FM * 16 * 64;
+        if (wk > 0) {
+            float* p = part + ((wk - 1) * WM * WN + wmn) * SUMS;
+#pragma unroll
+            for (int i = 0; i < FN * FM * 16; i++) p[i * 64] = acc[i / (16 * FM)][i / 16 % FM][i % 16];
+        }
+        __syncthreads();
+        if (wk == 0) {
+#pragma unroll
+            for (int g = 0; g < WK - 1; g++) {
+                const float* p = part + (g * WM * WN + wmn) * SUMS;
+#pragma unroll
+                for (int i = 0; i < FN * FM * 16; i++) acc[i / (16 * FM)][i / 16 % FM][i % 16] += p[i * 64];
+            }
+        }
+    }
+    if (WK > 1 && wk > 0) return;
+
+    // Lane (fr, fh) has of row m0 + wm TM + 32 j + fr the columns from n0 + wn TN + 2 C i + C fh on, C / 16 blocks' sums.
+    auto finish_all = [&](auto whole) {
+#pragma unroll
+        for (int j = 0; j < FM; j++)
+#pragma unroll
+            for (int i = 0; i < FN * 16 / C; i++) {
+                float v[C];
+#pragma unroll
+                for (int e = 0; e < C; e++) v[e] = acc[i * (C / 16) + e / 16][j][e % 16];
+                finish_block<TO, decltype(whole)::value>(a, m0 + wm * TM + 32 * j, n0 + wn * TN + 2 * C * i + C * fh, lane, v,
+                                                         EARLY ? early : nullptr);
+            }
+    };
+    if (rows_n == BN) finish_all(std::true_type{});
+    else finish_all(std::false_type{});
+}
+
+// ---- few rows ---------------------------------------------------------------------------------
+// M <= 16 rows: a workgroup takes 16 columns of Y, its wavefronts share K's blocks and are summed through LDS.  W moves HBM ->
+// registers, each byte once, 32 codes a lane (lane l: W row l % 16, codes 32 (l / 16) .. + 31 of a block), and is multiplied in four 16x16
+// steps of 8 of them; X, the B operand, comes from L2.  Bound by reading W.
+constexpr int kRowWaves = 8;
+template <bool WHOLE>
+__device__ __forceinline__ i32x8 load_codes(const unsigned char* p, int k, int K) {
+    typedef unsigned U4 __attribute__((ext_vector_type(4), aligned(1)));
+    i32x8 f;
+    if (WHOLE || k + 32 <= K) {
+        const U4 lo = *reinterpret_cast<const U4*>(p + k), hi = *reinterpret_cast<const U4*>(p + k + 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            f[e] = lo[e];
+            f[4 + e] = hi[e];
+        }
+        return f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        unsigned v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (k + 4 * e + i < K) v |= (unsigned)p[k + 4 * e + i] << (8 * i);
+        f[e] = v;
+    }
+    return f;
+}
+template <typename TO>
+__global__ __launch_bounds__(64 * kRowWaves) void linear_fp8_rows_kernel(LinearFp8Args args) {
+    const LinearArgs& a = args.l;
+    constexpr int NW = kRowWaves, U = 4;  // blocks in flight
+    __shared__ float sums[NW][16][20];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16, r = lane & 15, piece = lane >> 4;
+    const int n = n0 + r < a.N ? n0 + r : a.N - 1, m = r < a.M ? r : a.M - 1;  // (past them sums that are never stored)
+    const unsigned char* w = static_cast<const unsigned char*>(a.w) + (int64_t)n * a.ldw;
+    const unsigned char* x = static_cast<const unsigned char*>(a.x) + (int64_t)m * a.ldx;
+    const float* xs = args.xs + (int64_t)m * args.ldxs;
+    const uniform_ptr ws = uniform(args.ws + (int64_t)(n0 / kBlock) * args.ldws);
+    const int b0 = (int)((int64_t)args.blocks * wave / NW), b1 = (int)((int64_t)args.blocks * (wave + 1) / NW);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto run = [&](int b, auto whole, auto count) {
+        constexpr int N = decltype(count)::value;
+        i32x8 vw[N], vx[N];
+        float f[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int k = (b + i) * kBlock + 32 * piece;
+            vw[i] = load_codes<decltype(whole)::value>(w, k, a.K);
+            vx[i] = load_codes<decltype(whole)::value>(x, k, a.K);
+            f[i] = xs[b + i] * ws[b + i];
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 4; q++) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(vw[i], q), widen(vx[i], q), p, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] = fmaf(p[e], f[i], acc[e]);
+        }
+    };
+    const int whole = a.K / kBlock < b1 ? a.K / kBlock : b1;  // blocks with all of their codes
+    int b = b0;
+    for (; b + U <= whole; b += U) run(b, std::true_type{}, std::integral_constant<int, U>{});
+    for (; b < whole; b++) run(b, std::true_type{}, std::integral_constant<int, 1>{});
+    for (; b < b1; b++) run(b, std::false_type{}, std::integral_constant<int, 1>{});
+
+    // acc[e]: row m = r, column 4 piece + e.
+    *reinterpret_cast<float4*>(&sums[wave][r][4 * piece]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    const int mm = threadIdx.x >> 2, c = 4 * (threadIdx.x & 3);
+    if (threadIdx.x >= 64 || mm >= a.M || n0 + c >= a.N) return;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < NW; q++) {
+        const float4 p = *reinterpret_cast<const float4*>(&sums[q][mm][c]);
+        v[0] += p.x;
+        v[1] += p.y;
+        v[2] += p.z;
+        v[3] += p.w;
+    }
+    finish<TO>(a, mm, n0 + c, v);
+}
+
+template <typename TO>
+int launch_rows(const LinearFp8Args& a, hipStream_t st, bool go) {
+    const int64_t wgs = ((int64_t)a.l.N + 15) / 16;
+    if (wgs * (64 * kRowWaves) > UINT32_MAX) return -1;
+    if (go) linear_fp8_rows_kernel<TO><<<(unsigned)wgs, 64 * kRowWaves, 0, st>>>(a);
+    return 0;
+}
+
+template <typename TO, int BM, int BN, int WM, int WN, int WK, int STAGES, bool ASYNC>
+int launch_tiles(const LinearFp8Args& a, hipStream_t st, bool go) {
+    constexpr int THREADS = 64 * WM * WN * WK;
+    const int64_t wgs = (int64_t)((a.l.M + BM - 1) / BM) * ((a.l.N + BN - 1) / BN);
+    if (wgs * THREADS > UINT32_MAX) return -1;
+    if (go) linear_fp8_kernel<TO, BM, BN, WM, WN, WK, STAGES, ASYNC><<<(unsigned)wgs, THREADS, 0, st>>>(a);
+    return 0;
+}
+
+}  // namespace
+
+template <typename TO>
+int launch_linear_fp8(const LinearFp8Args& a, hipStream_t st, bool go) {
+    const LinearArgs& l = a.l;
+    if (l.M <= 16) return launch_rows<TO>(a, st, go);
+    // The buffer-to-LDS loads take dword-aligned rows, and windows of a tile's rows below 2^31 bytes.
+    constexpr int64_t FAR = (int64_t)1 << 22;
+    const bool async = !((reinterpret_cast<uintptr_t>(l.x) | reinterpret_cast<uintptr_t>(l.w) | l.ldx | l.ldw) & 3) && l.ldx <= FAR &&
+                       l.ldw <= FAR && l.K <= FAR && a.ldxs * 4 <= FAR;
+    if (!async) return launch_tiles<TO, 128, 128, 4, 2, 1, 2, false>(a, st, go);
+    if ((int64_t)((l.M + 127) / 128) * ((l.N + 127) / 128) < 256) return launch_tiles<TO, 64, 64, 2, 2, 2, 2, true>(a, st, go);
+    return launch_tiles<TO, 128, 128, 4, 2, 1, 2, true>(a, st, go);
+}
+
+template int launch_linear_fp8<bf16>(const LinearFp8Args&, hipStream_t, bool);
+template int launch_linear_fp8<f16>(const LinearFp8Args&, hipStream_t, bool);
+template int launch_linear_fp8<float>(const LinearFp8Args&, hipStream_t, bool);
+
+}  // namespace irodori

@@ -148,6 +148,25 @@ class CrossAttentionDescC(C.Structure):
                 [("mask_stride", C.c_int64)])
 
 
+NORMS = {"none": 0, "rms": 1, "layer": 2}
+
+
+class BlockNormDescC(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "stream_dtype", "h_dtype", "rows", "dim", "branch_norm", "norm", "mod_rows")] +
+                [(n, C.c_float) for n in ("branch_eps", "eps", "stream_scale", "branch_scale")] +
+                [(n, C.c_int64) for n in ("ldx", "ldb", "ldxo", "ldh", "ldhs", "ldm")])
+
+
+class BlockQuantizeDescC(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "rows", "dim", "block_rows", "gated", "activation")] +
+                [(n, C.c_int64) for n in ("ldx", "ldq", "lds")])
+
+
+class LinearFp8DescC(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("out_dtype", "m", "n", "k", "activation", "gate_rows")] +
+                [(n, C.c_int64) for n in ("ldx", "ldw", "ldy", "ldr", "ldxs", "ldws")])
+
+
 # name -> (restype, argtypes): every symbol include/irodori_hip.h declares.
 _vp = C.c_void_p
 SIGNATURES = {
@@ -208,6 +227,9 @@ SIGNATURES = {
     "irodori_op_cross_attention_workspace": (C.c_int, [C.POINTER(CrossAttentionDescC), C.POINTER(C.c_uint64)]),
     "irodori_op_cross_attention": (C.c_int, [C.POINTER(CrossAttentionDescC), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                              C.c_uint64, _vp]),
+    "irodori_op_block_norm": (C.c_int, [C.POINTER(BlockNormDescC)] + [_vp] * 13),
+    "irodori_op_block_quantize": (C.c_int, [C.POINTER(BlockQuantizeDescC), _vp, _vp, _vp, _vp]),
+    "irodori_op_linear_fp8": (C.c_int, [C.POINTER(LinearFp8DescC)] + [_vp] * 9),
     "irodori_op_mx_quantize": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp]),
     "irodori_op_gemm_fp8": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp]),
 }

@@ -618,6 +618,49 @@ class CrossAttentionDesc(L.CrossAttentionDescC):
               seq_kv if mask_stride is None else mask_stride)
 
 
+_H_DTYPES = dict(_OP_DTYPES, fp8=L.DTYPE_FP8)
+
+
+class BlockNormDesc(L.BlockNormDescC):
+    """A call's shape for ops.block_norm (irodori_block_norm_desc), made once and kept: x, branch, x_out and h [rows, dim],
+    gate, scale and shift a row of dim for every mod_rows rows."""
+
+    def __init__(self, rows: int, dim: int, *, dtype: str = "bf16", stream_dtype: str | None = None, h_dtype: str | None = None,
+                 branch_norm: str = "none", norm: str = "rms", branch_eps: float = 1e-5, eps: float = 1e-5,
+                 stream_scale: float = 1.0, branch_scale: float = 1.0, mod_rows: int = 0, ldx: int | None = None,
+                 ldb: int | None = None, ldxo: int | None = None, ldh: int | None = None, ldhs: int | None = None,
+                 ldm: int | None = None):
+        rest = [dim if ld is None else ld for ld in (ldx, ldb, ldxo, ldh)]
+        _fill(self, _choice(_OP_DTYPES, dtype, "dtype"), _choice(_OP_DTYPES, stream_dtype or dtype, "stream_dtype"),
+              _choice(_H_DTYPES, h_dtype or dtype, "h_dtype"), rows, dim, _choice(L.NORMS, branch_norm, "branch_norm"),
+              _choice(L.NORMS, norm, "norm"), mod_rows, branch_eps, eps, stream_scale, branch_scale, *rest,
+              -(-dim // 128) if ldhs is None else ldhs, dim if ldm is None else ldm)
+
+
+class BlockQuantizeDesc(L.BlockQuantizeDescC):
+    """A call's shape for ops.block_quantize (irodori_block_quantize_desc), made once and kept: x [rows, dim], or [rows, 2 dim]
+    where gated, q [rows, dim], scales [ceil(rows / block_rows), ceil(dim / 128)]."""
+
+    def __init__(self, rows: int, dim: int, *, dtype: str = "bf16", block_rows: int = 1, gated: bool = False,
+                 activation: str = "none", ldx: int | None = None, ldq: int | None = None, lds: int | None = None):
+        _fill(self, _choice(_OP_DTYPES, dtype, "dtype"), rows, dim, block_rows, int(gated),
+              _choice(L.ACTIVATIONS, activation, "activation"), (2 * dim if gated else dim) if ldx is None else ldx,
+              dim if ldq is None else ldq, -(-dim // 128) if lds is None else lds)
+
+
+class LinearFp8Desc(L.LinearFp8DescC):
+    """A call's shape for ops.linear_fp8 (irodori_linear_fp8_desc), made once and kept: codes x [m, k] and w [n, k],
+    scales [m, ceil(k / 128)] and [ceil(n / 128), ceil(k / 128)], y [m, n]."""
+
+    def __init__(self, m: int, n: int, k: int, *, out_dtype: str = "bf16", activation: str = "none", gate_rows: int = 0,
+                 ldx: int | None = None, ldw: int | None = None, ldy: int | None = None, ldr: int | None = None,
+                 ldxs: int | None = None, ldws: int | None = None):
+        blocks = -(-k // 128)
+        _fill(self, _choice(_OP_DTYPES, out_dtype, "out_dtype"), m, n, k, _choice(L.ACTIVATIONS, activation, "activation"), gate_rows,
+              k if ldx is None else ldx, k if ldw is None else ldw, n if ldy is None else ldy, n if ldr is None else ldr,
+              blocks if ldxs is None else ldxs, blocks if ldws is None else ldws)
+
+
 class ops:
     """Operator entry points (src/kernels analogues) on device pointers."""
 
@@ -684,3 +727,24 @@ class ops:
         """Attention of each query to its row's keys (mask uint8, lengths int32, each 0 for all)."""
         _check(L.load().irodori_op_cross_attention(desc, d_q, d_k, d_v, d_mask or None, d_q_len or None, d_kv_len or None,
                                                    d_out, d_workspace or None, _workspace_bytes(workspace_bytes), stream or None))
+
+    @staticmethod
+    def block_norm(desc: BlockNormDesc, d_x, d_branch=0, d_branch_weight=0, d_branch_bias=0, d_gate=0, d_x_out=0, d_weight=0,
+                   d_bias=0, d_scale=0, d_shift=0, d_h=0, d_h_scales=0, stream: int = 0) -> None:
+        """x_out = r = stream_scale x + branch_scale gate N_b(branch), h = N(r) (1 + scale) + shift; an argument that is
+        not there is 0."""
+        _check(L.load().irodori_op_block_norm(desc, d_x or None, d_branch or None, d_branch_weight or None, d_branch_bias or None,
+                                              d_gate or None, d_x_out or None, d_weight or None, d_bias or None, d_scale or None,
+                                              d_shift or None, d_h or None, d_h_scales or None, stream or None))
+
+    @staticmethod
+    def block_quantize(desc: BlockQuantizeDesc, d_x, d_q, d_scales, stream: int = 0) -> None:
+        """e4m3 codes and the f32 scales of their blocks."""
+        _check(L.load().irodori_op_block_quantize(desc, d_x or None, d_q or None, d_scales or None, stream or None))
+
+    @staticmethod
+    def linear_fp8(desc: LinearFp8Desc, d_x, d_x_scales, d_w, d_w_scales, d_y, d_bias=0, d_gate=0, d_residual=0,
+                   stream: int = 0) -> None:
+        """y = residual + gate * act(x w^T + bias) of e4m3 codes and their blocks' scales."""
+        _check(L.load().irodori_op_linear_fp8(desc, d_x or None, d_x_scales or None, d_w or None, d_w_scales or None, d_bias or None,
+                                              d_gate or None, d_residual or None, d_y or None, stream or None))
