@@ -295,7 +295,7 @@ void linear_kernel(LinearArgs a) {
                 float v[C];
 #pragma unroll
                 for (int e = 0; e < C; e++) v[e] = acc[i * (C / 16) + e / 16][j][e % 16];
-                finish_block<TO, decltype(whole)::value>(a, m0 + wm * TM + 32 * j, n0 + wn * TN + 2 * C * i + C * fh, lane, v,
+                finish_block<TO, decltype(whole)::value>(a, m0 + wm * TM + 32 * j + fr, n0 + wn * TN + 2 * C * i + C * fh, lane, v,
                                                          EARLY ? early : nullptr);
             }
     };

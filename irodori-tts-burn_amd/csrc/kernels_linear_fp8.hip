@@ -3,8 +3,8 @@
 //
 // A block's product starts from zero in registers of its own and joins the tile's sums by one multiply-add an element
 // with sx sw in f32: the product is formed transposed (W's rows are the A operand), so a lane has one row of Y and one factor a
-// block.  The 16 multiply-adds of a 32 x 32 block take half of the cycles of its two matrix instructions, and run beside
-// others'.  The epilogue is the linear operator's.
+// block.  The 16x16x128 step takes a block at once; its 4 multiply-adds take half of its cycles and run beside others' (register
+// to register, random codes: 3.1 PFLOP/s with them, 3.7 without; the 32x32x64 step 2.8 and 3.6).  The epilogue is the linear operator's.
 //
 // The fp8 matrix instructions align each 8 products of neighbouring codes to the largest and keep 13 bits below its exponent
 // (measured; beyond the 8 their sums are f32): 1.5e-5 relative L2 for normal operands, far below the rounding of a 16-bit Y (1.7e-3
@@ -27,9 +27,19 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef const __attribute__((address_space(4))) float* uniform_ptr;
 __device__ __forceinline__ uniform_ptr uniform(const float* p) { return (uniform_ptr)(uintptr_t)p; }
 
-// The 32 codes a lane supplies to a 64-deep step: K bytes 64 ks + 16 h .. + 15 and 32 more on, h = lane / 32.
-__device__ __forceinline__ f32x16 mma8(const i32x8& a, const i32x8& b, const f32x16& c) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);  // (the form without block scales)
+// The 32 codes a lane (row r, quarter g = lane / 16) supplies of a block: K bytes 16 g .. + 15 and 64 more on.  An LDS row has a
+// block, or several (RB bytes); b is the block in it.
+template <int RB>
+__device__ __forceinline__ i32x8 read_codes(const unsigned char* row, int r, int b, int g) {
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(row + (lswz<RB>(r, 8 * b + g) << 4));
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(row + (lswz<RB>(r, 8 * b + 4 + g) << 4));
+    i32x8 f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        f[e] = lo[e];
+        f[4 + e] = hi[e];
+    }
+    return f;
 }
 // Codes 8 q .. 8 q + 7 of a lane's 32 as bf16, exactly.
 __device__ __forceinline__ bf16x8 widen(const i32x8& v, int q) {
@@ -46,46 +56,82 @@ __device__ __forceinline__ bf16x8 widen(const i32x8& v, int q) {
     }
     return r;
 }
-template <int RB>
-__device__ __forceinline__ i32x8 read_codes(const unsigned char* row, int r, int ks, int h) {
-    const u32x4 lo = *reinterpret_cast<const u32x4*>(row + (lswz<RB>(r, 4 * ks + h) << 4));
-    const u32x4 hi = *reinterpret_cast<const u32x4*>(row + (lswz<RB>(r, 4 * ks + 2 + h) << 4));
-    i32x8 f;
+// A block's product: of the codes, or of their bf16 values.
+template <bool EXACT>
+struct Operand {
+    i32x8 v;
+    __device__ __forceinline__ void set(const i32x8& c) { v = c; }
+};
+template <>
+struct Operand<true> {
+    bf16x8 v[4];
+    __device__ __forceinline__ void set(const i32x8& c) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        f[e] = lo[e];
-        f[4 + e] = hi[e];
+        for (int q = 0; q < 4; q++) v[q] = widen(c, q);
     }
-    return f;
+};
+__device__ __forceinline__ f32x4 product(const Operand<false>& a, const Operand<false>& b) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, zero, 0, 0, 0, 0, 0, 0);  // (the form without block scales)
 }
+__device__ __forceinline__ f32x4 product(const Operand<true>& a, const Operand<true>& b) {
+    f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; q++) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], p, 0, 0, 0);
+    return p;
+}
+// 16 bytes a lane from a buffer window (a uniform offset beside the lane's) to LDS at `to` and 16 times the lane.  By hand, since behind the
+// builtin the compiler lets every LDS read wait for all loads on their way; the waits are wait_vm's.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is the compiler's, which has to know that it changes)
+typedef unsigned Window __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ Window make_window(const void* base, unsigned bytes) {
+    const uint64_t p = (uint64_t)(uintptr_t)base;
+    return Window{(unsigned)p, (unsigned)(p >> 32), bytes, 0x00020000u};
+}
+__device__ __forceinline__ void load_to_lds(Window w, unsigned lane_offset, unsigned offset, void* to) {
+    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)to;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(lane_offset), "s"(w), "s"(offset)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
 // The dword of codes that begins at k without those past K.
 __device__ __forceinline__ int cut_dword(int v, int k, int K) {
     const int left = K - k;
     return left >= 4 ? v : left <= 0 ? 0 : v & ((1 << 8 * left) - 1);
 }
+// W's row of a wave's 16 FN that operand row r of its block i takes, so that a lane ends with 4 FN neighbouring columns of one row of Y,
+// and the operand row of W's row w.
+template <int FN>
+__device__ __forceinline__ int w_row16(int i, int r) {
+    return 4 * FN * (r >> 2) + 4 * i + (r & 3);
+}
+template <int FN>
+__device__ __forceinline__ int operand_row16(int w) {
+    return 4 * (w / (4 * FN) % 4) + (w & 3);
+}
 
 // A tile of BM rows and BN columns of Y per workgroup of WM x WN x WK wavefronts.  K advances in slices of WK blocks of 128
 // codes, one for each of the WK, which are summed through LDS at the end.  ASYNC: slices move HBM -> LDS by
-// buffer_load_dwordx4 ... lds, which take dword-aligned rows, up to STAGES ahead; a piece that straddles K's end is cut in the
-// last slice's fragments.  Otherwise through registers.  The scales of X come along every fourth block.
-template <typename TO, int BM, int BN, int WM, int WN, int WK, int STAGES, bool ASYNC>
-__global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_eu(WM * WN * WK <= 4 ? 1 : 2)))
-void linear_fp8_kernel(LinearFp8Args args) {
+// buffer_load_dwordx4 ... lds, which take dword-aligned rows; a piece that straddles K's end is cut
+// in the last slice.  Otherwise through registers.  The scales of X come along every fourth block.
+template <typename TO, int BM, int BN, int WM, int WN, int WK, int STAGES, bool ASYNC, bool AHEAD, int EU>
+__global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_eu(EU, EU))) void linear_fp8_kernel(LinearFp8Args args) {
     const LinearArgs& a = args.l;
-    constexpr int NW = WM * WN * WK, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+    constexpr bool EXACT = sizeof(TO) == 4;
+    constexpr int NW = WM * WN * WK, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
     constexpr int RB = 128 * WK, ROWS = BM + BN, STAGE = ROWS * RB, RC = RB / 16;
     constexpr int RPI = 64 / RC, LPW = ROWS / RPI / NW;  // rows a load instruction fills, instructions per wave per slice
     constexpr int PER = 4 / WK, SLOTS = WK == 4 ? STAGES : 2;  // slices that share a load of scales, loads held
     constexpr int SROWS = BM < 64 ? 64 : BM;
-    constexpr bool PAIR = FN % 2 == 0 && sizeof(TO) == 2;
-    constexpr int C = PAIR ? 32 : 16;  // neighbouring columns of Y a lane ends with
+    constexpr int C = 4 * FN;  // neighbouring columns of Y a lane ends with
     static_assert(LPW * RPI * NW == ROWS && BN % RPI == 0 && NW * 64 >= SROWS && 128 % TN == 0, "slices split over the waves");
     static_assert(WK == 1 || (WK - 1) * BM * BN * 4 <= STAGES * STAGE, "the k groups' sums fit the ring");
-    static_assert(STAGES <= 3, "a load of scales is replaced when the slices of the one before it are all being read");
+    static_assert(STAGES <= 3, "a load of scales is replaced when the slices of the one before it are all read");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * STAGE];
     __shared__ __attribute__((aligned(1024))) float xscale[SLOTS][SROWS][4];
 
-    const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
+    const int lane = threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wk = wave / (WM * WN), wmn = wave % (WM * WN), wm = wmn / WN, wn = wmn % WN;
     // Groups of 8 row tiles sweep the column tiles, an XCD's workgroups consecutive.
@@ -107,15 +153,15 @@ void linear_fp8_kernel(LinearFp8Args args) {
     // lane -> row lane / RC, physical chunk lane % RC, which holds the row's chunk `chunk`.
     auto chunk = [&](int i) {
         const int r = (wave * LPW + i) * RPI + lane / RC;
-        return lswz<RB>(r < BN ? operand_row<PAIR>(r) : r, lane % RC);
+        return lswz<RB>(r < BN ? operand_row16<FN>(r) : r, lane % RC);
     };
-    [[maybe_unused]] __amdgpu_buffer_rsrc_t rX, rW, rS;
+    [[maybe_unused]] Window rX, rW, rS;
     [[maybe_unused]] unsigned voff[LPW], soff = 0;
     if constexpr (ASYNC) {
         // Windows end with the last row's last whole dword (its other bytes are in the same memory word).
-        rX = make_rsrc(X, ((unsigned)((int64_t)(rows_m - 1) * a.ldx + a.K) + 3) & ~3u);
-        rW = make_rsrc(W, ((unsigned)((int64_t)(rows_n - 1) * a.ldw + a.K) + 3) & ~3u);
-        rS = make_rsrc(XS, (unsigned)((int64_t)(rows_m - 1) * args.ldxs + args.blocks) * 4u);
+        rX = make_window(X, ((unsigned)((int64_t)(rows_m - 1) * a.ldx + a.K) + 3) & ~3u);
+        rW = make_window(W, ((unsigned)((int64_t)(rows_n - 1) * a.ldw + a.K) + 3) & ~3u);
+        rS = make_window(XS, (unsigned)((int64_t)(rows_m - 1) * args.ldxs + args.blocks) * 4u);
 #pragma unroll
         for (int i = 0; i < LPW; i++) {
             const int r = (wave * LPW + i) * RPI + lane / RC;
@@ -156,161 +202,167 @@ void linear_fp8_kernel(LinearFp8Args args) {
         if (kt % PER == 0 && wave < SROWS / 64) {
             float* dst = &xscale[kt / PER % SLOTS][64 * wave][0];
             if constexpr (ASYNC) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rS, (__attribute__((address_space(3))) void*)dst, 16, soff + kt * WK * 4u, 0, 0, 0);
+                load_to_lds(rS, soff + kt * WK * 4u, 0, dst);
             } else {
                 *reinterpret_cast<f32x4*>(dst + 4 * lane) = sstash;
             }
         }
         unsigned char* dst = smem + kt % STAGES * STAGE + wave * LPW * 1024;
+        if constexpr (ASYNC) {
+            auto load = [&](int i, unsigned vo, unsigned so) {
+                load_to_lds((wave * LPW + i) * RPI < BN ? rW : rX, vo, so, dst + i * 1024);
+            };
+            if ((kt + 1) * RB <= a.K) {
 #pragma unroll
-        for (int i = 0; i < LPW; i++) {
-            if constexpr (ASYNC) {
-                // Pieces past K read as zero (windows are below 2^31 bytes, the offsets whole in the checked part).
-                const unsigned vo = kt * RB + chunk(i) * 16 < a.K ? voff[i] + (unsigned)kt * RB : 0x80000000u;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds((wave * LPW + i) * RPI < BN ? rW : rX,
-                                                         (__attribute__((address_space(3))) void*)(dst + i * 1024), 16,
-                                                         vo, 0, 0, 0);
-            } else {
-                *reinterpret_cast<u32x4*>(dst + i * 1024 + 16 * lane) = stash[i];
+                for (int i = 0; i < LPW; i++) load(i, voff[i], kt * RB);
+            } else {  // pieces past K read as zero, the offsets whole in the part that is checked against the window
+#pragma unroll
+                for (int i = 0; i < LPW; i++) load(i, kt * RB + chunk(i) * 16 < a.K ? voff[i] + (unsigned)kt * RB : 0x80000000u, 0);
             }
-        }
-        if constexpr (!ASYNC) {
+        } else {
+#pragma unroll
+            for (int i = 0; i < LPW; i++) *reinterpret_cast<u32x4*>(dst + i * 1024 + 16 * lane) = stash[i];
             if (kt + 1 < nk) load_stash(kt + 1);
         }
     };
 
-    constexpr bool EXACT = sizeof(TO) == 4;
-    auto zeros = [] {
-        f32x16 z;
+    f32x4 acc[FM][FN];
 #pragma unroll
-        for (int e = 0; e < 16; e++) z[e] = 0.f;
-        return z;
-    };
-    f32x16 acc[FN][FM];
+    for (int j = 0; j < FM; j++)
 #pragma unroll
-    for (int i = 0; i < FN; i++)
+        for (int i = 0; i < FN; i++)
 #pragma unroll
-        for (int j = 0; j < FM; j++) acc[i][j] = zeros();
+            for (int e = 0; e < 4; e++) acc[j][i][e] = 0.f;
 
-    // One block a wavefront: its residual comes under the products.
-    constexpr bool EARLY = FM * FN == 1;
-    [[maybe_unused]] u32x4 early[kLanes<TO, C>];
-    if constexpr (EARLY) {
-        constexpr int Q = kLanes<TO, C>;
-        const int t = lane & (Q - 1);
-        if (a.residual && wk == 0) load_pieces<TO, false>(a, m0 + wm * TM + fr - t, n0 + wn * TN + 16 * fh + t * kPiece<TO>, early);
-    }
-
-    // Two sets of fragments: a slice's are read while the one before multiplies.  The slot that every wave has read by then is
-    // filled again.
-    i32x8 fw[2][FN][2], fx[2][FM][2];
-    float sx[2][FM], sw[2];
-    auto read_slice = [&](int kt, auto set) {
-        const unsigned char* st = smem + kt % STAGES * STAGE;
-        const int b = kt * WK + wk;
-        sw[set] = ws[b < args.blocks ? b : 0];
+    // Where K ends inside a 16-byte piece, its bytes past K in the last slice (they are the next row's) become zero.
+    [[maybe_unused]] auto cut_tail = [&](int kt) {
+        const int c = (a.K - kt * RB) / 16, left = a.K % 16;
+        for (int r = threadIdx.x; r < ROWS; r += 64 * NW) {
+            u32x4* piece = reinterpret_cast<u32x4*>(smem + kt % STAGES * STAGE + r * RB + (lswz<RB>(r < BN ? operand_row16<FN>(r) : r, c) << 4));
+            u32x4 v = *piece;
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-#pragma unroll
-            for (int i = 0; i < FN; i++) fw[set][i][s] = read_codes<RB>(st + (wn * TN + w_row<PAIR>(i, fr)) * RB, fr, 2 * wk + s, fh);
-#pragma unroll
-            for (int j = 0; j < FM; j++) fx[set][j][s] = read_codes<RB>(st + (BN + wm * TM + 32 * j + fr) * RB, fr, 2 * wk + s, fh);
+            for (int e = 0; e < 4; e++) v[e] = cut_dword(v[e], 4 * e, left);
+            *piece = v;
         }
+        wait_lds();
+        raw_barrier();
+    };
+    // Slice kt is there for every wave, and every wave has read the ones before it: of the later slices that were issued, `ahead` at most
+    // may be on their way.
+    auto arrive = [&](int kt, auto ahead) {
+        constexpr int A = decltype(ahead)::value;
+        if constexpr (ASYNC) wait_slices<A, LPW>(nk - 1 - kt < A ? nk - 1 - kt : A);
+        wait_lds();
+        raw_barrier();
+        if constexpr (ASYNC) {
+            if (kt == nk - 1 && a.K % 16) cut_tail(kt);
+        }
+    };
+    auto read_w = [&](int kt, int i) { return read_codes<RB>(smem + kt % STAGES * STAGE + (wn * TN + w_row16<FN>(i, fr)) * RB, fr, wk, fg); };
+    auto read_x = [&](int kt, int j) { return read_codes<RB>(smem + kt % STAGES * STAGE + (BN + wm * TM + 16 * j + fr) * RB, fr, wk, fg); };
+    // Of blocks past K, which a slice of several may have, X's scale is 0 (what is read for them is anything) and W's that of the first.
+    auto within = [&](int kt) { return WK == 1 || kt * WK + wk < args.blocks ? ~0u : 0u; };
+    auto read_scale = [&](int kt, int j) {
+        const float s = xscale[kt / PER % SLOTS][wm * TM + 16 * j + fr][(kt * WK + wk) % 4];
+        return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, s) & within(kt));
+    };
+    auto w_scale = [&](int kt) { return ws[within(kt) ? kt * WK + wk : 0]; };
+    // A product's sums are joined behind the next product, under its cycles.
+    f32x4 pending;
+    float pending_f = 0.f;
+    auto join = [&](int j, int i) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[j][i][e] = fmaf(pending[e], pending_f, acc[j][i][e]);
+    };
+    auto multiply = [&](const Operand<EXACT>& w, const Operand<EXACT>& x, float f, int j, int i) {
+        const f32x4 p = product(w, x);
+        if constexpr (!EXACT) __builtin_amdgcn_sched_barrier(0);
+        if (j > 0 || i > 0) join(i > 0 ? j : j - 1, i > 0 ? i - 1 : FN - 1);
+        pending = p;
+        pending_f = f;
+        if (j == FM - 1 && i == FN - 1) join(j, i);
+        if constexpr (!EXACT) __builtin_amdgcn_sched_barrier(0);
+    };
+    // Two ways through a slice.  AHEAD: the fragments of the next one are read under this one's products, from two sets, and the slot
+    // that every wave has read is filled again before the products: STAGES slices of lookahead.  Otherwise, where two sets are too
+    // many registers, W's fragments are held, X's come one block of 16 rows ahead: STAGES - 1 slices.
+    [[maybe_unused]] i32x8 cw[AHEAD ? 2 : 1][FN], cx[AHEAD ? 2 : 1][FM];
+    [[maybe_unused]] float sx[2][FM], sw[2];
+    [[maybe_unused]] auto read_slice = [&](int kt, auto set) {
+        sw[set] = w_scale(kt);
+#pragma unroll
+        for (int i = 0; i < FN; i++) cw[set][i] = read_w(kt, i);
 #pragma unroll
         for (int j = 0; j < FM; j++) {
-            const float s = xscale[kt / PER % SLOTS][wm * TM + 32 * j + fr][b % 4];
-            sx[set][j] = b < args.blocks ? s : 0.f;
+            cx[set][j] = read_x(kt, j);
+            sx[set][j] = read_scale(kt, j);
         }
     };
-    auto cut = [&](i32x8& f, int k) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = cut_dword(f[e], k + 4 * (e & 3) + 32 * (e >> 2), a.K);
-    };
-    auto slice = [&](int kt, auto cur, auto last) {
-        constexpr std::integral_constant<int, 1 - decltype(cur)::value> next;
-        if constexpr (!decltype(last)::value) {
-            const int left = nk - 2 - kt;
-            if constexpr (ASYNC) wait_slices<STAGES - 2, LPW>(left < STAGES - 2 ? left : STAGES - 2);
-            wait_lds();
-            raw_barrier();
-            read_slice(kt + 1, next);
+    [[maybe_unused]] auto slice_ahead = [&](int kt, auto cur) {
+        if (kt + 1 < nk) {
+            arrive(kt + 1, std::integral_constant<int, STAGES - 2>{});
+            read_slice(kt + 1, std::integral_constant<int, 1 - decltype(cur)::value>{});
             if (kt + STAGES < nk) issue(kt + STAGES);
-        } else if constexpr (ASYNC) {
-            if (a.K % 16) {
-#pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const int k = kt * RB + 128 * wk + 64 * s + 16 * fh;
-#pragma unroll
-                    for (int i = 0; i < FN; i++) cut(fw[cur][i][s], k);
-#pragma unroll
-                    for (int j = 0; j < FM; j++) cut(fx[cur][j][s], k);
-                }
-            }
         }
-        float f[FM];
+        Operand<EXACT> w[FN];
 #pragma unroll
-        for (int j = 0; j < FM; j++) f[j] = sx[cur][j] * sw[cur];
-        auto join = [&](const f32x16& p, int i, int j) {
+        for (int i = 0; i < FN; i++) w[i].set(cw[cur][i]);
 #pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = fmaf(p[e], f[j], acc[i][j][e]);
+        for (int j = 0; j < FM; j++) {
+            Operand<EXACT> x;
+            x.set(cx[cur][j]);
+            const float f = sx[cur][j] * sw[cur];
+#pragma unroll
+            for (int i = 0; i < FN; i++) multiply(w[i], x, f, j, i);
+        }
+    };
+    [[maybe_unused]] auto slice_held = [&](int kt) {
+        arrive(kt, std::integral_constant<int, STAGES - 2>{});
+        if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1);
+        const float ws = w_scale(kt);
+        Operand<EXACT> w[FN], x[2];
+        float f[2];
+        auto next_x = [&](int j) {
+            x[j & 1].set(read_x(kt, j));
+            f[j & 1] = read_scale(kt, j) * ws;
         };
-        if constexpr (EXACT) {
-            f32x16 p[FN][FM];
 #pragma unroll
-            for (int s = 0; s < 8; s++) {
-                bf16x8 bw[FN], bx[FM];
+        for (int i = 0; i < FN; i++) w[i].set(read_w(kt, i));
+        next_x(0);
 #pragma unroll
-                for (int i = 0; i < FN; i++) bw[i] = widen(fw[cur][i][s / 4], s % 4);
+        for (int j = 0; j < FM; j++) {
+            if (j + 1 < FM) next_x(j + 1);
 #pragma unroll
-                for (int j = 0; j < FM; j++) bx[j] = widen(fx[cur][j][s / 4], s % 4);
-#pragma unroll
-                for (int i = 0; i < FN; i++)
-#pragma unroll
-                    for (int j = 0; j < FM; j++) p[i][j] = mma32x16(bw[i], bx[j], s == 0 ? zeros() : p[i][j]);
-            }
-#pragma unroll
-            for (int i = 0; i < FN; i++)
-#pragma unroll
-                for (int j = 0; j < FM; j++) join(p[i][j], i, j);
-        } else {
-#pragma unroll
-            for (int i = 0; i < FN; i++)
-#pragma unroll
-                for (int j = 0; j < FM; j++)
-                    join(mma8(fw[cur][i][1], fx[cur][j][1], mma8(fw[cur][i][0], fx[cur][j][0], zeros())), i, j);
+            for (int i = 0; i < FN; i++) multiply(w[i], x[j & 1], f[j & 1], j, i);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     if constexpr (!ASYNC) load_stash(0);
 #pragma unroll
-    for (int s = 0; s < STAGES; s++)
+    for (int s = 0; s < (AHEAD ? STAGES : STAGES - 1); s++)
         if (s < nk) issue(s);
-    if constexpr (ASYNC) wait_slices<STAGES - 1, LPW>(nk - 1 < STAGES - 1 ? nk - 1 : STAGES - 1);
-    wait_lds();
-    raw_barrier();
-    constexpr std::integral_constant<int, 0> zero;
-    constexpr std::integral_constant<int, 1> one;
-    read_slice(0, zero);
-    int kt = 0;
-    for (; kt + 2 < nk; kt += 2) {
-        slice(kt, zero, std::false_type{});
-        slice(kt + 1, one, std::false_type{});
-    }
-    if (kt + 1 < nk) {
-        slice(kt, zero, std::false_type{});
-        slice(kt + 1, one, std::true_type{});
+    if constexpr (AHEAD) {
+        constexpr std::integral_constant<int, 0> zero;
+        constexpr std::integral_constant<int, 1> one;
+        arrive(0, std::integral_constant<int, STAGES - 1>{});
+        read_slice(0, zero);
+        for (int kt = 0; kt < nk; kt += 2) {
+            slice_ahead(kt, zero);
+            if (kt + 1 < nk) slice_ahead(kt + 1, one);
+        }
     } else {
-        slice(kt, zero, std::true_type{});
+        for (int kt = 0; kt < nk; kt++) slice_held(kt);
     }
 
     // The k groups' sums, added in their order.
     if constexpr (WK > 1) {
         __syncthreads();
         float* part = reinterpret_cast<float*>(smem) + lane;
-        constexpr int SUMS = FN * FM * 16 * 64;
+        constexpr int SUMS = FN * FM * 4 * 64;
         if (wk > 0) {
             float* p = part + ((wk - 1) * WM * WN + wmn) * SUMS;
 #pragma unroll
-            for (int i = 0; i < FN * FM * 16; i++) p[i * 64] = acc[i / (16 * FM)][i / 16 % FM][i % 16];
+            for (int i = 0; i < FN * FM * 4; i++) p[i * 64] = acc[i / (4 * FN)][i / 4 % FN][i % 4];
         }
         __syncthreads();
         if (wk == 0) {
@@ -318,24 +370,21 @@ void linear_fp8_kernel(LinearFp8Args args) {
             for (int g = 0; g < WK - 1; g++) {
                 const float* p = part + (g * WM * WN + wmn) * SUMS;
 #pragma unroll
-                for (int i = 0; i < FN * FM * 16; i++) acc[i / (16 * FM)][i / 16 % FM][i % 16] += p[i * 64];
+                for (int i = 0; i < FN * FM * 4; i++) acc[i / (4 * FN)][i / 4 % FN][i % 4] += p[i * 64];
             }
         }
     }
     if (WK > 1 && wk > 0) return;
 
-    // Lane (fr, fh) has of row m0 + wm TM + 32 j + fr the columns from n0 + wn TN + 2 C i + C fh on, C / 16 blocks' sums.
+    // Lane (fr, fg) has of row m0 + wm TM + 16 j + fr the columns from n0 + wn TN + C fg on.
     auto finish_all = [&](auto whole) {
 #pragma unroll
-        for (int j = 0; j < FM; j++)
+        for (int j = 0; j < FM; j++) {
+            float v[C];
 #pragma unroll
-            for (int i = 0; i < FN * 16 / C; i++) {
-                float v[C];
-#pragma unroll
-                for (int e = 0; e < C; e++) v[e] = acc[i * (C / 16) + e / 16][j][e % 16];
-                finish_block<TO, decltype(whole)::value>(a, m0 + wm * TM + 32 * j, n0 + wn * TN + 2 * C * i + C * fh, lane, v,
-                                                         EARLY ? early : nullptr);
-            }
+            for (int e = 0; e < C; e++) v[e] = acc[j][e / 4][e % 4];
+            finish_block<TO, decltype(whole)::value>(a, m0 + wm * TM + 16 * j + fr, n0 + wn * TN + C * fg, lane, v);
+        }
     };
     if (rows_n == BN) finish_all(std::true_type{});
     else finish_all(std::false_type{});
@@ -396,9 +445,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void linear_fp8_rows_kernel(LinearF
         }
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            f32x4 p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int q = 0; q < 4; q++) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(vw[i], q), widen(vx[i], q), p, 0, 0, 0);
+            Operand<true> ow, ox;
+            ow.set(vw[i]);
+            ox.set(vx[i]);
+            const f32x4 p = product(ow, ox);
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[e] = fmaf(p[e], f[i], acc[e]);
         }
@@ -434,12 +484,12 @@ int launch_rows(const LinearFp8Args& a, hipStream_t st, bool go) {
     return 0;
 }
 
-template <typename TO, int BM, int BN, int WM, int WN, int WK, int STAGES, bool ASYNC>
+template <typename TO, int BM, int BN, int WM, int WN, int WK, int STAGES, bool ASYNC, bool AHEAD, int EU>
 int launch_tiles(const LinearFp8Args& a, hipStream_t st, bool go) {
     constexpr int THREADS = 64 * WM * WN * WK;
     const int64_t wgs = (int64_t)((a.l.M + BM - 1) / BM) * ((a.l.N + BN - 1) / BN);
     if (wgs * THREADS > UINT32_MAX) return -1;
-    if (go) linear_fp8_kernel<TO, BM, BN, WM, WN, WK, STAGES, ASYNC><<<(unsigned)wgs, THREADS, 0, st>>>(a);
+    if (go) linear_fp8_kernel<TO, BM, BN, WM, WN, WK, STAGES, ASYNC, AHEAD, EU><<<(unsigned)wgs, THREADS, 0, st>>>(a);
     return 0;
 }
 
@@ -453,9 +503,9 @@ int launch_linear_fp8(const LinearFp8Args& a, hipStream_t st, bool go) {
     constexpr int64_t FAR = (int64_t)1 << 22;
     const bool async = !((reinterpret_cast<uintptr_t>(l.x) | reinterpret_cast<uintptr_t>(l.w) | l.ldx | l.ldw) & 3) && l.ldx <= FAR &&
                        l.ldw <= FAR && l.K <= FAR && a.ldxs * 4 <= FAR;
-    if (!async) return launch_tiles<TO, 128, 128, 4, 2, 1, 2, false>(a, st, go);
-    if ((int64_t)((l.M + 127) / 128) * ((l.N + 127) / 128) < 256) return launch_tiles<TO, 64, 64, 2, 2, 2, 2, true>(a, st, go);
-    return launch_tiles<TO, 128, 128, 4, 2, 1, 2, true>(a, st, go);
+    if (!async) return launch_tiles<TO, 128, 128, 4, 2, 1, 2, false, true, 2>(a, st, go);
+    if ((int64_t)((l.M + 127) / 128) * ((l.N + 127) / 128) < 256) return launch_tiles<TO, 64, 64, 2, 2, 2, 2, true, true, 2>(a, st, go);
+    return launch_tiles<TO, 128, 128, 4, 2, 1, 2, true, true, 2>(a, st, go);
 }
 
 template int launch_linear_fp8<bf16>(const LinearFp8Args&, hipStream_t, bool);

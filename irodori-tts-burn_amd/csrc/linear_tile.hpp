@@ -159,7 +159,7 @@ __device__ __forceinline__ void exchange(u32x4 (&p)[Q], int lane) {
             }
         }
     };
-    step(std::integral_constant<int, 1>{}, std::integral_constant<int, 0xb1>{});  // lane ^ 1
+    if constexpr (Q >= 2) step(std::integral_constant<int, 1>{}, std::integral_constant<int, 0xb1>{});  // lane ^ 1
     if constexpr (Q == 4) step(std::integral_constant<int, 2>{}, std::integral_constant<int, 0x4e>{});  // lane ^ 2
 }
 // Columns of Y in 16 bytes, and how many lanes exchange where each has C columns of a row.
@@ -188,12 +188,13 @@ __device__ __forceinline__ void load_pieces(const LinearArgs& a, int m, int n, u
         p[s] = __builtin_bit_cast(u32x4, o);
     }
 }
-// C columns of Y from n on, rows m0 + lane % 32, from their sums; by a whole wavefront.  WHOLE: all the columns are in Y.
+// C columns of Y from n on, of the lane's row m (neighbouring lanes have neighbouring rows), from their sums; by a whole wavefront.
+// WHOLE: all the columns are in Y.
 template <typename TO, bool WHOLE, int C>
-__device__ __forceinline__ void finish_block(const LinearArgs& a, int m0, int n, int lane, float (&v)[C], const u32x4* residual = nullptr) {
+__device__ __forceinline__ void finish_block(const LinearArgs& a, int m, int n, int lane, float (&v)[C], const u32x4* residual = nullptr) {
     constexpr int E = kPiece<TO>, Q = kLanes<TO, C>;
     typedef TO OE __attribute__((ext_vector_type(E), aligned(sizeof(TO))));
-    const int m = m0 + (lane & 31), t = lane & (Q - 1), mq = m - t, left = WHOLE ? C : a.N - n;
+    const int t = lane & (Q - 1), mq = m - t, left = WHOLE ? C : a.N - n;
     if (left > 0) {
         float f[C];
         if (a.bias) {
