@@ -29,10 +29,19 @@ __device__ __forceinline__ uniform_ptr uniform(const float* p) { return (uniform
 
 // The 32 codes a lane (row r, quarter g = lane / 16) supplies of a block: K bytes 16 g .. + 15 and 64 more on.  An LDS row has a
 // block, or several (RB bytes); b is the block in it.
+typedef const __attribute__((address_space(3))) unsigned char* lds_ptr;
+__device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(lds_ptr)p; }
+struct Pieces {
+    unsigned lo, hi;  // the LDS addresses of the two
+};
 template <int RB>
-__device__ __forceinline__ i32x8 read_codes(const unsigned char* row, int r, int b, int g) {
-    const u32x4 lo = *reinterpret_cast<const u32x4*>(row + (lswz<RB>(r, 8 * b + g) << 4));
-    const u32x4 hi = *reinterpret_cast<const u32x4*>(row + (lswz<RB>(r, 8 * b + 4 + g) << 4));
+__device__ __forceinline__ Pieces pieces_of(unsigned row, int r, int b, int g) {
+    return {row + (lswz<RB>(r, 8 * b + g) << 4), row + (lswz<RB>(r, 8 * b + 4 + g) << 4)};
+}
+// `further`: a constant number of bytes.
+__device__ __forceinline__ i32x8 read_codes(const Pieces& p, int further) {
+    typedef const __attribute__((address_space(3))) u32x4* piece_ptr;
+    const u32x4 lo = *(piece_ptr)((lds_ptr)(uintptr_t)p.lo + further), hi = *(piece_ptr)((lds_ptr)(uintptr_t)p.hi + further);
     i32x8 f;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -80,7 +89,7 @@ __device__ __forceinline__ f32x4 product(const Operand<true>& a, const Operand<t
     for (int q = 0; q < 4; q++) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], p, 0, 0, 0);
     return p;
 }
-// 16 bytes a lane from a buffer window (a uniform offset beside the lane's) to LDS at `to` and 16 times the lane.  By hand, since behind the
+// 16 bytes a lane from a buffer window to LDS at `to` (the same in every lane) and 16 times the lane.  By hand, since behind the
 // builtin the compiler lets every LDS read wait for all loads on their way; the waits are wait_vm's.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // (m0 is the compiler's, which has to know that it changes)
@@ -89,9 +98,9 @@ __device__ __forceinline__ Window make_window(const void* base, unsigned bytes) 
     const uint64_t p = (uint64_t)(uintptr_t)base;
     return Window{(unsigned)p, (unsigned)(p >> 32), bytes, 0x00020000u};
 }
-__device__ __forceinline__ void load_to_lds(Window w, unsigned lane_offset, unsigned offset, void* to) {
-    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)to;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(lane_offset), "s"(w), "s"(offset)
+__device__ __forceinline__ void load_to_lds(Window w, unsigned offset, unsigned to) {
+    const int at = __builtin_amdgcn_readfirstlane((int)to);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset), "s"(w)
                  : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -121,15 +130,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
     constexpr bool EXACT = sizeof(TO) == 4;
     constexpr int NW = WM * WN * WK, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
     constexpr int RB = 128 * WK, ROWS = BM + BN, STAGE = ROWS * RB, RC = RB / 16;
-    constexpr int RPI = 64 / RC, LPW = ROWS / RPI / NW;  // rows a load instruction fills, instructions per wave per slice
+    constexpr int RPI = 64 / RC, LPW = ROWS / RPI / NW, LW = BN / RPI / NW;  // rows a load instruction fills; a wave's per slice, W's of them
     constexpr int PER = 4 / WK, SLOTS = WK == 4 ? STAGES : 2;  // slices that share a load of scales, loads held
     constexpr int SROWS = BM < 64 ? 64 : BM;
     constexpr int C = 4 * FN;  // neighbouring columns of Y a lane ends with
-    static_assert(LPW * RPI * NW == ROWS && BN % RPI == 0 && NW * 64 >= SROWS && 128 % TN == 0, "slices split over the waves");
+    static_assert(LPW * RPI * NW == ROWS && LW * RPI * NW == BN && NW * 64 >= SROWS && 128 % TN == 0, "slices split over the waves");
     static_assert(WK == 1 || (WK - 1) * BM * BN * 4 <= STAGES * STAGE, "the k groups' sums fit the ring");
     static_assert(STAGES <= 3, "a load of scales is replaced when the slices of the one before it are all read");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * STAGE];
-    __shared__ __attribute__((aligned(1024))) float xscale[SLOTS][SROWS][4];
+    __shared__ __attribute__((aligned(1024))) float xscale[SLOTS][SROWS][4], wscale[SLOTS][64][4];
 
     const int lane = threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -144,44 +153,52 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
     const unsigned char* X = static_cast<const unsigned char*>(a.x) + (int64_t)m0 * a.ldx;
     const unsigned char* W = static_cast<const unsigned char*>(a.w) + (int64_t)n0 * a.ldw;
     const float* XS = args.xs + (int64_t)m0 * args.ldxs;
-    // The wave's columns share their scales (columns past N, which are not stored, take the last ones').
-    const int wblock = n0 + wn * TN < a.N ? (n0 + wn * TN) / kBlock : (a.N - 1) / kBlock;
-    const uniform_ptr ws = uniform(args.ws + (int64_t)wblock * args.ldws);
+    // The wave's columns share their scales.
+    const int wblock = (n0 % kBlock + wn * TN) / kBlock, wblocks = (n0 % kBlock + rows_n + kBlock - 1) / kBlock;
+    const float* WS = args.ws + (int64_t)(n0 / kBlock) * args.ldws;
     const int nk = (args.blocks + WK - 1) / WK;
 
-    // Load instruction i of this wave fills stage rows RPI (wave LPW + i) .. (W rows, then X rows):
+    // Load instruction i of this wave fills stage rows RPI (i NW + wave) .. (the first LW instructions W rows, the others X rows):
     // lane -> row lane / RC, physical chunk lane % RC, which holds the row's chunk `chunk`.
     auto chunk = [&](int i) {
-        const int r = (wave * LPW + i) * RPI + lane / RC;
-        return lswz<RB>(r < BN ? operand_row16<FN>(r) : r, lane % RC);
+        const int r = (i * NW + wave) * RPI + lane / RC;
+        return lswz<RB>(i < LW ? operand_row16<FN>(r) : r, lane % RC);
     };
-    [[maybe_unused]] Window rX, rW, rS;
-    [[maybe_unused]] unsigned voff[LPW], soff = 0;
+    [[maybe_unused]] Window rX, rW, rXS, rWS;
     if constexpr (ASYNC) {
         // Windows end with the last row's last whole dword (its other bytes are in the same memory word).
         rX = make_window(X, ((unsigned)((int64_t)(rows_m - 1) * a.ldx + a.K) + 3) & ~3u);
         rW = make_window(W, ((unsigned)((int64_t)(rows_n - 1) * a.ldw + a.K) + 3) & ~3u);
-        rS = make_window(XS, (unsigned)((int64_t)(rows_m - 1) * args.ldxs + args.blocks) * 4u);
-#pragma unroll
-        for (int i = 0; i < LPW; i++) {
-            const int r = (wave * LPW + i) * RPI + lane / RC;
-            // Rows past the last (which short strides would leave inside the window) lie behind it and read as zero.
-            const bool there = r < BN ? r < rows_n : r - BN < rows_m;
-            voff[i] = there ? (unsigned)(r < BN ? r * a.ldw : (r - BN) * a.ldx) + chunk(i) * 16u : 0x80000000u;
-        }
-        soff = 64 * wave + lane < rows_m ? (unsigned)((64 * wave + lane) * args.ldxs) * 4u : 0x80000000u;
+        rXS = make_window(XS, (unsigned)((int64_t)(rows_m - 1) * args.ldxs + args.blocks) * 4u);
+        rWS = make_window(WS, (unsigned)((int64_t)(wblocks - 1) * args.ldws + args.blocks) * 4u);
     }
+    // Where load instruction i of slice kt reads, whole in the part that is checked against the window.  Rows past the last lie behind it
+    // and read as zero, as do pieces of its last row past K (with rows closer than K apart they hold codes, which none of Y's sees).
+    constexpr int STEP = NW * RPI;  // rows from one instruction of a wave to the next
+    constexpr bool SAME = STEP % (16 * FN) == 0;  // a lane's chunk is the same in all of them
+    [[maybe_unused]] unsigned woff[SAME ? 1 : LW], xoff[SAME ? 1 : LPW - LW];
+    if constexpr (ASYNC) {
+#pragma unroll
+        for (int i = 0; i < (SAME ? 1 : LW); i++) woff[i] = (wave * RPI + lane / RC) * (unsigned)a.ldw + 16u * chunk(i);
+#pragma unroll
+        for (int i = 0; i < (SAME ? 1 : LPW - LW); i++) xoff[i] = (wave * RPI + lane / RC) * (unsigned)a.ldx + 16u * chunk(LW + i);
+    }
+    [[maybe_unused]] auto offset = [&](int kt, int i) __attribute__((always_inline)) {
+        const unsigned step = (i < LW ? i * (unsigned)a.ldw : (i - LW) * (unsigned)a.ldx) * STEP + kt * RB;
+        return (i < LW ? woff[SAME ? 0 : i] : xoff[SAME ? 0 : i - LW]) + step;
+    };
+    [[maybe_unused]] const unsigned xsoff = (64 * wave + lane) * (unsigned)args.ldxs * 4u, wsoff = lane * (unsigned)args.ldws * 4u;
     // Slice kt into its ring slot; without ASYNC the slice that `stash` holds, and the next into it.
     [[maybe_unused]] u32x4 stash[LPW];
-    [[maybe_unused]] f32x4 sstash;
-    [[maybe_unused]] auto load_stash = [&](int kt) {
+    [[maybe_unused]] f32x4 xstash, wstash;
+    [[maybe_unused]] auto load_stash = [&](int kt) __attribute__((always_inline)) {
         typedef unsigned U4 __attribute__((ext_vector_type(4), aligned(1)));
 #pragma unroll
         for (int i = 0; i < LPW; i++) {
-            const int r = (wave * LPW + i) * RPI + lane / RC, k = kt * RB + chunk(i) * 16, rr = r < BN ? r : r - BN;
+            const int r = (i * NW + wave) * RPI + lane / RC - (i < LW ? 0 : BN), k = kt * RB + chunk(i) * 16;
             u32x4 v = {0u, 0u, 0u, 0u};
-            if (rr < (r < BN ? rows_n : rows_m) && k < a.K) {
-                const unsigned char* src = (r < BN ? W + (int64_t)rr * a.ldw : X + (int64_t)rr * a.ldx) + k;
+            if (r < (i < LW ? rows_n : rows_m) && k < a.K) {
+                const unsigned char* src = (i < LW ? W + r * a.ldw : X + r * a.ldx) + k;
                 if (k + 16 <= a.K) {
                     v = *reinterpret_cast<const U4*>(src);
                 } else {
@@ -194,34 +211,31 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
         }
         if (kt % PER == 0) {
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                sstash[e] = (int)threadIdx.x < rows_m && kt * WK + e < args.blocks ? XS[threadIdx.x * args.ldxs + kt * WK + e] : 0.f;
+            for (int e = 0; e < 4; e++) {
+                const bool there = kt * WK + e < args.blocks;
+                xstash[e] = there && (int)threadIdx.x < rows_m ? XS[threadIdx.x * args.ldxs + kt * WK + e] : 0.f;
+                wstash[e] = there && lane < wblocks ? WS[lane * args.ldws + kt * WK + e] : 0.f;
+            }
         }
     };
-    auto issue = [&](int kt) {
-        if (kt % PER == 0 && wave < SROWS / 64) {
-            float* dst = &xscale[kt / PER % SLOTS][64 * wave][0];
+    auto issue = [&](int kt) __attribute__((always_inline)) {
+        if (kt % PER == 0) {
+            const int slot = kt / PER % SLOTS;
             if constexpr (ASYNC) {
-                load_to_lds(rS, soff + kt * WK * 4u, 0, dst);
+                if (wave < SROWS / 64) load_to_lds(rXS, xsoff + kt * WK * 4u, lds_address(xscale) + (slot * SROWS + 64 * wave) * 16);
+                if (wave == NW - 1) load_to_lds(rWS, wsoff + kt * WK * 4u, lds_address(wscale) + slot * 64 * 16);
             } else {
-                *reinterpret_cast<f32x4*>(dst + 4 * lane) = sstash;
+                if (wave < SROWS / 64) *reinterpret_cast<f32x4*>(&xscale[slot][64 * wave + lane][0]) = xstash;
+                if (wave == NW - 1) *reinterpret_cast<f32x4*>(&wscale[slot][lane][0]) = wstash;
             }
         }
-        unsigned char* dst = smem + kt % STAGES * STAGE + wave * LPW * 1024;
+        const int dst = kt % STAGES * STAGE + wave * 1024;
         if constexpr (ASYNC) {
-            auto load = [&](int i, unsigned vo, unsigned so) {
-                load_to_lds((wave * LPW + i) * RPI < BN ? rW : rX, vo, so, dst + i * 1024);
-            };
-            if ((kt + 1) * RB <= a.K) {
 #pragma unroll
-                for (int i = 0; i < LPW; i++) load(i, voff[i], kt * RB);
-            } else {  // pieces past K read as zero, the offsets whole in the part that is checked against the window
-#pragma unroll
-                for (int i = 0; i < LPW; i++) load(i, kt * RB + chunk(i) * 16 < a.K ? voff[i] + (unsigned)kt * RB : 0x80000000u, 0);
-            }
+            for (int i = 0; i < LPW; i++) load_to_lds(i < LW ? rW : rX, offset(kt, i), lds_address(smem) + dst + i * NW * 1024);
         } else {
 #pragma unroll
-            for (int i = 0; i < LPW; i++) *reinterpret_cast<u32x4*>(dst + i * 1024 + 16 * lane) = stash[i];
+            for (int i = 0; i < LPW; i++) *reinterpret_cast<u32x4*>(smem + dst + i * NW * 1024 + 16 * lane) = stash[i];
             if (kt + 1 < nk) load_stash(kt + 1);
         }
     };
@@ -234,14 +248,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[j][i][e] = 0.f;
 
-    // Where K ends inside a 16-byte piece, its bytes past K in the last slice (they are the next row's) become zero.
-    [[maybe_unused]] auto cut_tail = [&](int kt) {
-        const int c = (a.K - kt * RB) / 16, left = a.K % 16;
-        for (int r = threadIdx.x; r < ROWS; r += 64 * NW) {
-            u32x4* piece = reinterpret_cast<u32x4*>(smem + kt % STAGES * STAGE + r * RB + (lswz<RB>(r < BN ? operand_row16<FN>(r) : r, c) << 4));
+    // Where K ends inside the last slice, what lies past it (the next rows' codes) becomes zero.
+    [[maybe_unused]] auto cut_tail = [&](int kt) __attribute__((always_inline)) {
+        int t = threadIdx.x, left = a.K - kt * RB;
+        asm volatile("" : "+v"(t), "+s"(left));  // (formed here, not kept in registers through the loop)
+        for (int p = t; p < ROWS * RC; p += 64 * NW) {
+            const int r = p / RC, k = 16 * (p % RC);
+            if (k + 16 <= left) continue;
+            u32x4* piece = reinterpret_cast<u32x4*>(smem + kt % STAGES * STAGE + r * RB + (lswz<RB>(r < BN ? operand_row16<FN>(r) : r, p % RC) << 4));
             u32x4 v = *piece;
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = cut_dword(v[e], 4 * e, left);
+            for (int e = 0; e < 4; e++) v[e] = cut_dword(v[e], k + 4 * e, left);
             *piece = v;
         }
         wait_lds();
@@ -249,110 +266,140 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
     };
     // Slice kt is there for every wave, and every wave has read the ones before it: of the later slices that were issued, `ahead` at most
     // may be on their way.
-    auto arrive = [&](int kt, auto ahead) {
+    auto arrive = [&](int kt, auto ahead) __attribute__((always_inline)) {
         constexpr int A = decltype(ahead)::value;
         if constexpr (ASYNC) wait_slices<A, LPW>(nk - 1 - kt < A ? nk - 1 - kt : A);
         wait_lds();
         raw_barrier();
         if constexpr (ASYNC) {
-            if (kt == nk - 1 && a.K % 16) cut_tail(kt);
+            if (kt == nk - 1 && a.K % RB) cut_tail(kt);
         }
     };
-    auto read_w = [&](int kt, int i) { return read_codes<RB>(smem + kt % STAGES * STAGE + (wn * TN + w_row16<FN>(i, fr)) * RB, fr, wk, fg); };
-    auto read_x = [&](int kt, int j) { return read_codes<RB>(smem + kt % STAGES * STAGE + (BN + wm * TM + 16 * j + fr) * RB, fr, wk, fg); };
-    // Of blocks past K, which a slice of several may have, X's scale is 0 (what is read for them is anything) and W's that of the first.
-    auto within = [&](int kt) { return WK == 1 || kt * WK + wk < args.blocks ? ~0u : 0u; };
-    auto read_scale = [&](int kt, int j) {
-        const float s = xscale[kt / PER % SLOTS][wm * TM + 16 * j + fr][(kt * WK + wk) % 4];
-        return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, s) & within(kt));
+    // Where a lane's fragments lie in a slot: of W's block 0 and X's block 0, the others a constant further.
+    const Pieces w_at = pieces_of<RB>(lds_address(smem) + (wn * TN + w_row16<FN>(0, fr)) * RB, fr, wk, fg);
+    const Pieces x_at = pieces_of<RB>(lds_address(smem) + (BN + wm * TM + fr) * RB, fr, wk, fg);
+    const unsigned xs_at = lds_address(xscale) + (wm * TM + fr) * 16, ws_at = lds_address(wscale) + wblock * 16;
+    struct Place {  // of a slice
+        Pieces w, x;
+        unsigned xs, ws;
+        bool there;  // the wave's block is within K (a slice of several may end past it)
     };
-    auto w_scale = [&](int kt) { return ws[within(kt) ? kt * WK + wk : 0]; };
-    // A product's sums are joined behind the next product, under its cycles.
-    f32x4 pending;
-    float pending_f = 0.f;
-    auto join = [&](int j, int i) {
+    auto place = [&](int kt) __attribute__((always_inline)) {
+        const unsigned slot = kt % STAGES * STAGE, scales = kt / PER % SLOTS, b = (kt * WK + wk) % 4 * 4;
+        Place p{{w_at.lo + slot, w_at.hi + slot}, {x_at.lo + slot, x_at.hi + slot}, xs_at + scales * (SROWS * 16) + b, ws_at + scales * 1024 + b,
+                WK == 1 || kt * WK + wk < args.blocks};
+        asm volatile("" : "+v"(p.w.lo), "+v"(p.w.hi), "+v"(p.x.lo), "+v"(p.x.hi), "+v"(p.xs), "+v"(p.ws));  // (each read a constant further)
+        return p;
+    };
+    auto read_w = [&](const Place& p, int i) __attribute__((always_inline)) { return read_codes(p.w, 4 * i * RB); };
+    auto read_x = [&](const Place& p, int j) __attribute__((always_inline)) { return read_codes(p.x, 16 * j * RB); };
+    // The scales of rows 16 j + fr and of the wave's columns; past K both 0 (what is read there is anything).
+    auto read_scales = [&](const Place& p, int j, float& x, float& w) __attribute__((always_inline)) {
+        typedef const __attribute__((address_space(3))) float* float_ptr;
+        x = *(float_ptr)((lds_ptr)(uintptr_t)p.xs + 16 * 16 * j);
+        w = *(float_ptr)((lds_ptr)(uintptr_t)p.ws);
+        if (WK > 1) x = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & (p.there ? ~0u : 0u));
+        if (WK > 1) w = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, w) & (p.there ? ~0u : 0u));
+    };
+    // A product's sums are joined two products later, under their cycles (the last two of a slice by the next one).
+    f32x4 pending[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    float pending_f[2] = {0.f, 0.f};
+    constexpr int PRODUCTS = FM * FN;
+    static_assert(PRODUCTS % 2 == 0, "the pending two");
+    auto join = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[j][i][e] = fmaf(pending[e], pending_f, acc[j][i][e]);
+        for (int e = 0; e < 4; e++) acc[t / FN][t % FN][e] = fmaf(pending[t & 1][e], pending_f[t & 1], acc[t / FN][t % FN][e]);
+        asm volatile("" : "+v"(acc[t / FN][t % FN]));  // here, not where the compiler would gather them
     };
-    auto multiply = [&](const Operand<EXACT>& w, const Operand<EXACT>& x, float f, int j, int i) {
+    auto multiply = [&](const Operand<EXACT>& w, const Operand<EXACT>& x, float f, int t) __attribute__((always_inline)) {
         const f32x4 p = product(w, x);
         if constexpr (!EXACT) __builtin_amdgcn_sched_barrier(0);
-        if (j > 0 || i > 0) join(i > 0 ? j : j - 1, i > 0 ? i - 1 : FN - 1);
-        pending = p;
-        pending_f = f;
-        if (j == FM - 1 && i == FN - 1) join(j, i);
+        join((t + PRODUCTS - 2) % PRODUCTS);
+        pending[t & 1] = p;
+        pending_f[t & 1] = f;
         if constexpr (!EXACT) __builtin_amdgcn_sched_barrier(0);
     };
     // Two ways through a slice.  AHEAD: the fragments of the next one are read under this one's products, from two sets, and the slot
     // that every wave has read is filled again before the products: STAGES slices of lookahead.  Otherwise, where two sets are too
-    // many registers, W's fragments are held, X's come one block of 16 rows ahead: STAGES - 1 slices.
-    [[maybe_unused]] i32x8 cw[AHEAD ? 2 : 1][FN], cx[AHEAD ? 2 : 1][FM];
-    [[maybe_unused]] float sx[2][FM], sw[2];
-    [[maybe_unused]] auto read_slice = [&](int kt, auto set) {
-        sw[set] = w_scale(kt);
+    // many registers, W's fragments have two sets and X's come one block of 16 rows ahead; the slot is filled again, and the next slice's first
+    // fragments are read, under the products of the last 16 rows.
+    Operand<EXACT> w[AHEAD ? 1 : 2][FN], x[2];
+    [[maybe_unused]] i32x8 cw[2][AHEAD ? FN : 1], cx[2][AHEAD ? FM : 1];
+    float sx[2][AHEAD ? FM : 1], sw[2];
+    Place at;
+    [[maybe_unused]] auto read_slice = [&](int kt, auto set) __attribute__((always_inline)) {
+        at = place(kt);
 #pragma unroll
-        for (int i = 0; i < FN; i++) cw[set][i] = read_w(kt, i);
+        for (int i = 0; i < FN; i++) cw[set][i] = read_w(at, i);
 #pragma unroll
         for (int j = 0; j < FM; j++) {
-            cx[set][j] = read_x(kt, j);
-            sx[set][j] = read_scale(kt, j);
+            cx[set][j] = read_x(at, j);
+            read_scales(at, j, sx[set][j], sw[set]);
         }
     };
-    [[maybe_unused]] auto slice_ahead = [&](int kt, auto cur) {
-        if (kt + 1 < nk) {
-            arrive(kt + 1, std::integral_constant<int, STAGES - 2>{});
-            read_slice(kt + 1, std::integral_constant<int, 1 - decltype(cur)::value>{});
-            if (kt + STAGES < nk) issue(kt + STAGES);
-        }
-        Operand<EXACT> w[FN];
+    // (After the last slice the reads are of whatever the slot holds, which no product takes: no branch around registers.)
+    [[maybe_unused]] auto slice_ahead = [&](int kt, auto cur) __attribute__((always_inline)) {
+        if (kt + 1 < nk) arrive(kt + 1, std::integral_constant<int, STAGES - 2>{});
+        read_slice(kt + 1, std::integral_constant<int, 1 - decltype(cur)::value>{});
+        if (kt + STAGES < nk) issue(kt + STAGES);
 #pragma unroll
-        for (int i = 0; i < FN; i++) w[i].set(cw[cur][i]);
+        for (int i = 0; i < FN; i++) w[0][i].set(cw[cur][i]);
 #pragma unroll
         for (int j = 0; j < FM; j++) {
-            Operand<EXACT> x;
-            x.set(cx[cur][j]);
+            x[j & 1].set(cx[cur][j]);
             const float f = sx[cur][j] * sw[cur];
 #pragma unroll
-            for (int i = 0; i < FN; i++) multiply(w[i], x, f, j, i);
+            for (int i = 0; i < FN; i++) multiply(w[0][i], x[j & 1], f, j * FN + i);
         }
     };
-    [[maybe_unused]] auto slice_held = [&](int kt) {
-        arrive(kt, std::integral_constant<int, STAGES - 2>{});
-        if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1);
-        const float ws = w_scale(kt);
-        Operand<EXACT> w[FN], x[2];
-        float f[2];
-        auto next_x = [&](int j) {
-            x[j & 1].set(read_x(kt, j));
-            f[j & 1] = read_scale(kt, j) * ws;
-        };
-#pragma unroll
-        for (int i = 0; i < FN; i++) w[i].set(read_w(kt, i));
+    [[maybe_unused]] auto next_x = [&](int j) __attribute__((always_inline)) {
+        x[j & 1].set(read_x(at, j));
+        read_scales(at, j, sx[j & 1][0], sw[j & 1]);
+    };
+    [[maybe_unused]] auto first_fragments = [&](int kt, auto set) __attribute__((always_inline)) {
+        at = place(kt);
         next_x(0);
 #pragma unroll
-        for (int j = 0; j < FM; j++) {
-            if (j + 1 < FM) next_x(j + 1);
+        for (int i = 0; i < FN; i++) w[set][i].set(read_w(at, i));
+    };
+    [[maybe_unused]] auto slice_held = [&](int kt, auto cur) __attribute__((always_inline)) {
+        static_assert(AHEAD || FM % 2 == 0, "the next slice's first rows take the other set");
 #pragma unroll
-            for (int i = 0; i < FN; i++) multiply(w[i], x[j & 1], f[j & 1], j, i);
+        for (int j = 0; j < FM; j++) {
+            const float f = sx[j & 1][0] * sw[j & 1];
+            if (j + 1 < FM) {
+                next_x(j + 1);
+            } else {
+                if (kt + 1 < nk) arrive(kt + 1, std::integral_constant<int, STAGES - 2>{});
+                if (kt + STAGES < nk) issue(kt + STAGES);
+                first_fragments(kt + 1, std::integral_constant<int, 1 - decltype(cur)::value>{});
+            }
+#pragma unroll
+            for (int i = 0; i < FN; i++) multiply(w[cur][i], x[j & 1], f, j * FN + i);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     if constexpr (!ASYNC) load_stash(0);
 #pragma unroll
-    for (int s = 0; s < (AHEAD ? STAGES : STAGES - 1); s++)
+    for (int s = 0; s < STAGES; s++)
         if (s < nk) issue(s);
-    if constexpr (AHEAD) {
-        constexpr std::integral_constant<int, 0> zero;
-        constexpr std::integral_constant<int, 1> one;
-        arrive(0, std::integral_constant<int, STAGES - 1>{});
-        read_slice(0, zero);
-        for (int kt = 0; kt < nk; kt += 2) {
-            slice_ahead(kt, zero);
-            if (kt + 1 < nk) slice_ahead(kt + 1, one);
-        }
-    } else {
-        for (int kt = 0; kt < nk; kt++) slice_held(kt);
+    constexpr std::integral_constant<int, 0> zero;
+    constexpr std::integral_constant<int, 1> one;
+    arrive(0, std::integral_constant<int, STAGES - 1>{});
+    if constexpr (AHEAD) read_slice(0, zero);
+    else first_fragments(0, zero);
+    auto slice = [&](int kt, auto cur) __attribute__((always_inline)) {
+        if constexpr (AHEAD) slice_ahead(kt, cur);
+        else slice_held(kt, cur);
+    };
+    int kt = 0;
+    for (; kt + 1 < nk; kt += 2) {
+        slice(kt, zero);
+        slice(kt + 1, one);
     }
+    if (kt < nk) slice(kt, zero);
+    join(PRODUCTS - 2);
+    join(PRODUCTS - 1);
 
     // The k groups' sums, added in their order.
     if constexpr (WK > 1) {
@@ -502,7 +549,7 @@ int launch_linear_fp8(const LinearFp8Args& a, hipStream_t st, bool go) {
     // The buffer-to-LDS loads take dword-aligned rows, and windows of a tile's rows below 2^31 bytes.
     constexpr int64_t FAR = (int64_t)1 << 22;
     const bool async = !((reinterpret_cast<uintptr_t>(l.x) | reinterpret_cast<uintptr_t>(l.w) | l.ldx | l.ldw) & 3) && l.ldx <= FAR &&
-                       l.ldw <= FAR && l.K <= FAR && a.ldxs * 4 <= FAR;
+                       l.ldw <= FAR && l.K <= FAR && a.ldxs * 4 <= FAR && a.ldws * 4 <= FAR;
     if (!async) return launch_tiles<TO, 128, 128, 4, 2, 1, 2, false, true, 2>(a, st, go);
     if ((int64_t)((l.M + 127) / 128) * ((l.N + 127) / 128) < 256) return launch_tiles<TO, 64, 64, 2, 2, 2, 2, true, true, 2>(a, st, go);
     return launch_tiles<TO, 128, 128, 4, 2, 1, 2, true, true, 2>(a, st, go);
