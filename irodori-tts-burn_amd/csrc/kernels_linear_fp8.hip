@@ -140,23 +140,36 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
     __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * STAGE];
     __shared__ __attribute__((aligned(1024))) float xscale[SLOTS][SROWS][4], wscale[SLOTS][64][4];
 
+    __shared__ __attribute__((aligned(1024))) u32x4 turned[AHEAD ? 1 : NW][128];  // 16 rows of Y on their way out
+
     const int lane = threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wk = wave / (WM * WN), wmn = wave % (WM * WN), wm = wmn / WN, wn = wmn % WN;
-    // Groups of 8 row tiles sweep the column tiles, an XCD's workgroups consecutive.
-    const int pid = xcd_remap(blockIdx.x, gridDim.x);
-    const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN;
-    const int group = pid / (8 * tiles_n), first = group * 8;
-    const int gm = tiles_m - first < 8 ? tiles_m - first : 8, local = pid - group * 8 * tiles_n;
-    const int m0 = (first + local % gm) * BM, n0 = (local / gm) * BN;
-    const int rows_m = a.M - m0 < BM ? a.M - m0 : BM, rows_n = a.N - n0 < BN ? a.N - n0 : BN;
-    const unsigned char* X = static_cast<const unsigned char*>(a.x) + (int64_t)m0 * a.ldx;
-    const unsigned char* W = static_cast<const unsigned char*>(a.w) + (int64_t)n0 * a.ldw;
-    const float* XS = args.xs + (int64_t)m0 * args.ldxs;
-    // The wave's columns share their scales.
-    const int wblock = (n0 % kBlock + wn * TN) / kBlock, wblocks = (n0 % kBlock + rows_n + kBlock - 1) / kBlock;
-    const float* WS = args.ws + (int64_t)(n0 / kBlock) * args.ldws;
     const int nk = (args.blocks + WK - 1) / WK;
+    // Groups of 8 row tiles sweep the column tiles.  An XCD takes a run of neighbouring tiles: each of its workgroups one, or, where the
+    // launch has fewer workgroups than tiles, every stride-th of the run.
+    const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN;
+    struct Tile {
+        int m0, n0, rows_m, rows_n;
+    };
+    auto locate = [&](int pid) __attribute__((always_inline)) {
+        const int group = pid / (8 * tiles_n), first = group * 8;
+        const int gm = tiles_m - first < 8 ? tiles_m - first : 8, local = pid - group * 8 * tiles_n;
+        const int m0 = (first + local % gm) * BM, n0 = (local / gm) * BN;
+        return Tile{m0, n0, a.M - m0 < BM ? a.M - m0 : BM, a.N - n0 < BN ? a.N - n0 : BN};
+    };
+    int pid, last = 0, stride = 1;  // this workgroup's tiles: pid, pid + stride, .. below last
+    if (AHEAD || gridDim.x % 8) {
+        pid = xcd_remap(blockIdx.x, gridDim.x);
+    } else {
+        const int64_t tiles = (int64_t)tiles_m * tiles_n, xcd = blockIdx.x % 8;
+        stride = gridDim.x / 8;
+        pid = (int)(tiles * xcd / 8) + blockIdx.x / 8;
+        last = (int)(tiles * (xcd + 1) / 8);
+        if (pid >= last) return;
+    }
+    int now = pid;  // the tile that is multiplied; pid the one that is loaded
+    Tile tile = locate(now);
 
     // Load instruction i of this wave fills stage rows RPI (i NW + wave) .. (the first LW instructions W rows, the others X rows):
     // lane -> row lane / RC, physical chunk lane % RC, which holds the row's chunk `chunk`.
@@ -165,13 +178,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
         return lswz<RB>(i < LW ? operand_row16<FN>(r) : r, lane % RC);
     };
     [[maybe_unused]] Window rX, rW, rXS, rWS;
-    if constexpr (ASYNC) {
+    [[maybe_unused]] auto look_at = [&](const Tile& t) __attribute__((always_inline)) {  // the windows of a tile's operands
+        const int wblocks = (t.n0 % kBlock + t.rows_n + kBlock - 1) / kBlock;
         // Windows end with the last row's last whole dword (its other bytes are in the same memory word).
-        rX = make_window(X, ((unsigned)((int64_t)(rows_m - 1) * a.ldx + a.K) + 3) & ~3u);
-        rW = make_window(W, ((unsigned)((int64_t)(rows_n - 1) * a.ldw + a.K) + 3) & ~3u);
-        rXS = make_window(XS, (unsigned)((int64_t)(rows_m - 1) * args.ldxs + args.blocks) * 4u);
-        rWS = make_window(WS, (unsigned)((int64_t)(wblocks - 1) * args.ldws + args.blocks) * 4u);
-    }
+        rX = make_window(static_cast<const unsigned char*>(a.x) + (int64_t)t.m0 * a.ldx, ((unsigned)((int64_t)(t.rows_m - 1) * a.ldx + a.K) + 3) & ~3u);
+        rW = make_window(static_cast<const unsigned char*>(a.w) + (int64_t)t.n0 * a.ldw, ((unsigned)((int64_t)(t.rows_n - 1) * a.ldw + a.K) + 3) & ~3u);
+        rXS = make_window(args.xs + (int64_t)t.m0 * args.ldxs, (unsigned)((int64_t)(t.rows_m - 1) * args.ldxs + args.blocks) * 4u);
+        rWS = make_window(args.ws + (int64_t)(t.n0 / kBlock) * args.ldws, (unsigned)((int64_t)(wblocks - 1) * args.ldws + args.blocks) * 4u);
+    };
+    if constexpr (ASYNC) look_at(tile);
     // Where load instruction i of slice kt reads, whole in the part that is checked against the window.  Rows past the last lie behind it
     // and read as zero, as do pieces of its last row past K (with rows closer than K apart they hold codes, which none of Y's sees).
     constexpr int STEP = NW * RPI;  // rows from one instruction of a wave to the next
@@ -192,12 +207,16 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
     [[maybe_unused]] u32x4 stash[LPW];
     [[maybe_unused]] f32x4 xstash, wstash;
     [[maybe_unused]] auto load_stash = [&](int kt) __attribute__((always_inline)) {
+        const unsigned char* X = static_cast<const unsigned char*>(a.x) + (int64_t)tile.m0 * a.ldx;
+        const unsigned char* W = static_cast<const unsigned char*>(a.w) + (int64_t)tile.n0 * a.ldw;
+        const float *XS = args.xs + (int64_t)tile.m0 * args.ldxs, *WS = args.ws + (int64_t)(tile.n0 / kBlock) * args.ldws;
+        const int wblocks = (tile.n0 % kBlock + tile.rows_n + kBlock - 1) / kBlock;
         typedef unsigned U4 __attribute__((ext_vector_type(4), aligned(1)));
 #pragma unroll
         for (int i = 0; i < LPW; i++) {
             const int r = (i * NW + wave) * RPI + lane / RC - (i < LW ? 0 : BN), k = kt * RB + chunk(i) * 16;
             u32x4 v = {0u, 0u, 0u, 0u};
-            if (r < (i < LW ? rows_n : rows_m) && k < a.K) {
+            if (r < (i < LW ? tile.rows_n : tile.rows_m) && k < a.K) {
                 const unsigned char* src = (i < LW ? W + r * a.ldw : X + r * a.ldx) + k;
                 if (k + 16 <= a.K) {
                     v = *reinterpret_cast<const U4*>(src);
@@ -213,14 +232,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const bool there = kt * WK + e < args.blocks;
-                xstash[e] = there && (int)threadIdx.x < rows_m ? XS[threadIdx.x * args.ldxs + kt * WK + e] : 0.f;
+                xstash[e] = there && (int)threadIdx.x < tile.rows_m ? XS[threadIdx.x * args.ldxs + kt * WK + e] : 0.f;
                 wstash[e] = there && lane < wblocks ? WS[lane * args.ldws + kt * WK + e] : 0.f;
             }
         }
     };
-    auto issue = [&](int kt) __attribute__((always_inline)) {
+    // (ring, scales: the numbers of the slices and of the loads of scales so far.)
+    auto issue = [&](int kt, int ring, int scales) __attribute__((always_inline)) {
         if (kt % PER == 0) {
-            const int slot = kt / PER % SLOTS;
+            const int slot = scales % SLOTS;
             if constexpr (ASYNC) {
                 if (wave < SROWS / 64) load_to_lds(rXS, xsoff + kt * WK * 4u, lds_address(xscale) + (slot * SROWS + 64 * wave) * 16);
                 if (wave == NW - 1) load_to_lds(rWS, wsoff + kt * WK * 4u, lds_address(wscale) + slot * 64 * 16);
@@ -229,7 +249,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
                 if (wave == NW - 1) *reinterpret_cast<f32x4*>(&wscale[slot][lane][0]) = wstash;
             }
         }
-        const int dst = kt % STAGES * STAGE + wave * 1024;
+        const int dst = ring % STAGES * STAGE + wave * 1024;
         if constexpr (ASYNC) {
 #pragma unroll
             for (int i = 0; i < LPW; i++) load_to_lds(i < LW ? rW : rX, offset(kt, i), lds_address(smem) + dst + i * NW * 1024);
@@ -249,13 +269,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
             for (int e = 0; e < 4; e++) acc[j][i][e] = 0.f;
 
     // Where K ends inside the last slice, what lies past it (the next rows' codes) becomes zero.
-    [[maybe_unused]] auto cut_tail = [&](int kt) __attribute__((always_inline)) {
+    [[maybe_unused]] auto cut_tail = [&](int kt, int ring) __attribute__((always_inline)) {
         int t = threadIdx.x, left = a.K - kt * RB;
         asm volatile("" : "+v"(t), "+s"(left));  // (formed here, not kept in registers through the loop)
         for (int p = t; p < ROWS * RC; p += 64 * NW) {
             const int r = p / RC, k = 16 * (p % RC);
             if (k + 16 <= left) continue;
-            u32x4* piece = reinterpret_cast<u32x4*>(smem + kt % STAGES * STAGE + r * RB + (lswz<RB>(r < BN ? operand_row16<FN>(r) : r, p % RC) << 4));
+            u32x4* piece = reinterpret_cast<u32x4*>(smem + ring % STAGES * STAGE + r * RB + (lswz<RB>(r < BN ? operand_row16<FN>(r) : r, p % RC) << 4));
             u32x4 v = *piece;
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = cut_dword(v[e], k + 4 * e, left);
@@ -264,29 +284,36 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
         wait_lds();
         raw_barrier();
     };
-    // Slice kt is there for every wave, and every wave has read the ones before it: of the later slices that were issued, `ahead` at most
-    // may be on their way.
-    auto arrive = [&](int kt, auto ahead) __attribute__((always_inline)) {
+    // Slice kt is there for every wave, and every wave has read the ones before it: of the later slices that were issued, A at most may
+    // be on their way, and the stores of a tile that were issued after its loads (the counter keeps their order).
+    [[maybe_unused]] int stores = 0;
+    auto arrive = [&](int kt, int ring, auto ahead) __attribute__((always_inline)) {
         constexpr int A = decltype(ahead)::value;
-        if constexpr (ASYNC) wait_slices<A, LPW>(nk - 1 - kt < A ? nk - 1 - kt : A);
+        if constexpr (!AHEAD) {
+            if (stores) wait_vm<2 * FM>();
+            else wait_vm<0>();
+            stores = 0;
+        } else if constexpr (ASYNC) {
+            wait_slices<A, LPW>(nk - 1 - kt < A ? nk - 1 - kt : A);
+        }
         wait_lds();
         raw_barrier();
         if constexpr (ASYNC) {
-            if (kt == nk - 1 && a.K % RB) cut_tail(kt);
+            if (kt == nk - 1 && a.K % RB) cut_tail(kt, ring);
         }
     };
     // Where a lane's fragments lie in a slot: of W's block 0 and X's block 0, the others a constant further.
     const Pieces w_at = pieces_of<RB>(lds_address(smem) + (wn * TN + w_row16<FN>(0, fr)) * RB, fr, wk, fg);
     const Pieces x_at = pieces_of<RB>(lds_address(smem) + (BN + wm * TM + fr) * RB, fr, wk, fg);
-    const unsigned xs_at = lds_address(xscale) + (wm * TM + fr) * 16, ws_at = lds_address(wscale) + wblock * 16;
+    const unsigned xs_at = lds_address(xscale) + (wm * TM + fr) * 16, ws_at = lds_address(wscale) + wn * TN / kBlock * 16;  // (a wave's columns share a scale)
     struct Place {  // of a slice
         Pieces w, x;
         unsigned xs, ws;
         bool there;  // the wave's block is within K (a slice of several may end past it)
     };
-    auto place = [&](int kt) __attribute__((always_inline)) {
-        const unsigned slot = kt % STAGES * STAGE, scales = kt / PER % SLOTS, b = (kt * WK + wk) % 4 * 4;
-        Place p{{w_at.lo + slot, w_at.hi + slot}, {x_at.lo + slot, x_at.hi + slot}, xs_at + scales * (SROWS * 16) + b, ws_at + scales * 1024 + b,
+    auto place = [&](int kt, int ring, int scales) __attribute__((always_inline)) {
+        const unsigned slot = ring % STAGES * STAGE, from = scales % SLOTS, b = (kt * WK + wk) % 4 * 4;
+        Place p{{w_at.lo + slot, w_at.hi + slot}, {x_at.lo + slot, x_at.hi + slot}, xs_at + from * (SROWS * 16) + b, ws_at + from * 1024 + b,
                 WK == 1 || kt * WK + wk < args.blocks};
         asm volatile("" : "+v"(p.w.lo), "+v"(p.w.hi), "+v"(p.x.lo), "+v"(p.x.hi), "+v"(p.xs), "+v"(p.ws));  // (each read a constant further)
         return p;
@@ -328,7 +355,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
     float sx[2][AHEAD ? FM : 1], sw[2];
     Place at;
     [[maybe_unused]] auto read_slice = [&](int kt, auto set) __attribute__((always_inline)) {
-        at = place(kt);
+        at = place(kt, kt, kt / PER);
 #pragma unroll
         for (int i = 0; i < FN; i++) cw[set][i] = read_w(at, i);
 #pragma unroll
@@ -339,9 +366,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
     };
     // (After the last slice the reads are of whatever the slot holds, which no product takes: no branch around registers.)
     [[maybe_unused]] auto slice_ahead = [&](int kt, auto cur) __attribute__((always_inline)) {
-        if (kt + 1 < nk) arrive(kt + 1, std::integral_constant<int, STAGES - 2>{});
+        if (kt + 1 < nk) arrive(kt + 1, kt + 1, std::integral_constant<int, STAGES - 2>{});
         read_slice(kt + 1, std::integral_constant<int, 1 - decltype(cur)::value>{});
-        if (kt + STAGES < nk) issue(kt + STAGES);
+        if (kt + STAGES < nk) issue(kt + STAGES, kt + STAGES, (kt + STAGES) / PER);
 #pragma unroll
         for (int i = 0; i < FN; i++) w[0][i].set(cw[cur][i]);
 #pragma unroll
@@ -356,51 +383,192 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
         x[j & 1].set(read_x(at, j));
         read_scales(at, j, sx[j & 1][0], sw[j & 1]);
     };
-    [[maybe_unused]] auto first_fragments = [&](int kt, auto set) __attribute__((always_inline)) {
-        at = place(kt);
+    // The slices of the tiles one after the other, as the loads are issued and as they are multiplied: slice kt of a tile is the ring-th.
+    struct Course {
+        int kt = 0, ring = 0, scales = 0;
+        __device__ __forceinline__ bool next(int nk) {  // true: a tile is done
+            ring++;
+            const bool done = ++kt == nk;
+            if (done) kt = 0;
+            if (kt % PER == 0) scales++;
+            return done;
+        }
+    };
+    Course loads, products;
+    bool more = true;  // tiles to load from
+    [[maybe_unused]] auto issue_next = [&]() __attribute__((always_inline)) {
+        if (!more) return;
+        issue(loads.kt, loads.ring, loads.scales);
+        if (loads.next(nk)) {
+            pid += stride;
+            more = pid < last;
+            if (more) look_at(locate(pid));
+        }
+    };
+    [[maybe_unused]] auto first_fragments = [&](auto set) __attribute__((always_inline)) {
+        at = place(products.kt, products.ring, products.scales);
         next_x(0);
 #pragma unroll
         for (int i = 0; i < FN; i++) w[set][i].set(read_w(at, i));
     };
-    [[maybe_unused]] auto slice_held = [&](int kt, auto cur) __attribute__((always_inline)) {
-        static_assert(AHEAD || FM % 2 == 0, "the next slice's first rows take the other set");
+    [[maybe_unused]] auto slice_held = [&](auto cur) __attribute__((always_inline)) {
+        static_assert(AHEAD || (ASYNC && FM % 2 == 0 && STAGES == 2 && WK == 1), "the next slice's first rows take the other set; one slice on its way");
 #pragma unroll
         for (int j = 0; j < FM; j++) {
             const float f = sx[j & 1][0] * sw[j & 1];
             if (j + 1 < FM) {
                 next_x(j + 1);
             } else {
-                if (kt + 1 < nk) arrive(kt + 1, std::integral_constant<int, STAGES - 2>{});
-                if (kt + STAGES < nk) issue(kt + STAGES);
-                first_fragments(kt + 1, std::integral_constant<int, 1 - decltype(cur)::value>{});
+                products.next(nk);
+                arrive(products.kt, products.ring, std::integral_constant<int, 0>{});
+                issue_next();
+                first_fragments(std::integral_constant<int, 1 - decltype(cur)::value>{});
             }
 #pragma unroll
             for (int i = 0; i < FN; i++) multiply(w[cur][i], x[j & 1], f, j * FN + i);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    if constexpr (!ASYNC) load_stash(0);
-#pragma unroll
-    for (int s = 0; s < STAGES; s++)
-        if (s < nk) issue(s);
     constexpr std::integral_constant<int, 0> zero;
     constexpr std::integral_constant<int, 1> one;
-    arrive(0, std::integral_constant<int, STAGES - 1>{});
-    if constexpr (AHEAD) read_slice(0, zero);
-    else first_fragments(0, zero);
+    if constexpr (!ASYNC) load_stash(0);
+    if constexpr (AHEAD) {
+#pragma unroll
+        for (int s = 0; s < STAGES; s++)
+            if (s < nk) issue(s, s, s / PER);
+        arrive(0, 0, std::integral_constant<int, STAGES - 1>{});
+        read_slice(0, zero);
+    } else {
+        issue_next();
+        arrive(0, 0, std::integral_constant<int, 0>{});
+        issue_next();
+        first_fragments(zero);
+    }
     auto slice = [&](int kt, auto cur) __attribute__((always_inline)) {
         if constexpr (AHEAD) slice_ahead(kt, cur);
-        else slice_held(kt, cur);
+        else slice_held(cur);
     };
-    int kt = 0;
-    for (; kt + 1 < nk; kt += 2) {
-        slice(kt, zero);
-        slice(kt + 1, one);
+    auto all_slices = [&]() __attribute__((always_inline)) {
+        int kt = 0;
+        for (; kt + 1 < nk; kt += 2) {
+            slice(kt, zero);
+            slice(kt + 1, one);
+        }
+        if (kt < nk) {
+            slice(kt, zero);
+            if constexpr (!AHEAD) {
+#pragma unroll
+                for (int i = 0; i < FN; i++) w[0][i] = w[1][i];  // the next tile's
+            }
+        }
+        join(PRODUCTS - 2);
+        join(PRODUCTS - 1);
+    };
+    // Lane (fr, fg) has of row m0 + wm TM + 16 j + fr the columns from n0 + wn TN + C fg on.
+    // A tile inside Y (16-bit outputs): a wave turns 16 rows of 64 columns in LDS, so that 8 neighbouring lanes store a row's 128 bytes.
+    // The wave's LDS operations keep their order, so nothing waits but the stores; addresses are a uniform one and a lane's offset.
+    [[maybe_unused]] auto finish_inner = [&](auto plain, auto past) __attribute__((always_inline)) {
+        constexpr int E = kPiece<TO>, Q = kLanes<TO, C>;
+        typedef TO OE __attribute__((ext_vector_type(E), aligned(sizeof(TO))));
+        static_assert(AHEAD || (C == 16 && E == 8), "16 columns a lane, in two pieces");
+        u32x4* stage = turned[wave];
+        auto at = [&](int row, int c) __attribute__((always_inline)) { return row * 8 + (c ^ (row >> 1 & 7)); };  // piece c of a row
+        const int n = tile.n0 + wn * TN, row = lane >> 3;
+        const unsigned out = (row * (unsigned)a.ldy + (lane & 7) * E) * (unsigned)sizeof(TO);
+#pragma unroll
+        for (int j = 0; j < FM; j++) {
+            const int m = tile.m0 + wm * TM + 16 * j;
+            float v[C];
+#pragma unroll
+            for (int e = 0; e < C; e++) v[e] = acc[j][e / 4][e % 4];
+            if constexpr (!decltype(plain)::value) {
+                if (a.bias) {
+                    float f[C];
+                    load_cols(a.bias + n + C * fg, C, f);
+#pragma unroll
+                    for (int e = 0; e < C; e++) v[e] += f[e];
+                }
+                activate<TO>(v, a.act);
+                if (a.gate) {
+                    float f[C];
+                    load_cols(a.gate + (int64_t)((m + fr) / a.gate_rows) * a.N + n + C * fg, C, f);
+#pragma unroll
+                    for (int e = 0; e < C; e++) v[e] *= f[e];
+                }
+                if (a.residual) {
+                    u32x4 p[Q];
+                    const int t = lane & (Q - 1);
+                    load_pieces<TO, true>(a, m + fr - t, n + C * fg + t * E, p);
+                    exchange(p, lane);
+#pragma unroll
+                    for (int s = 0; s < Q; s++) {
+                        const OE o = __builtin_bit_cast(OE, p[s]);
+#pragma unroll
+                        for (int e = 0; e < E; e++) v[s * E + e] += static_cast<float>(o[e]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                OE o;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] = static_cast<TO>(v[s * E + e]);
+                stage[at(fr, 2 * fg + s)] = __builtin_bit_cast(u32x4, o);
+            }
+            char* y = static_cast<char*>(a.y) + ((int64_t)m * a.ldy + n) * (int64_t)sizeof(TO);
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                OE* to = reinterpret_cast<OE*>(y + (int64_t)(8 * s) * a.ldy * (int64_t)sizeof(TO) + out);
+                const OE o = __builtin_bit_cast(OE, stage[at(8 * s + row, lane & 7)]);
+                if constexpr (decltype(past)::value) {
+                    __builtin_nontemporal_store(o, to);
+                    asm volatile("");  // (else the compiler takes this code and the other's for the same)
+                } else {
+                    *to = o;
+                }
+            }
+        }
+    };
+    auto finish_tile = [&]() __attribute__((always_inline)) {
+        auto all = [&](auto whole) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < FM; j++) {
+                float v[C];
+#pragma unroll
+                for (int e = 0; e < C; e++) v[e] = acc[j][e / 4][e % 4];
+                finish_block<TO, decltype(whole)::value>(a, tile.m0 + wm * TM + 16 * j + fr, tile.n0 + wn * TN + C * fg, lane, v);
+            }
+        };
+        if constexpr (!AHEAD) {
+            stores = tile.rows_m == BM && tile.rows_n == BN ? 2 * FM : 0;
+            if (stores == 0) all(std::false_type{});
+            else if (a.bias || a.act != IRODORI_ACT_NONE || a.gate || a.residual) finish_inner(std::false_type{}, std::true_type{});
+            // A Y that the L2s (32 MB) do not hold goes past them: 24000 x 5632 x 1024 154 against 163 us, x 512 92 against 103.
+            else if ((int64_t)a.M * a.N * (int64_t)sizeof(TO) > (32 << 20)) finish_inner(std::true_type{}, std::true_type{});
+            else finish_inner(std::true_type{}, std::false_type{});
+        } else {
+            if (tile.rows_n == BN) all(std::true_type{});
+            else all(std::false_type{});
+        }
+    };
+    if constexpr (!AHEAD) {
+        for (;;) {
+            all_slices();
+            finish_tile();  // the next tile's first slices are on their way
+            now += stride;
+            if (now >= last) return;
+            tile = locate(now);
+#pragma unroll
+            for (int t = 0; t < PRODUCTS; t++) acc[t / FN][t % FN] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                pending[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                pending_f[i] = 0.f;
+            }
+        }
     }
-    if (kt < nk) slice(kt, zero);
-    join(PRODUCTS - 2);
-    join(PRODUCTS - 1);
 
+    all_slices();
     // The k groups' sums, added in their order.
     if constexpr (WK > 1) {
         __syncthreads();
@@ -423,18 +591,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
     }
     if (WK > 1 && wk > 0) return;
 
-    // Lane (fr, fg) has of row m0 + wm TM + 16 j + fr the columns from n0 + wn TN + C fg on.
-    auto finish_all = [&](auto whole) {
-#pragma unroll
-        for (int j = 0; j < FM; j++) {
-            float v[C];
-#pragma unroll
-            for (int e = 0; e < C; e++) v[e] = acc[j][e / 4][e % 4];
-            finish_block<TO, decltype(whole)::value>(a, m0 + wm * TM + 16 * j + fr, n0 + wn * TN + C * fg, lane, v);
-        }
-    };
-    if (rows_n == BN) finish_all(std::true_type{});
-    else finish_all(std::false_type{});
+    finish_tile();
 }
 
 // ---- few rows ---------------------------------------------------------------------------------
@@ -531,13 +688,48 @@ int launch_rows(const LinearFp8Args& a, hipStream_t st, bool go) {
     return 0;
 }
 
+constexpr int kResident = 256;  // workgroups of the large tiles: one a CU
 template <typename TO, int BM, int BN, int WM, int WN, int WK, int STAGES, bool ASYNC, bool AHEAD, int EU>
 int launch_tiles(const LinearFp8Args& a, hipStream_t st, bool go) {
     constexpr int THREADS = 64 * WM * WN * WK;
-    const int64_t wgs = (int64_t)((a.l.M + BM - 1) / BM) * ((a.l.N + BN - 1) / BN);
-    if (wgs * THREADS > UINT32_MAX) return -1;
+    const int64_t tiles = (int64_t)((a.l.M + BM - 1) / BM) * ((a.l.N + BN - 1) / BN);
+    if (tiles * THREADS > UINT32_MAX) return -1;
+    const int64_t wgs = AHEAD || tiles < kResident ? tiles : kResident;
     if (go) linear_fp8_kernel<TO, BM, BN, WM, WN, WK, STAGES, ASYNC, AHEAD, EU><<<(unsigned)wgs, THREADS, 0, st>>>(a);
     return 0;
+}
+
+// The tiles a launch takes: of these, the one whose busiest CU is done first, by the microseconds of a tile (f + a a block of K) fitted to
+// all tiles' times at 110 sizes (16-bit outputs) and 80 (f32): M from 17 to 30 000, N from 64 to 7360, K from 128 to 3680.  The choice
+// loses 0.7 % (0.9 %) on the best of them on average; over 10 % at two sizes (one), 26 % at 225 x 2048 x 2048 (9.0 against 7.1 us).
+// Tiles that share a CU overlap where they wait (rounds count in parts).  E.g. in bf16 with 64 x 64 / 128 x 128 / 128 x 256 / 192 x 256 /
+// 256 x 256 tiles: 1500 x 1024 x 2816 12.4 / 19.5 / 24.3 / 32.0 / 39.6 us, 3000 x 5632 x 1024 45 / 38 / 31 / 30 / 40, 12000 x 1280 x 2816
+// 84 / 79 / 53 / 63 / 50, 24000 x 5632 x 1024 327 / 253 / 177 / 156 / 159, 8192^3 934 / 987 / 618 / 550 / 482.
+struct TileCost {
+    int bm, bn;
+    float f, a;
+    int parts;
+    float alone;
+};
+constexpr TileCost kTiles16[] = {{32, 32, 0.634f, 0.0974f, 4, 1.f},  {64, 64, 0.67f, 0.182f, 1, 1.08f},   {128, 128, 1.27f, 0.5475f, 1, 0.8f},
+                                 {128, 256, 1.02f, 1.007f, 1, 1.f},  {192, 256, 1.62f, 1.3445f, 1, 1.f}, {256, 256, 3.45f, 1.67f, 1, 1.f}};
+constexpr TileCost kTiles32[] = {{32, 32, 1.09f, 0.1005f, 4, 1.f}, {64, 64, 1.13f, 0.2566f, 1, 1.f}, {64, 128, 2.37f, 0.4985f, 1, 1.f},
+                                 {128, 128, 1.62f, 0.968f, 1, 1.f}};
+template <int N>
+int best_tiles(const TileCost (&t)[N], const LinearFp8Args& a) {
+    constexpr int CUS = 256;
+    int best = 0;
+    double least = 0.;
+    for (int i = 0; i < N; i++) {
+        const int64_t n = ((int64_t)(a.l.M + t[i].bm - 1) / t[i].bm) * ((a.l.N + t[i].bn - 1) / t[i].bn);
+        const double rounds = n <= CUS ? t[i].alone : (double)((n * t[i].parts + CUS - 1) / CUS) / t[i].parts;
+        const double c = rounds * (t[i].f + (double)t[i].a * a.blocks);
+        if (i == 0 || c < least) {
+            least = c;
+            best = i;
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -549,10 +741,30 @@ int launch_linear_fp8(const LinearFp8Args& a, hipStream_t st, bool go) {
     // The buffer-to-LDS loads take dword-aligned rows, and windows of a tile's rows below 2^31 bytes.
     constexpr int64_t FAR = (int64_t)1 << 22;
     const bool async = !((reinterpret_cast<uintptr_t>(l.x) | reinterpret_cast<uintptr_t>(l.w) | l.ldx | l.ldw) & 3) && l.ldx <= FAR &&
-                       l.ldw <= FAR && l.K <= FAR && a.ldxs * 4 <= FAR && a.ldws * 4 <= FAR;
-    if (!async) return launch_tiles<TO, 128, 128, 4, 2, 1, 2, false, true, 2>(a, st, go);
-    if ((int64_t)((l.M + 127) / 128) * ((l.N + 127) / 128) < 256) return launch_tiles<TO, 64, 64, 2, 2, 2, 2, true, true, 2>(a, st, go);
-    return launch_tiles<TO, 128, 128, 4, 2, 1, 2, true, true, 2>(a, st, go);
+                       l.ldw <= FAR && l.K <= FAR && a.ldxs * 4 <= FAR && a.ldws * 4 <= FAR && l.ldy <= FAR && l.ldr <= FAR;
+    if (!async) {
+        // Through registers: 64 x 64 against 128 x 128 tiles 11.3 / 15.4 us at 500 x 1024 x 1001 (128 tiles of 64), 33.7 / 16.1 at 1536 x 2048
+        // (768), 1115 / 422 at 20000 x 5632: the smaller ones while they all run at once.
+        if (((int64_t)l.M + 63) / 64 * ((l.N + 63) / 64) <= 256) return launch_tiles<TO, 64, 64, 2, 2, 2, 2, false, true, 2>(a, st, go);
+        return launch_tiles<TO, 128, 128, 4, 2, 1, 2, false, true, 2>(a, st, go);
+    }
+    if constexpr (sizeof(TO) == 4) {
+        switch (best_tiles(kTiles32, a)) {
+            case 0: return launch_tiles<TO, 32, 32, 1, 1, 4, 2, true, true, 2>(a, st, go);
+            case 1: return launch_tiles<TO, 64, 64, 1, 2, 2, 2, true, true, 2>(a, st, go);
+            case 2: return launch_tiles<TO, 64, 128, 2, 2, 2, 2, true, true, 2>(a, st, go);
+            default: return launch_tiles<TO, 128, 128, 4, 2, 1, 2, true, true, 2>(a, st, go);
+        }
+    } else {
+        switch (best_tiles(kTiles16, a)) {
+            case 0: return launch_tiles<TO, 32, 32, 1, 1, 4, 2, true, true, 2>(a, st, go);
+            case 1: return launch_tiles<TO, 64, 64, 2, 2, 2, 2, true, true, 4>(a, st, go);
+            case 2: return launch_tiles<TO, 128, 128, 4, 2, 1, 2, true, true, 2>(a, st, go);
+            case 3: return launch_tiles<TO, 128, 256, 2, 4, 1, 2, true, false, 2>(a, st, go);
+            case 4: return launch_tiles<TO, 192, 256, 2, 4, 1, 2, true, false, 2>(a, st, go);
+            default: return launch_tiles<TO, 256, 256, 2, 4, 1, 2, true, false, 2>(a, st, go);
+        }
+    }
 }
 
 template int launch_linear_fp8<bf16>(const LinearFp8Args&, hipStream_t, bool);
