@@ -90,7 +90,8 @@ __device__ __forceinline__ f32x4 product(const Operand<true>& a, const Operand<t
     return p;
 }
 // 16 bytes a lane from a buffer window to LDS at `to` (the same in every lane) and 16 times the lane.  By hand, since behind the
-// builtin the compiler lets every LDS read wait for all loads on their way; the waits are wait_vm's.
+// builtin the compiler lets every LDS read wait for all loads on their way; the waits are wait_vm's.  (5 wait states: what a window in
+// registers that the vector unit has just written takes; the compiler does not look for hazards in here.)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // (m0 is the compiler's, which has to know that it changes)
 typedef unsigned Window __attribute__((ext_vector_type(4)));
@@ -100,7 +101,7 @@ __device__ __forceinline__ Window make_window(const void* base, unsigned bytes) 
 }
 __device__ __forceinline__ void load_to_lds(Window w, unsigned offset, unsigned to) {
     const int at = __builtin_amdgcn_readfirstlane((int)to);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset), "s"(w)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset), "s"(w)
                  : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
     constexpr int RB = 128 * WK, ROWS = BM + BN, STAGE = ROWS * RB, RC = RB / 16;
     constexpr int RPI = 64 / RC, LPW = ROWS / RPI / NW, LW = BN / RPI / NW;  // rows a load instruction fills; a wave's per slice, W's of them
     constexpr int PER = 4 / WK, SLOTS = WK == 4 ? STAGES : 2;  // slices that share a load of scales, loads held
-    constexpr int SROWS = BM < 64 ? 64 : BM;
+    constexpr int SROWS = (BM + 63) / 64 * 64;
     constexpr int C = 4 * FN;  // neighbouring columns of Y a lane ends with
     static_assert(LPW * RPI * NW == ROWS && LW * RPI * NW == BN && NW * 64 >= SROWS && 128 % TN == 0, "slices split over the waves");
     static_assert(WK == 1 || (WK - 1) * BM * BN * 4 <= STAGES * STAGE, "the k groups' sums fit the ring");
@@ -199,7 +200,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
         for (int i = 0; i < (SAME ? 1 : LPW - LW); i++) xoff[i] = (wave * RPI + lane / RC) * (unsigned)a.ldx + 16u * chunk(LW + i);
     }
     [[maybe_unused]] auto offset = [&](int kt, int i) __attribute__((always_inline)) {
-        const unsigned step = (i < LW ? i * (unsigned)a.ldw : (i - LW) * (unsigned)a.ldx) * STEP + kt * RB;
+        unsigned step = (i < LW ? i * (unsigned)a.ldw : (i - LW) * (unsigned)a.ldx) * STEP + kt * RB;
+        if constexpr (!AHEAD) asm volatile("" : "+s"(step));  // (added where it is used: registers are few)
         return (i < LW ? woff[SAME ? 0 : i] : xoff[SAME ? 0 : i - LW]) + step;
     };
     [[maybe_unused]] const unsigned xsoff = (64 * wave + lane) * (unsigned)args.ldxs * 4u, wsoff = lane * (unsigned)args.ldws * 4u;
@@ -700,21 +702,22 @@ int launch_tiles(const LinearFp8Args& a, hipStream_t st, bool go) {
 }
 
 // The tiles a launch takes: of these, the one whose busiest CU is done first, by the microseconds of a tile (f + a a block of K) fitted to
-// all tiles' times at 110 sizes (16-bit outputs) and 80 (f32): M from 17 to 30 000, N from 64 to 7360, K from 128 to 3680.  The choice
-// loses 0.7 % (0.9 %) on the best of them on average; over 10 % at two sizes (one), 26 % at 225 x 2048 x 2048 (9.0 against 7.1 us).
-// Tiles that share a CU overlap where they wait (rounds count in parts).  E.g. in bf16 with 64 x 64 / 128 x 128 / 128 x 256 / 192 x 256 /
-// 256 x 256 tiles: 1500 x 1024 x 2816 12.4 / 19.5 / 24.3 / 32.0 / 39.6 us, 3000 x 5632 x 1024 45 / 38 / 31 / 30 / 40, 12000 x 1280 x 2816
-// 84 / 79 / 53 / 63 / 50, 24000 x 5632 x 1024 327 / 253 / 177 / 156 / 159, 8192^3 934 / 987 / 618 / 550 / 482.
+// all tiles' times at 110 sizes (16-bit outputs) and 90 (f32): M from 17 to 30 000, N from 64 to 7360, K from 128 to 3680.  On 50 (40)
+// others the choice loses 1.2 % (0.6 %) on the best of them on average, 17 % (13 %) at most.  Tiles that share a CU overlap where they
+// wait (rounds count in parts).  E.g. in bf16 with 64 x 64 / 96 x 64 / 128 x 128 / 128 x 256 / 192 x 256 / 256 x 256 tiles: 1500 x 1024 x 2816
+// 12.3 / 10.8 / 16.2 / 24.4 / 31.5 / 39 us, 12000 x 1280 x 2816 84 / - / 79 / 53 / 63 / 50, 24000 x 5632 x 1024 327 / - / 253 / 170 / 151 / 156,
+// 8192^3 934 / - / 987 / 612 / 533 / 483; into f32 with 64 x 64 / 96 x 64 / 64 x 128 / 128 x 128 1500 x 1024 x 2816 17.0 / 14.9 / 16.2 / 25.9.
 struct TileCost {
     int bm, bn;
     float f, a;
     int parts;
     float alone;
 };
-constexpr TileCost kTiles16[] = {{32, 32, 0.634f, 0.0974f, 4, 1.f},  {64, 64, 0.67f, 0.182f, 1, 1.08f},   {128, 128, 1.27f, 0.5475f, 1, 0.8f},
-                                 {128, 256, 1.02f, 1.007f, 1, 1.f},  {192, 256, 1.62f, 1.3445f, 1, 1.f}, {256, 256, 3.45f, 1.67f, 1, 1.f}};
-constexpr TileCost kTiles32[] = {{32, 32, 1.09f, 0.1005f, 4, 1.f}, {64, 64, 1.13f, 0.2566f, 1, 1.f}, {64, 128, 2.37f, 0.4985f, 1, 1.f},
-                                 {128, 128, 1.62f, 0.968f, 1, 1.f}};
+constexpr TileCost kTiles16[] = {{32, 32, 0.761f, 0.0915f, 4, 1.f},  {64, 64, 0.81f, 0.182f, 1, 1.08f},   {96, 64, 1.833f, 0.2393f, 1, 1.f},
+                                 {128, 128, 1.04f, 0.4946f, 1, 1.f}, {128, 256, 0.832f, 0.9837f, 1, 0.93f}, {192, 256, 1.41f, 1.2633f, 1, 1.f},
+                                 {256, 256, 2.939f, 1.7536f, 1, 1.f}};
+constexpr TileCost kTiles32[] = {{32, 32, 1.254f, 0.0789f, 4, 1.36f}, {64, 64, 1.197f, 0.2262f, 1, 1.f}, {96, 64, 1.466f, 0.4601f, 1, 1.f},
+                                 {64, 128, 1.883f, 0.4832f, 1, 1.f},  {128, 128, 1.171f, 0.9313f, 1, 1.f}};
 template <int N>
 int best_tiles(const TileCost (&t)[N], const LinearFp8Args& a) {
     constexpr int CUS = 256;
@@ -752,16 +755,18 @@ int launch_linear_fp8(const LinearFp8Args& a, hipStream_t st, bool go) {
         switch (best_tiles(kTiles32, a)) {
             case 0: return launch_tiles<TO, 32, 32, 1, 1, 4, 2, true, true, 2>(a, st, go);
             case 1: return launch_tiles<TO, 64, 64, 1, 2, 2, 2, true, true, 2>(a, st, go);
-            case 2: return launch_tiles<TO, 64, 128, 2, 2, 2, 2, true, true, 2>(a, st, go);
+            case 2: return launch_tiles<TO, 96, 64, 2, 2, 2, 2, true, true, 2>(a, st, go);
+            case 3: return launch_tiles<TO, 64, 128, 2, 2, 2, 2, true, true, 2>(a, st, go);
             default: return launch_tiles<TO, 128, 128, 4, 2, 1, 2, true, true, 2>(a, st, go);
         }
     } else {
         switch (best_tiles(kTiles16, a)) {
             case 0: return launch_tiles<TO, 32, 32, 1, 1, 4, 2, true, true, 2>(a, st, go);
             case 1: return launch_tiles<TO, 64, 64, 2, 2, 2, 2, true, true, 4>(a, st, go);
-            case 2: return launch_tiles<TO, 128, 128, 4, 2, 1, 2, true, true, 2>(a, st, go);
-            case 3: return launch_tiles<TO, 128, 256, 2, 4, 1, 2, true, false, 2>(a, st, go);
-            case 4: return launch_tiles<TO, 192, 256, 2, 4, 1, 2, true, false, 2>(a, st, go);
+            case 2: return launch_tiles<TO, 96, 64, 2, 2, 2, 3, true, true, 2>(a, st, go);
+            case 3: return launch_tiles<TO, 128, 128, 4, 2, 1, 3, true, true, 2>(a, st, go);
+            case 4: return launch_tiles<TO, 128, 256, 2, 4, 1, 2, true, false, 2>(a, st, go);
+            case 5: return launch_tiles<TO, 192, 256, 2, 4, 1, 2, true, false, 2>(a, st, go);
             default: return launch_tiles<TO, 256, 256, 2, 4, 1, 2, true, false, 2>(a, st, go);
         }
     }

@@ -535,6 +535,23 @@ def test_linear_fp8_edges_of_large_tiles(out, m, n, k, pad):
     assert (outside(flat, m, n, pad) == CANARY).all()
 
 
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(4090, 4090, 900), (9000, 2900, 388), (650, 2816, 520), (8191, 4092, 1100), (5100, 5632, 128), (6100, 5632, 132)])
+def test_linear_fp8_tiles_one_after_another(out, m, n, k):
+    """Workgroups that take several tiles, one load ahead of the products across them, with one block of K or an odd or even
+    number, whole and cut; inner tiles and edges; each part of the epilogue."""
+    ops = operands(m, n, k)
+    bias, gate, res = randn(3, n), randn(5, -(-m // 7), n), randn(4, m, n, dtype=out)
+    y = torch.full((m, n), CANARY, dtype=TYPE[out], device="cuda")
+    run_linear(*ops, y, out)
+    close(y, *linear_ref(*ops, out), "plain")
+    run_linear(*ops, y, out, "tanh", bias=bias)
+    close(y, *linear_ref(*ops, out, "tanh", bias), "bias")
+    ref = linear_ref(*ops, out, "none", None, gate, 7, res)
+    run_linear(*ops, res, out, gate=gate, gate_rows=7, residual=res)
+    close(res, *ref, "gated residual")
+
+
 @pytest.mark.parametrize("m", [5, 40, 300])
 def test_linear_fp8_broadcast_rows(m):
     # A stride of 0 repeats one row of x, of its scales and of the residual; shorter strides than k overlap.
