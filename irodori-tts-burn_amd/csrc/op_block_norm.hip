@@ -5,8 +5,13 @@
 //   N(v) = v / sqrt(mean(v^2) + eps)  or  (v - mean(v)) / sqrt(var(v) + eps)
 //
 // HBM-bound: a row is read once into registers (8 neighbouring elements a lane and chunk), its sums are formed
-// there, and it is written once; h is formed from the unrounded r.  Rows of up to 2048 take a wavefront, wider ones as many
-// wavefronts as it takes.
+// there, and it is written once; h is formed from the unrounded r.  Rows of up to 2048 take a wavefront (a reduction is then a
+// dozen VALU operations and no barrier), wider ones as many wavefronts as it takes.  The weights and the modulation come from L2 under
+// the reductions.
+//
+// Measured a call, host side included (floor at a large copy's 5.1 TB/s in brackets): 4 x 1280 bf16 7.5 us (the call; 5.3 of kernel),
+// 253 x 1280 f32 7.4 (the call; 4.7 of kernel), 1500 x 1024 with gate and modulation into codes 8.2 [3.3] (7.8 of kernel: 375 workgroups, two
+// chains of load, reduction and load), 24000 x 1280 around an f32 stream 74 [72].
 #include "common.hpp"
 #include "fp8_block.hpp"
 #include "op_util.hpp"

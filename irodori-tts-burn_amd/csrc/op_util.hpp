@@ -1,5 +1,5 @@
 // Host checks and device element helpers shared by the described operators (op_rope.hip,
-// op_linear.hip, op_cross_attention.hip).
+// op_linear.hip, op_cross_attention.hip, op_block_norm.hip, op_block_quantize.hip, op_linear_fp8.hip).
 #pragma once
 
 #include <algorithm>

@@ -588,6 +588,25 @@ def test_linear_fp8_specials_stay_in_their_rows(m, n):
     close(y[6, :n - 1], ref[6, :n - 1], tol[6, :n - 1])
 
 
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n", [(9, 300), (70, 300), (600, 1000), (1500, 1024), (6100, 2816), (24000, 1024)])
+def test_linear_fp8_specials_stay_in_their_rows_of_16_bits(out, m, n):
+    # (Of the last two a workgroup takes several tiles: none keeps anything of the one before it.)
+    k = 400
+    x, xs, w, ws = operands(m, n, k)
+    clean, y = (torch.empty(m, n, dtype=TYPE[out], device="cuda") for _ in range(2))
+    run_linear(x, xs, w, ws, clean, out)
+    bad = torch.zeros(m, n, dtype=torch.bool, device="cuda")
+    x[m - 2, 399], xs[4, 1], w[n - 1, 3] = 0x7f, math.inf, 0xff
+    bad[m - 2], bad[4], bad[:, n - 1] = True, True, True
+    for i in range(130, m - 2, 260):
+        x[i, i % k] = 0x7f
+        bad[i] = True
+    run_linear(x, xs, w, ws, y, out)
+    assert not torch.isfinite(y[bad]).any()
+    assert torch.equal(y[~bad], clean[~bad])
+
+
 @pytest.mark.parametrize("m", [4, 40, 300])
 def test_linear_fp8_rows_far_apart(m):
     # Rows of x, w, y and the scales some 2^27 bytes apart or more: offsets past 32 bits.
