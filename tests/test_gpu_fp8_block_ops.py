@@ -276,6 +276,16 @@ def test_block_norm_constant_rows():
         assert (n.h == 0).all(), v
 
 
+@pytest.mark.parametrize("dim", [2, 1024, 4096])
+def test_block_norm_constant_rows_whose_sum_passes_the_range(dim):
+    # (Sums of a power of two of powers of two are exact, so the differences are 0.)
+    for v in (2.0 ** 126, -(2.0 ** 127), 2.0 ** 127):
+        n = Norms(2, dim, "f32", norm="layer", has_branch=False, x_out=False)
+        n.x.fill_(v)
+        n()
+        assert (n.h == n.b).all(), v
+
+
 @pytest.mark.parametrize("dim", [256, 2304])
 def test_block_norm_specials_stay_in_their_row(dim):
     n = Norms(5, dim, "bf16", "f32", "fp8", branch="rms", norm="rms", affine=False)
