@@ -64,11 +64,14 @@ struct RowSum {
         return make_float2(a, b);
     }
 };
-constexpr int kSlots = 8;  // two norms, two sums each, each formed twice at most
+constexpr int kSlots = 12;  // two norms, three sums each, each formed twice at most
 
 // The norm of a row as v -> ((v pre - mean) - rest) r.  The mean is that of f32 sums and the rest what they missed: the mean
-// of the differences, which are exact where they are small.  Where the sums pass f32's range they are formed again from
-// values times 2^-80, of which no sum passes it.
+// of the differences, which are exact where they are small.  Where that rest is more than 1/64 of the differences, as in rows whose
+// spread is in their last bits, the variance E d^2 - rest^2 would be a difference of near numbers and the rest's own rounding as large as what it
+// leaves: the rest joins the mean, rounded, and the differences are formed again.  They are whole numbers of half steps of f32, their mean
+// at most half a step, so rest^2 <= variance; and all 0 where the row is a constant.  Where the sums pass f32's range they are
+// formed again from values times 2^-80, of which no sum passes it.
 struct Norm {
     float pre = 1.f, mean = 0.f, rest = 0.f, r = 1.f;
     __device__ __forceinline__ float operator()(float v) const {
@@ -92,20 +95,27 @@ __device__ __forceinline__ Norm norm_of(const float (&v)[CH][8], const int (&n)[
 #pragma unroll
                 for (int i = 0; i < 8; i++) s = fmaf(v[c][i], f.pre, s);
             f.mean = sum(s, 0.f).x * inv;
-            float d1 = 0.f, d2 = 0.f;
+            auto differences = [&]() __attribute__((always_inline)) {
+                float d1 = 0.f, d2 = 0.f;
 #pragma unroll
-            for (int c = 0; c < CH; c++)
+                for (int c = 0; c < CH; c++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float d = fmaf(v[c][i], f.pre, -f.mean);
-                    d = i < n[c] ? d : 0.f;
-                    d1 += d;
-                    d2 = fmaf(d, d, d2);
-                }
-            const float2 t = sum(d1, d2);
-            f.rest = t.x * inv;
-            square = fmaxf(t.y * inv - f.rest * f.rest, 0.f);
-            if (!(t.y < __builtin_inff())) square = t.y;
+                    for (int i = 0; i < 8; i++) {
+                        float d = fmaf(v[c][i], f.pre, -f.mean);
+                        d = i < n[c] ? d : 0.f;
+                        d1 += d;
+                        d2 = fmaf(d, d, d2);
+                    }
+                const float2 t = sum(d1, d2);
+                f.rest = t.x * inv;
+                return t.y;
+            };
+            float squares = differences();
+            if (__builtin_expect(f.rest != 0.f && squares < __builtin_inff() && f.rest * f.rest >= 0x1p-12f * (squares * inv), false)) {
+                f.mean += f.rest;
+                squares = differences();
+            }
+            square = squares < __builtin_inff() ? fmaxf(squares * inv - f.rest * f.rest, 0.f) : squares;
         } else {
             float s = 0.f;
 #pragma unroll

@@ -286,6 +286,45 @@ def test_block_norm_constant_rows_whose_sum_passes_the_range(dim):
         assert (n.h == n.b).all(), v
 
 
+@pytest.mark.parametrize("eps", [1e-5, 1e-30])
+@pytest.mark.parametrize("dim", [3, 250, 777, 1000, 2048, 2816, 5632, 16384])
+def test_block_norm_constant_rows_far_from_zero(dim, eps):
+    """Constants of any mantissa, a row each: their sums round, and yet the differences from the mean are all 0."""
+    g = torch.Generator().manual_seed(dim)
+    v = torch.exp(torch.empty(400).uniform_(math.log(1e-3), math.log(3e38), generator=g)) * (1 - 2 * torch.randint(0, 2, (400,), generator=g))
+    v[:6] = torch.tensor([9.90373153e14, 7.56785854e14, 8e11, 1e18, -3.3e9, 1.7e10])
+    for dtype in ("f32", "bf16"):
+        n = Norms(400, dim, dtype, norm="layer", has_branch=False, affine=False, x_out=False, eps=eps)
+        n.x.copy_(v[:, None].to(TYPE[dtype]).expand(-1, dim))
+        n()
+        assert (n.h == 0).all(), n.x[(n.h != 0).any(1), 0].tolist()[:8]
+    m = Norms(400, dim, "bf16", "f32", branch="layer", norm="none", affine=False, x_out=False, beps=eps)  # the branch's norm: r = x
+    m.x.zero_()
+    m.y.copy_(v[:, None].to(torch.bfloat16).expand(-1, dim))
+    m()
+    assert (m.h == 0).all()
+
+
+@pytest.mark.parametrize("dim", [3, 250, 1000, 2816, 16384])
+@pytest.mark.parametrize("few", [0.001, 0.2, 0.5])
+def test_block_norm_rows_within_a_few_steps_of_a_constant(dim, few):
+    """Rows of a constant and its f32 neighbours: all of the spread is in the last bits.
+
+    The differences from the rounded mean are whole numbers of half steps d, those of the mean at most half a step, so
+    that mean(d)^2 <= var: E d^2 <= 2 var and E |d| <= 1.5 s.  A sum has at most 48 roundings in a row, so mean(d) is off by 48 F 1.5 s = 72 F s;
+    the variance by 50 F E d^2 + 2 mean(d) 72 F s + 2 F var <= 246 F var, its root by half of that, and 3 F of quotient and product."""
+    g = torch.Generator().manual_seed(dim)
+    v = torch.exp(torch.empty(300, 1).uniform_(math.log(1e3), math.log(1e36), generator=g)) * (1 - 2 * torch.randint(0, 2, (300, 1), generator=g))
+    steps = torch.where(torch.rand(300, dim, generator=g) < few, torch.randint(-2, 3, (300, dim), generator=g), torch.zeros((), dtype=torch.long))
+    x = (v.view(torch.int32) + steps.int()).view(torch.float32).cuda()
+    n = Norms(300, dim, "f32", norm="layer", has_branch=False, affine=False, x_out=False, eps=1e-20)
+    n.x.copy_(x)
+    n()
+    away = x.double() - x.double()[:, :1]  # exact
+    y, _ = norm_ref(away, "layer", 1e-20, torch.zeros_like(away))
+    close(n.h, y, F * (126 * y.abs() + 72) + u("f32") * y.abs(), "steps")
+
+
 @pytest.mark.parametrize("dim", [256, 2304])
 def test_block_norm_specials_stay_in_their_row(dim):
     n = Norms(5, dim, "bf16", "f32", "fp8", branch="rms", norm="rms", affine=False)
