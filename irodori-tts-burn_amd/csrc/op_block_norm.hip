@@ -127,8 +127,8 @@ __device__ __forceinline__ Norm norm_of(const float (&v)[CH][8], const int (&n)[
                 }
             square = sum(s, 0.f).x * inv;
         }
-        const float under = square + eps * (f.pre * f.pre);
-        f.r = under == 0.f ? 0.f : 1.f / sqrtf(under);  // (eps 2^-160 is 0, and all of a row may be its mean)
+        const float under = square + eps * f.pre * f.pre;  // (2^-160 is no f32 number, a large eps times it is)
+        f.r = under == 0.f ? 0.f : 1.f / sqrtf(under);  // (a small one is 0, and all of a row may be its mean)
         if (square < __builtin_inff() || turn == 1) break;
         f.pre = 0x1p-80f;
     }

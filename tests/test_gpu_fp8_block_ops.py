@@ -325,6 +325,18 @@ def test_block_norm_rows_within_a_few_steps_of_a_constant(dim, few):
     close(n.h, y, F * (126 * y.abs() + 72) + u("f32") * y.abs(), "steps")
 
 
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("dim", [1000, 5632, 16384])
+def test_block_norm_keeps_a_large_eps_where_squares_pass_the_range(kind, dim):
+    # The least rows whose squares' sum is infinite in f32: there an eps of 1e30 is 5e-5 of the mean square at 16384 columns.
+    sign = 1 - 2 * (torch.arange(dim, device="cuda") % 2)
+    for factor in (1.01, 1.5, 30.0):
+        n = Norms(3, dim, "f32", norm=kind, has_branch=False, affine=False, x_out=False, eps=1e30)
+        n.x.copy_((sign * factor * math.sqrt(2.0 ** 128 / dim)).float().expand(3, -1))
+        n()
+        n.check("%s %g" % (kind, factor))
+
+
 @pytest.mark.parametrize("dim", [256, 2304])
 def test_block_norm_specials_stay_in_their_row(dim):
     n = Norms(5, dim, "bf16", "f32", "fp8", branch="rms", norm="rms", affine=False)
