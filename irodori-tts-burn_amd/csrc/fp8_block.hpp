@@ -40,14 +40,24 @@ __device__ __forceinline__ float finite_abs_max(const float (&v)[N]) {
 __device__ __forceinline__ float scale_of(float amax) { return fmaxf(__fdiv_rn(amax, 448.f), 1.1754943508222875e-38f); }
 
 // The codes of 8 values: the correctly rounded quotients v / s (the product with the rounded reciprocal, corrected once by
-// its exact remainder), rounded to nearest even by the converter.  An infinity's remainder is a NaN.
+// its exact remainder), rounded to nearest even by the converter.  An infinity's remainder is a NaN.  Remainders of quotients down to the least
+// midpoint, 2^-10, have bits down to 2^-56 s, which f32 holds from s = 2^-93 on: below 2^-64 values and scale are multiplied by 2^64 first,
+// which is exact.
 __device__ __forceinline__ uint2 codes8(const float (&v)[8], float s) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = v[i];
+    if (__builtin_expect(s < 0x1p-64f, false)) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] *= 0x1p64f;
+        s *= 0x1p64f;
+    }
     const float inv = __fdiv_rn(1.f, s);
     float q[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float q0 = v[i] * inv;
-        q[i] = fmaf(fmaf(-q0, s, v[i]), inv, q0);
+        const float q0 = x[i] * inv;
+        q[i] = fmaf(fmaf(-q0, s, x[i]), inv, q0);
     }
     return make_uint2(pack_e4m3(q[0], q[1], q[2], q[3]), pack_e4m3(q[4], q[5], q[6], q[7]));
 }

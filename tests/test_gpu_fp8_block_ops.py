@@ -409,6 +409,40 @@ def test_block_quantize_ties_and_limits():
         same_codes(q, rq)
 
 
+@pytest.mark.parametrize("factor", [1.2345 * 2.0 ** -126, 1.9 * 2.0 ** -126, 1.1 * 2.0 ** -125, 1.7 * 2.0 ** -122, 1.3 * 2.0 ** -112, 1.9 * 2.0 ** -104,
+                                    1.6 * 2.0 ** -95, 1.45 * 2.0 ** -93, 1.3 * 2.0 ** -65, 1.3 * 2.0 ** -64, 1.7 * 2.0 ** -63, 1.2 * 2.0 ** -20, 1.55, 1.3 * 2.0 ** 118])
+def test_block_quantize_next_to_midpoints(factor):
+    """Values at and a step beside the midpoints of two codes, under scales of any mantissa down to the least: rows quantized one by
+    one, tile by tile, and behind a norm that passes its rows on."""
+    codes = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    mids = ((codes[:-1] + codes[1:]) / 2).double()
+    g = torch.Generator().manual_seed(3)
+    rows = []
+    for i in range(300):
+        top = torch.tensor(448 * factor * (1 + 0.001 * i if factor < 2.0 ** 118 else 1), dtype=torch.float32)
+        s = (top / 448).double()
+        row = (mids * s).float()[torch.randperm(126, generator=g)]
+        step = torch.randint(-1, 2, (126,), generator=g, dtype=torch.int32)
+        row = (row.view(torch.int32) + step).view(torch.float32) * (1 - 2 * torch.randint(0, 2, (126,), generator=g))
+        rows.append(torch.cat([row, torch.zeros(1), top[None]]))
+    x = torch.stack(rows).cuda()
+    q, s = torch.zeros(300, 128, dtype=torch.uint8, device="cuda"), torch.empty(300, 1, device="cuda")
+    rq, rs = codes_ref(x)
+    run_quantize(x, 128, "f32", q, s)
+    assert torch.equal(s.cpu(), rs)
+    same_codes(q, rq)
+    q.zero_()
+    d = ih.BlockNormDesc(300, 128, dtype="f32", h_dtype="fp8", norm="none")
+    ih.ops.block_norm(d, ptr(x), d_h=ptr(q), d_h_scales=ptr(s), stream=stream())
+    assert torch.equal(s.cpu(), rs)
+    same_codes(q, rq)
+    for i in (0, 7, 299):  # (a tile has one scale)
+        t = x[i:i + 1].contiguous()
+        run_quantize(t, 128, "f32", q[i:i + 1], s[i:i + 1], block_rows=128)
+        assert torch.equal(s[i].cpu(), rs[i])
+        same_codes(q[i], rq[i])
+
+
 def test_block_quantize_largest_of_many_blocks():
     # The largest magnitude's quotient may round to above 448: its code is 448 all the same.
     x = randn(7, 4096, 128) * torch.exp(8 * randn(8, 4096, 1))
