@@ -638,6 +638,8 @@ int irodori_op_block_quantize(const irodori_block_quantize_desc* desc, const voi
  *   sum_b x_scales[m, b] w_scales[n / 128, b] sum_{k in block b} x[m, k] w[n, k])
  * with x [m, k] and w [n, k] e4m3 codes, b the blocks of 128 along k, x_scales [m, blocks] and w_scales [ceil(n / 128),
  * blocks]; the blocks' sums, the scales and everything after them in f32, rounded once to out_dtype (F32, BF16 or F16).
+ * Scales are any f32 numbers: their product may pass f32's range where its term does not; where it is less than 2^-126 the term is
+ * off by up to 2^-125.
  * Products of an F32 output are exact; for 16-bit outputs of more than 16 rows the matrix cores keep 13 bits below the
  * largest of each 8 neighbouring products (1.5e-5 of the sum, relative L2).  Codes are not looked at: NaN codes and
  * scales reach the outputs whose sums they are in, and no others.

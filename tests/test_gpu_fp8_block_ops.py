@@ -702,6 +702,41 @@ def test_linear_fp8_specials_stay_in_their_rows_of_16_bits(out, m, n):
     assert torch.equal(y[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 300), (9, 300, 700), (16, 130, 5000), (40, 70, 130), (70, 300, 1300), (130, 260, 384), (600, 1000, 400), (1500, 1024, 520),
+                                   (101, 333, 1001), (1100, 2050, 71), (6100, 2816, 260), (12000, 1280, 264), (9000, 2900, 388), (8191, 4092, 600)])
+def test_linear_fp8_scales_whose_product_leaves_the_range(out, m, n, k):
+    """Scales whose product is no normal f32 number though the term is one, in every third row between ordinary rows and rows of
+    zero scales, behind a gate and onto a residual as well.  A subnormal product is off by 2^-150, times a block's sum of at most 128 448^2 <
+    2^25; sums that are subnormal round to 2^-150, one a block."""
+    x, xs, w, ws = operands(m, n, k)
+    mant = lambda s: torch.where(s < 0, -1.0, 1.0) * (1 + (s.abs() * 4096) % 1)  # noqa: E731
+    power = lambda e: torch.tensor(2.0, dtype=torch.float64, device="cuda") ** e  # noqa: E731
+    gate, res = 1 + randn(5, -(-m // 7), n, std=0.1), randn(4, m, n, dtype=out)
+    for e_x, e_w in ((-70, -70), (-76, -76), (-100, -40), (-126, -15), (-149, 10), (64, 64), (66, 66), (126, 3), (20, 110)):
+        a, b, s = x, w, mant(xs)
+        s[0::3] = (s[0::3] * power(e_x)).float()
+        s[1::3] = (s[1::3] * power(-6)).float()
+        s[2::3] = 0.0
+        t = (mant(ws) * power(e_w)).float()
+        if e_x > 0:  # no more than 4 of the least products a block, and rows and columns of zeros of either sign
+            a = torch.where(torch.arange(k, device="cuda") % 37 == 3, x & 0x81, x & 0x80)
+            a[6::12] &= 0x80
+            b = w & 0x81
+            b[5::9] &= 0x80
+            b[n // 2:n // 2 + 128] &= 0x80
+        what = "2^%d 2^%d" % (e_x, e_w)
+        lost = blocks(k) * (2.0 ** -150 + (2.0 ** -125 if e_x < 0 else 0))
+        y = torch.full((m, n), CANARY, dtype=TYPE[out], device="cuda")
+        run_linear(a, s, b, t, y, out)
+        ref, tol = linear_ref(a, s, b, t, out)
+        close(y, ref, tol + lost, what)
+        y = res.clone()
+        ref, tol = linear_ref(a, s, b, t, out, "none", None, gate, 7, res)
+        run_linear(a, s, b, t, y, out, gate=gate, gate_rows=7, residual=y)
+        close(y, ref, tol + 2 * lost, what + " onto the residual")
+
+
 @pytest.mark.parametrize("m", [4, 40, 300])
 def test_linear_fp8_rows_far_apart(m):
     # Rows of x, w, y and the scales some 2^27 bytes apart or more: offsets past 32 bits.
