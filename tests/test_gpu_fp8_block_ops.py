@@ -737,6 +737,38 @@ def test_linear_fp8_scales_whose_product_leaves_the_range(out, m, n, k):
         close(y, ref, tol + 2 * lost, what + " onto the residual")
 
 
+@pytest.mark.parametrize("channels", [1.0, 16.0])
+@pytest.mark.parametrize("m,n,k", [(16, 300, 1000), (64, 64, 1000), (300, 520, 900), (253, 1280, 250), (113, 333, 1001), (1500, 1024, 1024), (6100, 2816, 400),
+                                   (24000, 1024, 250), (12000, 1280, 900)])
+def test_linear_fp8_bits_of_16_bit_outputs(m, n, k, channels):
+    """The products' own error, apart from the output's rounding: the residual takes the rounded result away, and what is left is rounded to
+    2^-11 of at most 2^-11 of it.  Of each 8 neighbouring products a part below 2^-13 of the largest one's power of two is lost, of a sign of its own;
+    where no bit lies there, nothing is; up to 16 rows nothing at all.  `channels`: every 16th column of x as many times the rest."""
+    wide = torch.where(torch.arange(k, device="cuda") % 16 == 5, channels, 1.0)
+    x, w = randn(1, m, k) * wide, randn(2, n, k, std=k ** -0.5)
+    xq, xs = torch.empty(m, k, dtype=torch.uint8, device="cuda"), torch.empty(m, blocks(k), device="cuda")
+    wq, ws = torch.empty(n, k, dtype=torch.uint8, device="cuda"), torch.empty(blocks(n), blocks(k), device="cuda")
+    run_quantize(x, k, "f32", xq, xs)
+    run_quantize(w, k, "f32", wq, ws, block_rows=128)
+    ref, _ = linear_ref(xq, xs, wq, ws, "f32")
+    y = -ref.to(torch.float16)
+    want = ref + y.double()
+    run_linear(xq, xs, wq, ws, y, "f16", residual=y)
+    rows, cols = torch.arange(0, m, -(-m // 64), device="cuda"), torch.arange(0, n, -(-n // 64), device="cuda")
+    err = (y.double() - want)[rows][:, cols]
+    lost = torch.zeros((), dtype=torch.float64, device="cuda")
+    for b in range(blocks(k) if m > 16 else 0):
+        part = lambda q: torch.nn.functional.pad(values(q[:, 128 * b:128 * b + 128]), (0, -(k - 128 * b) % 8 if b == blocks(k) - 1 else 0))  # noqa: E731
+        p = (part(xq[rows])[:, None] * part(wq[cols])[None]).unflatten(2, (-1, 8))
+        step = torch.exp2(torch.floor(torch.log2(p.abs().amax(3, keepdim=True).clamp(min=2.0 ** -20))) - 13)
+        f = xs[rows, b].double()[:, None] * ws[cols // 128, b].double()[None]
+        lost += ((torch.remainder(p.abs(), step) != 0) * step.square()).sum(dim=(2, 3)).mul(f.square()).sum()
+    # f32: as in linear_ref, most of it 2 F of the magnitudes in a row, roundings of independent signs.
+    size = ref[rows][:, cols].norm()
+    got = float(err.norm() / size)
+    assert got <= float(lost.sqrt() / size) + 2.0 ** -22 + 4 * F * math.sqrt(k / 8)
+
+
 @pytest.mark.parametrize("m", [4, 40, 300])
 def test_linear_fp8_rows_far_apart(m):
     # Rows of x, w, y and the scales some 2^27 bytes apart or more: offsets past 32 bits.
