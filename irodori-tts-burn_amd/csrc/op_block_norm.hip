@@ -301,11 +301,11 @@ int launch(const NormArgs& a, int fp8, hipStream_t st, bool go) {
     const int64_t threads = waves == 1 ? ((int64_t)a.rows + 3) / 4 * 256 : (int64_t)a.rows * waves * 64;
     if (threads > UINT32_MAX) return -1;
     if (!go) return 0;
-    const int per = waves == 1 ? 256 : waves * 64;
+    const int per = waves == 1 ? 256 : waves * 64;  // (rows of several wavefronts have 3 or 4 chunks)
     auto run = [&](auto ch) {
         constexpr int CH = decltype(ch)::value;
         if (waves == 1) block_norm_kernel<T, TS, CH, true><<<(unsigned)(threads / per), per, 0, st>>>(a, fp8);
-        else if constexpr (CH > 1) block_norm_kernel<T, TS, CH, false><<<(unsigned)(threads / per), per, 0, st>>>(a, fp8);
+        else if constexpr (CH > 2) block_norm_kernel<T, TS, CH, false><<<(unsigned)(threads / per), per, 0, st>>>(a, fp8);
     };
     switch (chunks) {
         case 1: run(std::integral_constant<int, 1>{}); break;
