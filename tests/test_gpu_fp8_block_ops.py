@@ -737,6 +737,25 @@ def test_linear_fp8_scales_whose_product_leaves_the_range(out, m, n, k):
         close(y, ref, tol + 2 * lost, what + " onto the residual")
 
 
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(9, 300, 700), (40, 70, 130), (70, 300, 1300), (600, 1000, 400), (1500, 1024, 520), (101, 333, 1001), (6100, 2816, 260),
+                                   (12000, 1280, 264), (9000, 2900, 388)])
+def test_linear_fp8_rows_beside_scales_out_of_range(out, m, n, k):
+    """Rows whose own scales are ordinary hold the same bits whatever their neighbours' are, everything after the product with them."""
+    x, xs, w, ws = operands(m, n, k)
+    xs, ws = xs * 2.0 ** -60, ws * 2.0 ** 60
+    bias, gate, res = randn(3, n), randn(5, -(-m // 7), n), randn(4, m, n, dtype=out)
+    clean, y = (torch.empty(m, n, dtype=TYPE[out], device="cuda") for _ in range(2))
+    for act in ("none", "silu"):
+        for kw in (dict(), dict(bias=bias, gate=gate, gate_rows=7, residual=res)):
+            run_linear(x, xs, w, ws, clean, out, act, **kw)
+            far = xs.clone()
+            far[1::3, 0] = 2.0 ** 110
+            run_linear(x, far, w, ws, y, out, act, **kw)
+            for i in (0, 2):
+                assert torch.equal(y[i::3], clean[i::3]), (act, len(kw), i)
+
+
 @pytest.mark.parametrize("channels", [1.0, 16.0])
 @pytest.mark.parametrize("m,n,k", [(16, 300, 1000), (64, 64, 1000), (300, 520, 900), (253, 1280, 250), (113, 333, 1001), (1500, 1024, 1024), (6100, 2816, 400),
                                    (24000, 1024, 250), (12000, 1280, 900)])
