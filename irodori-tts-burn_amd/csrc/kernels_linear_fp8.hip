@@ -13,12 +13,12 @@
 //
 // Large tiles (128 x 256 and up, 16-bit outputs) are taken one after another by a workgroup a CU, whose loads run a slice ahead of its
 // products across them.  Measured a call, host side included (the operator's floor at the library's 2489 TFLOP/s, or a copy's 5.1 TB/s):
-//   4 x 7360 x 1280                      7.2 us [1.9]   the call; W at 1.9 TB/s in 4.9 us of kernel
+//   4 x 7360 x 1280                      7.2 us [1.9]   the call; W at 1.8 TB/s in 5.1 us of kernel
 //   253 x 1280 x 1000 f16, gelu          7.6 [0.4]      the call; a chain of two slices and the epilogue
 //   1500 x 1024 x 2816 -> f32, gate, residual  16.4 [3.8]  bf16 products (7.4 at the library's rate): 11 slices a tile of which the codes'
 //                                        widening takes as many cycles as the products
-//   24000 x 5632 x 1024                  148-158 [111]  126 us without the epilogue, its stores 20-28 (53 at a copy's rate, the rest under
-//                                        products); 8192^3 takes 482 where the library's product without blocks' scales takes 442
+//   24000 x 5632 x 1024                  152-160 [111]  by machine; on one 148, and 126 without the epilogue: its stores 22 (53 at a copy's rate, the
+//                                        rest under products); 8192^3 takes 482-513 where the library's product without blocks' scales takes 442
 #include <type_traits>
 
 #include "attn_util.hpp"
@@ -734,6 +734,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) __attribute__((amdgpu_waves_per_
                     for (int e = 0; e < C; e++) v[e] = acc[j][e / 4][e % 4];
                     finish_block<TO, false>(a, tile.m0 + wm * TM + 16 * j + fr, tile.n0 + wn * TN + C * fg, lane, v);
                 }
+            // Behind an epilogue past the L2s: 6000 x 1024 x 2816 with gate and residual 30.4 against 34.3 us, 3000 x 2816 x 1024 22.9 against 23.9,
+            // 24000 x 1024 x 2816 96.2 against 97.1.
             } else if (!plain) {
                 finish_inner(std::false_type{}, std::true_type{});
             // A Y that the L2s (32 MB) do not hold goes past them: 24000 x 5632 x 1024 154 against 163 us, x 512 92 against 103.
@@ -929,7 +931,7 @@ int launch_linear_fp8(const LinearFp8Args& a, hipStream_t st, bool go) {
                        l.ldw <= FAR && l.K <= FAR && a.ldxs * 4 <= FAR && a.ldws * 4 <= FAR && l.ldy <= FAR && l.ldr <= FAR;
     if (!async) {
         // Through registers: 64 x 64 against 128 x 128 tiles 11.3 / 15.4 us at 500 x 1024 x 1001 (128 tiles of 64), 33.7 / 16.1 at 1536 x 2048
-        // (768), 1115 / 422 at 20000 x 5632: the smaller ones while they all run at once.
+        // (768), 1115 / 422 at 20000 x 5632 (159 where K is 1000): the smaller ones while they all run at once.
         if (((int64_t)l.M + 63) / 64 * ((l.N + 63) / 64) <= 256) return launch_tiles<TO, 64, 64, 2, 2, 2, 2, false, true, 2>(a, st, go);
         return launch_tiles<TO, 128, 128, 4, 2, 1, 2, false, true, 2>(a, st, go);
     }

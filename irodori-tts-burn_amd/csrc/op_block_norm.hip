@@ -9,9 +9,12 @@
 // dozen VALU operations and no barrier), wider ones as many wavefronts as it takes.  The weights and the modulation come from L2 under
 // the reductions.
 //
-// Measured a call, host side included (floor at a large copy's 5.1 TB/s in brackets): 4 x 1280 bf16 7.5 us (the call; 5.3 of kernel),
-// 253 x 1280 f32 7.4 (the call; 4.7 of kernel), 1500 x 1024 with gate and modulation into codes 8.2 [3.3] (7.8 of kernel: 375 workgroups, two
-// chains of load, reduction and load), 24000 x 1280 around an f32 stream 74 [72].
+// Measured a call, host side included (floor at a large copy's 5.1 TB/s in brackets): 4 x 1280 bf16 7.5 us (the call; 5.2 of kernel),
+// 253 x 1280 f32 7.5 (the call; 4.9 of kernel), 1500 x 1024 with gate and modulation into codes 8.2 [3.3] (8.1 of kernel: 375 workgroups, two
+// chains of load, reduction and load, of which the second's loads could go out with the first's), 24000 x 1280 around an f32 stream 75 [72].
+// Other widths, 24000 rows of bf16 around an f32 stream with gate and modulation: 64 16.8 [3.6] and 333 37.7 [18.8] (most lanes idle),
+// 1024 68 [58], 2048 135 [116], 2816 190 [159], 3680 240 [208], 5632 440 [318] (4 chunks a lane: two wavefronts a SIMD, and with several wavefronts a row
+// 36 bytes of scratch a lane); 6000 x 16384 327 [231].
 #include "common.hpp"
 #include "fp8_block.hpp"
 #include "op_util.hpp"

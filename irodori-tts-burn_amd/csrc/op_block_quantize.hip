@@ -5,7 +5,7 @@
 // over a row of lanes, and the codes leave as 128 neighbouring bytes; four blocks' loads are on their way at once.
 //
 // Measured a call, host side included (floor at a large copy's 5.1 TB/s in brackets): silu(a) b of 8 x 2816 bf16 7.3 us (the call; 4.9 of
-// kernel), of 24000 x 2816 64 [67: a copy writes half of its bytes, this a fifth], a 5632 x 1024 f32 weight 8.3 [5.6] (352 workgroups: latency).
+// kernel), of 24000 x 2816 64 [67: a copy writes half of its bytes, this a fifth], a 5632 x 1024 f32 weight 8.4 [5.6] (352 workgroups: latency).
 #include "common.hpp"
 #include "fp8_block.hpp"
 #include "linear_tile.hpp"
